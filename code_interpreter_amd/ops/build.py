@@ -57,6 +57,9 @@ def _compile(output: Path, sources, verbose: bool) -> None:
         hipcc,
         f"--offload-arch={ARCH}",
         "-O3",
+        # packed fp32 arithmetic, which the compiler makes of ordinary float
+        # code, has given wrong results in some of its forms
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-std=c++17",
         "-fPIC",
         "-shared",
