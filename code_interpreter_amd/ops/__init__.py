@@ -1,8 +1,9 @@
 """gfx950 HIP kernel library + numpy routing.
 
 ``_hipops`` (C extension, built in-tree by ops/build.py) provides the raw
-device API; ``hipnp`` provides DeviceArray and the numpy patches. Both are
-import-path-flat so sandbox children can load them standalone via
+device API; ``hipnp`` provides DeviceArray and the numpy patches; ``hipmx``
+and ``hiplm`` provide microscaled 4-bit products and the scoring of logits
+for torch tensors (kernels: ``_hiplm``). All are import-path-flat so sandbox children can load them standalone via
 APP_OPS_DIR without pulling in the control plane.
 """
 
@@ -30,3 +31,15 @@ def load_hipnp():
     import hipnp
 
     return hipnp
+
+
+def load_hipmx():
+    import hipmx
+
+    return hipmx
+
+
+def load_hiplm():
+    import hiplm
+
+    return hiplm

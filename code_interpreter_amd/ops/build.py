@@ -1,4 +1,4 @@
-"""In-tree build of the _hipops extension for gfx950.
+"""In-tree build of the gfx950 extensions (_hipops, _hipgemm, _hiplm).
 
 hipcc cross-compiles without a GPU, and the resulting .so lives next to
 this file (in-tree, so it travels to GPU boxes with the repo snapshot).
@@ -35,6 +35,20 @@ SOURCES = [
 GEMM_OUTPUT = OPS_DIR / "_hipgemm.so"
 GEMM_MODULE_SOURCES = [HIP_DIR / "hipgemm.cpp", *GEMM_SOURCES]
 
+# _hiplm: the language-model kernels, for torch tensors too.
+LM_OUTPUT = OPS_DIR / "_hiplm.so"
+LM_MODULE_SOURCES = [
+    HIP_DIR / "hiplm.cpp",
+    HIP_DIR / "mxfp4_quant.hip",
+    HIP_DIR / "mxfp4_gemm.hip",
+    HIP_DIR / "scoring.hip",
+]
+MODULES = [
+    (OUTPUT, SOURCES),
+    (GEMM_OUTPUT, GEMM_MODULE_SOURCES),
+    (LM_OUTPUT, LM_MODULE_SOURCES),
+]
+
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
 
@@ -42,12 +56,12 @@ def _needs(output: Path, sources) -> bool:
     if not output.exists():
         return True
     out_mtime = output.stat().st_mtime
-    deps = list(sources) + [HIP_DIR / "common.h", Path(__file__)]
+    deps = [*sources, *HIP_DIR.glob("*.h"), Path(__file__)]
     return any(p.stat().st_mtime > out_mtime for p in deps)
 
 
 def needs_build() -> bool:
-    return _needs(OUTPUT, SOURCES) or _needs(GEMM_OUTPUT, GEMM_MODULE_SOURCES)
+    return any(_needs(out, sources) for out, sources in MODULES)
 
 
 def _compile(output: Path, sources, verbose: bool) -> None:
@@ -76,10 +90,9 @@ def _compile(output: Path, sources, verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = True) -> Path:
-    if force or _needs(OUTPUT, SOURCES):
-        _compile(OUTPUT, SOURCES, verbose)
-    if force or _needs(GEMM_OUTPUT, GEMM_MODULE_SOURCES):
-        _compile(GEMM_OUTPUT, GEMM_MODULE_SOURCES, verbose)
+    for out, sources in MODULES:
+        if force or _needs(out, sources):
+            _compile(out, sources, verbose)
     return OUTPUT
 
 

@@ -1,0 +1,924 @@
+// Rows of logits: log probabilities of given tokens, entropies, the most
+// likely alternatives, and distillation from recorded teacher logits, with
+// their backward passes.
+//
+// Mathematics. With c = log2(e) / T, m = max x, e_j = 2^(c (x_j - m)):
+//   S = sum e_j, U = sum e_j c (x_j - m)
+//   ln p_j = (x_j - m) / T - ln S,  H = ln S - ln 2 * U / S
+// A thread keeps (m, S, U) of what it has seen; a new maximum m' scales
+//   S by r = 2^(c (m - m')), and U becomes r (U + S c (m - m'))
+// which also joins two threads', waves' or blocks' triples. So a row is
+// read once. The difference x - m is taken before the product with c: of a
+// mask of the type's lowest value, c x alone would be an infinity.
+//
+// An element of -inf has no share: e is 0, and the exponent that U takes is
+// held at kLow, since 0 * -inf is no number. A row with nothing but -inf
+// has m = -inf and S = 0 and is reported as empty. A NaN or +inf makes S
+// NaN, and with it all of the row's numbers.
+//
+// All sums are 32-bit, over a fixed split of the row and in a fixed order:
+// the same input gives the same bits.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "lm.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLow = -16384.f;  // 2^kLow is 0
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+// 16 bytes at any element's address: the hardware takes vector loads and
+// stores at 2-byte alignment, so rows of odd length need no path of their own
+using raw16 = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+
+template <LmType T>
+struct Elem;
+template <>
+struct Elem<LmType::F32> {
+  using type = float;
+  static constexpr int kVec = 4;
+  static constexpr uint32_t kNegInf = 0xFF800000u;  // in every lane of a word
+  static __device__ float get(const u32x4& w, int i) {
+    return __uint_as_float(w[i]);
+  }
+  static __device__ void put(u32x4& w, int i, uint32_t bits) { w[i] = bits; }
+  static __device__ float load(const type* p) { return *p; }
+  static __device__ uint32_t bits(const type* p) { return __float_as_uint(*p); }
+  static __device__ void store(type* p, float f) { *p = f; }
+};
+template <>
+struct Elem<LmType::BF16> {
+  using type = uint16_t;
+  static constexpr int kVec = 8;
+  static constexpr uint32_t kNegInf = 0xFF80FF80u;
+  static __device__ float get(const u32x4& w, int i) {
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+  }
+  static __device__ void put(u32x4& w, int i, uint32_t b) {
+    w[i >> 1] = i & 1 ? (w[i >> 1] & 0xFFFFu) | b << 16
+                      : (w[i >> 1] & 0xFFFF0000u) | b;
+  }
+  static __device__ float load(const type* p) {
+    return __uint_as_float((uint32_t)*p << 16);
+  }
+  static __device__ uint32_t bits(const type* p) { return *p; }
+  static __device__ void store(type* p, float f) {
+    __bf16 h = (__bf16)f;
+    __builtin_memcpy(p, &h, 2);
+  }
+};
+template <>
+struct Elem<LmType::F16> {
+  using type = uint16_t;
+  static constexpr int kVec = 8;
+  static constexpr uint32_t kNegInf = 0xFC00FC00u;
+  static __device__ float half(uint32_t b) {
+    uint16_t u = (uint16_t)b;
+    _Float16 h;
+    __builtin_memcpy(&h, &u, 2);
+    return (float)h;
+  }
+  static __device__ float get(const u32x4& w, int i) {
+    return half(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
+  }
+  static __device__ void put(u32x4& w, int i, uint32_t b) {
+    Elem<LmType::BF16>::put(w, i, b);
+  }
+  static __device__ float load(const type* p) { return half(*p); }
+  static __device__ uint32_t bits(const type* p) { return *p; }
+  static __device__ void store(type* p, float f) {
+    _Float16 h = (_Float16)f;
+    __builtin_memcpy(p, &h, 2);
+  }
+};
+
+// f32 values rounded to the type, into a 16-byte word
+template <LmType T>
+__device__ u32x4 pack(const float* f) {
+  u32x4 w;
+  if constexpr (T == LmType::F32) {
+    for (int i = 0; i < 4; i++) w[i] = __float_as_uint(f[i]);
+  } else if constexpr (T == LmType::BF16) {
+    using b2 = __bf16 __attribute__((ext_vector_type(2)));
+    using f2 = float __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      b2 h = __builtin_convertvector((f2{f[2 * i], f[2 * i + 1]}), b2);
+      uint32_t u;
+      __builtin_memcpy(&u, &h, 4);
+      w[i] = u;
+    }
+  } else {
+    using h2 = _Float16 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      h2 h = {(_Float16)f[2 * i], (_Float16)f[2 * i + 1]};
+      uint32_t u;
+      __builtin_memcpy(&u, &h, 4);
+      w[i] = u;
+    }
+  }
+  return w;
+}
+
+// elements [at, at + kVec) of a row of `end` elements; -inf behind its end
+template <LmType T>
+__device__ u32x4 load_vec(const typename Elem<T>::type* row, int64_t at,
+                          int64_t end) {
+  using E = Elem<T>;
+  if (at + E::kVec <= end) return *(const raw16*)(row + at);
+  u32x4 w = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+#pragma unroll
+  for (int i = 0; i < E::kVec; i++)
+    if (at + i < end) E::put(w, i, E::bits(row + at + i));
+  return w;
+}
+
+__device__ __forceinline__ float exp2_raw(float x) {
+  return __builtin_amdgcn_exp2f(x);
+}
+
+struct Triple {
+  float m, s, u;
+};
+
+__device__ __forceinline__ float or_zero(float m) {
+  return m == -INFINITY ? 0.f : m;
+}
+
+// a's sums under the maximum m >= a.m
+__device__ __forceinline__ Triple under(Triple a, float m, float c) {
+  float y = (a.m - or_zero(m)) * c;
+  float r = exp2_raw(y);
+  return {m, a.s * r, (a.u + a.s * fmaxf(y, kLow)) * r};
+}
+
+__device__ __forceinline__ Triple join(Triple a, Triple b, float c) {
+  float m = fmaxf(a.m, b.m);
+  Triple x = under(a, m, c), y = under(b, m, c);
+  return {m, x.s + y.s, x.u + y.u};
+}
+
+__device__ Triple join_wave(Triple a, float c) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1)
+    a = join(a, {__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.u, d)},
+             c);
+  return a;
+}
+
+// order-preserving bits of a value above, the complement of its index
+// below: a larger key is a better alternative, of equal values the earlier.
+// 0 stands for none. Both zeros are one value.
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t index) {
+  uint32_t b = __float_as_uint(x + 0.f);
+  b = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (uint64_t)b << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  uint32_t b = (uint32_t)(key >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) {
+  return ~(uint32_t)key;
+}
+
+// ---------------------------------------------------------------------------
+// alternatives
+// ---------------------------------------------------------------------------
+constexpr int kCap = 2048;  // candidates that are ranked at a time
+
+struct TopShared {
+  uint64_t keys[kCap];   // the best so far, then candidates
+  uint64_t best[kMaxTop];
+  uint64_t wave_key[kWaves];
+  float thread_max[kThreads];
+  float least;           // candidates are larger than this
+  int have;              // entries of the best so far
+  int count;             // entries of keys
+};
+
+// keys[0 .. n) -> the k best, sorted, at keys[0 ..), by counting for each
+// key how many are larger: keys are all different
+__device__ void rank_keys(TopShared& sh, int n, int k) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    uint64_t key = sh.keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += sh.keys[j] > key;
+    if (rank < k) sh.best[rank] = key;
+  }
+  __syncthreads();
+  int have = min(n, k);
+  for (int i = threadIdx.x; i < have; i += kThreads) sh.keys[i] = sh.best[i];
+  if (threadIdx.x == 0) {
+    sh.have = sh.count = have;
+    if (have == k) sh.least = key_value(sh.best[k - 1]);
+  }
+  __syncthreads();
+}
+
+// Takes the candidates of a chunk that the block holds in registers: words
+// w[0 .. U) of each thread, thread t's word i at element base + (i * 256 +
+// t) * kVec. Chunks come in the order of their indexes, so that an element
+// must be larger than the last of the k best so far to displace it.
+//
+// The k-th largest of the threads' own maxima is a lower bound of the
+// chunk's k-th largest element. At most k - 1 threads hold larger elements
+// than it, so few pass it but where many are equal. Where the candidates
+// still do not fit, the k best are taken one by one.
+template <LmType T, int U>
+__device__ void take_candidates(TopShared& sh, const u32x4* w, int64_t base,
+                                float thread_max, int k) {
+  using E = Elem<T>;
+  const int tid = threadIdx.x;
+  float least = sh.least;
+  auto append = [&](float floor_) {
+    if (thread_max > least && thread_max >= floor_) {
+#pragma unroll
+      for (int i = 0; i < U; i++)
+#pragma unroll
+        for (int j = 0; j < E::kVec; j++) {
+          float x = E::get(w[i], j);
+          if (x > least && x >= floor_) {
+            int at = atomicAdd(&sh.count, 1);
+            if (at < kCap)
+              sh.keys[at] = make_key(
+                  x, (uint32_t)(base + (i * kThreads + tid) * E::kVec + j));
+          }
+        }
+    }
+    __syncthreads();
+    int n = sh.count;
+    __syncthreads();
+    if (n > kCap && tid == 0) sh.count = sh.have;
+    return n;
+  };
+  int n = kCap + 1;
+  if (sh.have == k) n = append(-INFINITY);
+  if (n > kCap) {
+    sh.thread_max[tid] = thread_max;
+    __syncthreads();
+    // of equal maxima the threads' order decides: one thread has rank k - 1
+    int rank = 0;
+    for (int j = 0; j < kThreads; j++) {
+      float o = sh.thread_max[j];
+      rank += o > thread_max || (o == thread_max && j < tid);
+    }
+    __syncthreads();
+    if (rank == k - 1) sh.thread_max[0] = thread_max;
+    __syncthreads();
+    n = append(sh.thread_max[0]);
+  }
+  if (n > kCap) {
+    __syncthreads();  // sh.count is back at sh.have
+    uint64_t last = ~0ull;
+    for (int r = 0; r < k; r++) {
+      uint64_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < U; i++)
+#pragma unroll
+        for (int j = 0; j < E::kVec; j++) {
+          float x = E::get(w[i], j);
+          uint64_t key = make_key(
+              x, (uint32_t)(base + (i * kThreads + tid) * E::kVec + j));
+          if (x > least && key < last && key > mine) mine = key;
+        }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) {
+        uint64_t o = __shfl_xor((unsigned long long)mine, d);
+        mine = o > mine ? o : mine;
+      }
+      if ((tid & 63) == 0) sh.wave_key[tid >> 6] = mine;
+      __syncthreads();
+      uint64_t best = 0;
+      for (int j = 0; j < kWaves; j++)
+        best = sh.wave_key[j] > best ? sh.wave_key[j] : best;
+      __syncthreads();
+      if (!best) break;
+      if (tid == 0) sh.keys[sh.count++] = best;
+      last = best;
+    }
+    __syncthreads();
+    n = sh.count;
+  }
+  rank_keys(sh, n, k);
+}
+
+// ---------------------------------------------------------------------------
+// one pass over a row, or over one of `splits` parts of it
+// ---------------------------------------------------------------------------
+struct Part {
+  Triple t;
+  float pad;
+};
+
+template <LmType T, int U, bool kEntropy, bool kTop>
+__global__ __launch_bounds__(kThreads) void score_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
+    int splits, int64_t part_len, float c, int k, Part* __restrict__ parts,
+    uint64_t* __restrict__ part_keys) {
+  using E = Elem<T>;
+  constexpr int kChunk = kThreads * E::kVec * U;
+  __shared__ typename std::conditional<kTop, TopShared, int>::type sh;
+  __shared__ Triple wave_t[kWaves];
+
+  const int64_t row = blockIdx.x / (unsigned)splits;
+  const int64_t begin = (blockIdx.x % (unsigned)splits) * part_len;
+  const int64_t end = min(v, begin + part_len);
+  const typename E::type* src = x + row * stride;
+  const int tid = threadIdx.x;
+
+  if constexpr (kTop) {
+    if (tid == 0) {
+      sh.have = sh.count = 0;
+      sh.least = -INFINITY;
+    }
+    __syncthreads();
+  }
+
+  Triple t = {-INFINITY, 0.f, 0.f};
+  u32x4 next[U];
+#pragma unroll
+  for (int i = 0; i < U; i++)
+    next[i] = load_vec<T>(src, begin + (int64_t)(i * kThreads + tid) * E::kVec,
+                          end);
+  for (int64_t base = begin; base < end; base += kChunk) {
+    u32x4 w[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) w[i] = next[i];
+    if (base + kChunk < end) {
+#pragma unroll
+      for (int i = 0; i < U; i++)
+        next[i] = load_vec<T>(
+            src, base + kChunk + (int64_t)(i * kThreads + tid) * E::kVec, end);
+    }
+    float chunk_max = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++)
+        chunk_max = fmaxf(chunk_max, E::get(w[i], j));
+    if (chunk_max > t.m) t = under(t, chunk_max, c);
+    const float m = or_zero(t.m);
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++) {
+        float y = (E::get(w[i], j) - m) * c;
+        float e = exp2_raw(y);
+        s += e;
+        if constexpr (kEntropy) u = fmaf(e, fmaxf(y, kLow), u);
+      }
+    t.s += s;
+    t.u += u;
+    if constexpr (kTop) {
+      if (__syncthreads_or(chunk_max > sh.least))
+        take_candidates<T, U>(sh, w, base, chunk_max, k);
+    }
+  }
+
+  t = join_wave(t, c);
+  if ((tid & 63) == 0) wave_t[tid >> 6] = t;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kWaves; i++) t = join(t, wave_t[i], c);
+    parts[blockIdx.x].t = t;
+  }
+  if constexpr (kTop) {
+    for (int i = tid; i < k; i += kThreads)
+      part_keys[(int64_t)blockIdx.x * k + i] = i < sh.have ? sh.keys[i] : 0;
+  }
+}
+
+// the parts of a row, by one wave
+__device__ Triple join_parts(const Part* parts, int splits, float c) {
+  Triple t = {-INFINITY, 0.f, 0.f};
+  for (int i = threadIdx.x & 63; i < splits; i += 64)
+    t = join(t, parts[i].t, c);
+  return join_wave(t, c);
+}
+
+// ---------------------------------------------------------------------------
+// token log probabilities
+// ---------------------------------------------------------------------------
+// a wave a row: what needs no alternatives
+template <LmType T>
+__global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride,
+    int64_t rows, int64_t v, const int64_t* __restrict__ tokens,
+    int64_t ignore, float inv_t, float c, const Part* __restrict__ parts,
+    int splits, float* __restrict__ logprobs, float* __restrict__ entropy,
+    RowStats* __restrict__ stats) {
+  int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  Triple t = join_parts(parts + row * splits, splits, c);
+  if (threadIdx.x & 63) return;
+  int64_t token = tokens[row];
+  bool ignored = token == ignore;
+  bool outside = !ignored && (token < 0 || token >= v);
+  bool empty = t.m == -INFINITY && t.s == 0.f;
+  float log2_sum = log2f(t.s);
+  float lp, h;
+  if (ignored) {
+    lp = h = 0.f;
+  } else if (outside) {
+    lp = h = NAN;
+  } else if (empty) {
+    lp = -INFINITY;
+    h = 0.f;
+  } else {
+    float xt = Elem<T>::load(x + row * stride + token);
+    lp = (xt - t.m) * inv_t - log2_sum * kLn2;
+    h = (log2_sum - t.u / t.s) * kLn2;
+    if (!(t.s == t.s)) lp = NAN;
+  }
+  logprobs[row] = lp;
+  entropy[row] = h;
+  if (stats)
+    stats[row] = {outside ? NAN : t.m, log2_sum, h,
+                  ignored || (empty && !outside) ? 0.f : 1.f};
+}
+
+// a block a row: joins the parts' sorted lists of alternatives.
+// Of `splits` lists each element in place ceil(k / splits) or before: there
+// are k of them, so the least of these places' keys is a lower bound of the
+// k-th best; so is any list's own k-th. What passes both is ranked.
+__global__ __launch_bounds__(kThreads) void top_rows_kernel(
+    const uint64_t* __restrict__ part_keys, const Part* __restrict__ parts,
+    int splits, int k, const int64_t* __restrict__ tokens, int64_t ignore,
+    float inv_t, float c, float* __restrict__ top_lp,
+    int64_t* __restrict__ top_ids) {
+  extern __shared__ uint64_t keys[];  // splits * k
+  __shared__ uint64_t best[kMaxTop];
+  __shared__ unsigned long long bound_all, bound_any;
+  __shared__ int count;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const uint64_t* src = part_keys + row * splits * k;
+  if (tid == 0) {
+    bound_all = ~0ull;
+    bound_any = 0;
+    count = 0;
+  }
+  if (tid < k) best[tid] = 0;
+  __syncthreads();
+  const int place = (k + splits - 1) / splits - 1;
+  for (int i = tid; i < splits; i += kThreads) {
+    atomicMin(&bound_all, (unsigned long long)src[(int64_t)i * k + place]);
+    atomicMax(&bound_any, (unsigned long long)src[(int64_t)i * k + k - 1]);
+  }
+  __syncthreads();
+  uint64_t bound = bound_all > bound_any ? bound_all : bound_any;
+  if (!bound) bound = 1;  // none is no alternative
+  for (int i = tid; i < splits * k; i += kThreads) {
+    uint64_t key = src[i];
+    if (key >= bound) keys[atomicAdd(&count, 1)] = key;
+  }
+  __syncthreads();
+  const int n = count;
+  for (int i = tid; i < n; i += kThreads) {
+    uint64_t key = keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += keys[j] > key;
+    if (rank < k) best[rank] = key;
+  }
+  __syncthreads();
+  Triple t = join_parts(parts + row * splits, splits, c);
+  const float log_sum = log2f(t.s) * kLn2;
+  const bool ignored = tokens[row] == ignore;
+  for (int i = tid; i < k; i += kThreads) {
+    uint64_t key = ignored ? 0 : best[i];
+    top_lp[row * k + i] =
+        key ? (key_value(key) - t.m) * inv_t - log_sum : -INFINITY;
+    top_ids[row * k + i] = key ? (int64_t)key_index(key) : -1;
+  }
+}
+
+// dx_j = -p_j (a + b ln p_j) at every j, and g_lp / T more at the token,
+// with a = (g_lp + g_H H) / T, b = g_H / T
+template <LmType T, int U>
+__global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
+    int chunks, const int64_t* __restrict__ tokens, float inv_t, float c,
+    const RowStats* __restrict__ stats, const float* __restrict__ g_lp,
+    const float* __restrict__ g_h, typename Elem<T>::type* __restrict__ dx) {
+  using E = Elem<T>;
+  const int64_t row = blockIdx.x / (unsigned)chunks;
+  const int64_t base =
+      (int64_t)(blockIdx.x % (unsigned)chunks) * (kThreads * E::kVec * U);
+  const RowStats st = stats[row];
+  const float g = g_lp ? g_lp[row] : 0.f, gh = g_h ? g_h[row] : 0.f;
+  const float a = (g + gh * st.entropy) * inv_t, b = gh * inv_t * kLn2;
+  const bool live = st.live != 0.f;
+  const int64_t token = live ? tokens[row] : -1;
+  const typename E::type* src = x + row * stride;
+  typename E::type* dst = dx + row * v;
+  u32x4 w[U];
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      w[i] = load_vec<T>(
+          src, base + (int64_t)(i * kThreads + threadIdx.x) * E::kVec, v);
+  }
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    const int64_t at = base + (int64_t)(i * kThreads + threadIdx.x) * E::kVec;
+    if (at >= v) continue;
+    float d[E::kVec];
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++) {
+        float y = (E::get(w[i], j) - st.max) * c - st.log2_sum;
+        d[j] = -exp2_raw(y) * fmaf(b, fmaxf(y, kLow), a);
+      }
+      if ((uint64_t)(token - at) < (uint64_t)E::kVec) {
+#pragma unroll
+        for (int j = 0; j < E::kVec; j++)
+          if (token - at == j) d[j] += g * inv_t;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++) d[j] = 0.f;
+    }
+    if (at + E::kVec <= v) {
+      *(raw16*)(dst + at) = pack<T>(d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++)
+        if (at + j < v) E::store(dst + at + j, d[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// distillation
+// ---------------------------------------------------------------------------
+__device__ float load_any(LmType t, const void* p, int64_t i) {
+  switch (t) {
+    case LmType::F32:
+      return ((const float*)p)[i];
+    case LmType::BF16:
+      return Elem<LmType::BF16>::load((const uint16_t*)p + i);
+    default:
+      return Elem<LmType::F16>::load((const uint16_t*)p + i);
+  }
+}
+
+__device__ float wave_sum(float a) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
+  return a;
+}
+__device__ float wave_max(float a) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) a = fmaxf(a, __shfl_xor(a, d));
+  return a;
+}
+
+// a wave a row: the teacher's softmax over its record, and
+// T^2 sum q (ln q - ln p)
+template <LmType T>
+__global__ __launch_bounds__(kThreads) void distill_rows_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride,
+    int64_t rows, int64_t v, LmType tt, const void* __restrict__ teacher,
+    const int64_t* __restrict__ ids, int k, float inv_t, float c,
+    const Part* __restrict__ parts, int splits, float* __restrict__ row_loss,
+    float* __restrict__ q, RowStats* __restrict__ stats) {
+  constexpr int kMine = kMaxRecord / 64;
+  int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63;
+  Triple t = join_parts(parts + row * splits, splits, c);
+  const bool empty = t.m == -INFINITY && t.s == 0.f;
+  const float log2_sum = log2f(t.s);
+  float z[kMine];
+  int64_t id[kMine];
+  float top = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    int at = lane + 64 * i;
+    id[i] = at < k ? ids[row * k + at] : -1;
+    z[i] = id[i] != -1 ? load_any(tt, teacher, row * k + at) : -INFINITY;
+    if (z[i] == -INFINITY) id[i] = -1;
+    bad |= z[i] != z[i] || z[i] == INFINITY ||
+           (id[i] != -1 && (id[i] < 0 || id[i] >= v));
+    top = fmaxf(top, z[i]);
+  }
+  bad = __any(bad);
+  top = wave_max(top);
+  const bool absent = top == -INFINITY && !bad;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    sum += id[i] != -1 ? exp2_raw((z[i] - top) * c) : 0.f;
+  sum = wave_sum(sum);
+  const float log2_q = log2f(sum);
+  float loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    int at = lane + 64 * i;
+    float share = 0.f;
+    if (id[i] != -1 && !bad) {
+      float lq = (z[i] - top) * c - log2_q;
+      share = exp2_raw(lq);
+      float lp = empty ? -INFINITY
+                       : (Elem<T>::load(x + row * stride + id[i]) - t.m) * c -
+                             log2_sum;
+      if (share > 0.f) loss = fmaf(share, lq - lp, loss);
+    }
+    if (at < k) q[row * k + at] = share;
+  }
+  loss = wave_sum(loss) * (kLn2 / (inv_t * inv_t));
+  if (lane == 0) {
+    row_loss[row] = absent ? 0.f : bad ? NAN : loss;
+    stats[row] = {bad ? NAN : t.m, log2_sum, 0.f,
+                  absent || (empty && !bad) ? 0.f : 1.f};
+    // a row counts in the mean where it has a record
+    stats[row].entropy = absent ? 0.f : 1.f;
+  }
+}
+
+// sum or mean of the rows' losses, in a fixed order, in 64 bits; one block
+__global__ __launch_bounds__(1024) void distill_total_kernel(
+    const float* __restrict__ row_loss, const RowStats* __restrict__ stats,
+    int64_t rows, int mean, float* __restrict__ total) {
+  __shared__ double wave_s[16];
+  __shared__ double wave_n[16];
+  double s = 0, n = 0;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    s += row_loss[i];
+    n += stats[i].entropy;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    s += __shfl_xor(s, d);
+    n += __shfl_xor(n, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    wave_s[threadIdx.x >> 6] = s;
+    wave_n[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < 16; i++) {
+    s += wave_s[i];
+    n += wave_n[i];
+  }
+  double by = mean && n > 1 ? n : 1;
+  total[0] = (float)(s / by);
+  total[1] = (float)by;
+}
+
+// dx_j = g T (p_j - sum of q at j). The block writes p_j of its chunk, and
+// then the few elements that the record names once more: whole values, from
+// the logit itself, so that each is rounded once.
+template <LmType T, int U>
+__global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
+    int chunks, const int64_t* __restrict__ ids, const float* __restrict__ q,
+    int k, float inv_t, float c, const RowStats* __restrict__ stats,
+    const float* __restrict__ grad, int64_t grad_stride,
+    const float* __restrict__ count, typename Elem<T>::type* __restrict__ dx) {
+  using E = Elem<T>;
+  constexpr int kChunk = kThreads * E::kVec * U;
+  __shared__ int64_t s_id[kMaxRecord];
+  __shared__ float s_q[kMaxRecord];
+  const int64_t row = blockIdx.x / (unsigned)chunks;
+  const int64_t base = (int64_t)(blockIdx.x % (unsigned)chunks) * kChunk;
+  const int tid = threadIdx.x;
+  const RowStats st = stats[row];
+  const bool live = st.live != 0.f;
+  const float g = live ? grad[row * grad_stride] /
+                             ((count ? *count : 1.f) * inv_t)
+                       : 0.f;
+  const typename E::type* src = x + row * stride;
+  typename E::type* dst = dx + row * v;
+  u32x4 w[U];
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      w[i] = load_vec<T>(src, base + (int64_t)(i * kThreads + tid) * E::kVec,
+                         v);
+    if (tid < k) {
+      s_id[tid] = ids[row * k + tid];
+      s_q[tid] = q[row * k + tid];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    const int64_t at = base + (int64_t)(i * kThreads + tid) * E::kVec;
+    if (at >= v) continue;
+    float d[E::kVec];
+#pragma unroll
+    for (int j = 0; j < E::kVec; j++)
+      d[j] = live ? g * exp2_raw((E::get(w[i], j) - st.max) * c - st.log2_sum)
+                  : 0.f;
+    if (at + E::kVec <= v) {
+      *(raw16*)(dst + at) = pack<T>(d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++)
+        if (at + j < v) E::store(dst + at + j, d[j]);
+    }
+  }
+  if (!live) return;
+  __syncthreads();  // also orders the block's stores
+  if (tid >= k) return;
+  const int64_t id = s_id[tid];
+  if (id < base || id >= min(v, base + kChunk)) return;
+  float share = 0.f;
+  for (int j = 0; j < k; j++) {
+    if (s_id[j] != id) continue;
+    if (j < tid) return;  // the first of equal ids writes
+    share += s_q[j];
+  }
+  float p = exp2_raw((E::load(src + id) - st.max) * c - st.log2_sum);
+  E::store(dst + id, g * (p - share));
+}
+
+// ---------------------------------------------------------------------------
+// launching
+// ---------------------------------------------------------------------------
+// Parts of a row. A block keeps about 16 KB in flight, and a few blocks a
+// compute unit are needed to keep memory busy: rows are split until there
+// are kWant blocks, into parts of whole chunks.
+constexpr int64_t kWant = 1024;
+constexpr int64_t kMaxSplits = 64;
+constexpr int64_t kMaxKeys = 4096;  // that top_rows_kernel joins, 32 KB
+
+struct Plan {
+  int unroll;        // words of 16 bytes a thread holds at a time
+  int64_t splits, part_len;
+};
+
+int vec_of(LmType t) { return t == LmType::F32 ? 4 : 8; }
+
+Plan plan_of(LmType t, int64_t rows, int64_t v, int top) {
+  Plan p;
+  int64_t word = (int64_t)kThreads * vec_of(t);
+  p.unroll = rows * ((v + 4 * word - 1) / (4 * word)) >= kWant ? 4 : 1;
+  int64_t chunk = word * p.unroll;
+  int64_t chunks = (v + chunk - 1) / chunk;
+  int64_t splits = std::min(std::min(chunks, kMaxSplits),
+                            std::max<int64_t>(1, kWant / rows));
+  if (top) splits = std::min(splits, kMaxKeys / top);
+  p.part_len = (chunks + splits - 1) / splits * chunk;
+  p.splits = (v + p.part_len - 1) / p.part_len;
+  return p;
+}
+
+void check_grid(int64_t blocks) {
+  if (blocks >= (int64_t)1 << 31)
+    throw std::runtime_error("too many rows for one launch");
+}
+
+template <class F>
+void by_type(LmType t, F f) {
+  switch (t) {
+    case LmType::F32:
+      f(std::integral_constant<LmType, LmType::F32>{});
+      break;
+    case LmType::BF16:
+      f(std::integral_constant<LmType, LmType::BF16>{});
+      break;
+    case LmType::F16:
+      f(std::integral_constant<LmType, LmType::F16>{});
+      break;
+  }
+  HIP_CHECK(hipGetLastError());
+}
+
+template <bool kEntropy>
+void run_score(LmType t, const void* x, int64_t stride, int64_t rows,
+               int64_t v, const Plan& p, float c, int top, Part* parts,
+               uint64_t* keys, hipStream_t stream) {
+  check_grid(rows * p.splits);
+  auto go = [&](auto type, auto unroll, auto with_top) {
+    constexpr LmType T = decltype(type)::value;
+    score_kernel<T, decltype(unroll)::value, kEntropy,
+                 decltype(with_top)::value>
+        <<<dim3((unsigned)(rows * p.splits)), kThreads, 0, stream>>>(
+            (const typename Elem<T>::type*)x, stride, v, (int)p.splits,
+            p.part_len, c, top, parts, keys);
+  };
+  auto by_top = [&](auto type, auto unroll) {
+    if constexpr (kEntropy) {
+      if (top) return go(type, unroll, std::true_type{});
+    }
+    go(type, unroll, std::false_type{});
+  };
+  auto by_unroll = [&](auto type) {
+    if (p.unroll == 4)
+      by_top(type, std::integral_constant<int, 4>{});
+    else
+      by_top(type, std::integral_constant<int, 1>{});
+  };
+  by_type(t, by_unroll);
+}
+
+}  // namespace
+
+int64_t score_workspace(LmType t, int64_t rows, int64_t v, int top) {
+  Plan p = plan_of(t, rows, v, top);
+  return rows * p.splits * (int64_t)(sizeof(Part) + 8 * (int64_t)top);
+}
+
+void launch_token_logprobs(LmType t, const void* x, int64_t stride,
+                           int64_t rows, int64_t v, const int64_t* tokens,
+                           int64_t ignore, float inv_t, int top,
+                           float* logprobs, float* entropy, float* top_lp,
+                           int64_t* top_ids, RowStats* stats, void* ws,
+                           hipStream_t stream) {
+  Plan p = plan_of(t, rows, v, top);
+  const float c = inv_t * kLog2e;
+  Part* parts = (Part*)ws;
+  uint64_t* keys = (uint64_t*)(parts + rows * p.splits);
+  run_score<true>(t, x, stride, rows, v, p, c, top, parts, keys, stream);
+  by_type(t, [&](auto type) {
+    constexpr LmType T = decltype(type)::value;
+    logprobs_rows_kernel<T>
+        <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
+           stream>>>((const typename Elem<T>::type*)x, stride, rows, v,
+                     tokens, ignore, inv_t, c, parts, (int)p.splits, logprobs,
+                     entropy, stats);
+  });
+  if (top) {
+    top_rows_kernel<<<dim3((unsigned)rows), kThreads,
+                      (size_t)p.splits * top * 8, stream>>>(
+        keys, parts, (int)p.splits, top, tokens, ignore, inv_t, c, top_lp,
+        top_ids);
+    HIP_CHECK(hipGetLastError());
+  }
+}
+
+void launch_token_logprobs_bwd(LmType t, const void* x, int64_t stride,
+                               int64_t rows, int64_t v,
+                               const int64_t* tokens, float inv_t,
+                               const RowStats* stats, const float* g_lp,
+                               const float* g_h, void* dx,
+                               hipStream_t stream) {
+  by_type(t, [&](auto type) {
+    constexpr LmType T = decltype(type)::value;
+    constexpr int U = 4;
+    constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * U;
+    int64_t chunks = (v + chunk - 1) / chunk;
+    check_grid(rows * chunks);
+    logprobs_bwd_kernel<T, U>
+        <<<dim3((unsigned)(rows * chunks)), kThreads, 0, stream>>>(
+            (const typename Elem<T>::type*)x, stride, v, (int)chunks, tokens,
+            inv_t, inv_t * kLog2e, stats, g_lp, g_h,
+            (typename Elem<T>::type*)dx);
+  });
+}
+
+void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
+                    int64_t v, LmType tt, const void* teacher,
+                    const int64_t* ids, int k, float inv_t, float* row_loss,
+                    float* q, RowStats* stats, float* total, bool mean,
+                    void* ws, hipStream_t stream) {
+  Plan p = plan_of(t, rows, v, 0);
+  const float c = inv_t * kLog2e;
+  Part* parts = (Part*)ws;
+  run_score<false>(t, x, stride, rows, v, p, c, 0, parts, nullptr, stream);
+  by_type(t, [&](auto type) {
+    constexpr LmType T = decltype(type)::value;
+    distill_rows_kernel<T>
+        <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
+           stream>>>((const typename Elem<T>::type*)x, stride, rows, v, tt,
+                     teacher, ids, k, inv_t, c, parts, (int)p.splits,
+                     row_loss, q, stats);
+  });
+  if (total) {
+    distill_total_kernel<<<1, 1024, 0, stream>>>(row_loss, stats, rows, mean,
+                                                 total);
+    HIP_CHECK(hipGetLastError());
+  }
+}
+
+void launch_distill_bwd(LmType t, const void* x, int64_t stride,
+                        int64_t rows, int64_t v, const int64_t* ids,
+                        const float* q, int k, float inv_t,
+                        const RowStats* stats, const float* grad,
+                        int64_t grad_stride, const float* count, void* dx,
+                        hipStream_t stream) {
+  by_type(t, [&](auto type) {
+    constexpr LmType T = decltype(type)::value;
+    constexpr int U = 4;
+    constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * U;
+    int64_t chunks = (v + chunk - 1) / chunk;
+    check_grid(rows * chunks);
+    distill_bwd_kernel<T, U>
+        <<<dim3((unsigned)(rows * chunks)), kThreads, 0, stream>>>(
+            (const typename Elem<T>::type*)x, stride, v, (int)chunks, ids, q,
+            k, inv_t, inv_t * kLog2e, stats, grad, grad_stride, count,
+            (typename Elem<T>::type*)dx);
+  });
+}

@@ -1,0 +1,356 @@
+"""Scoring rows of logits for sandboxed user code: log probabilities of given
+tokens with entropies and top alternatives, and distillation from a teacher's
+recorded top logits, with their backward passes, on gfx950 kernels.
+
+Importable standalone inside the sandbox (APP_OPS_DIR is on sys.path), next
+to torch:
+
+    import hiplm
+    r = hiplm.token_logprobs(logits, tokens, top=20)
+    r.logprobs, r.entropy, r.top_logprobs, r.top_tokens
+    loss = hiplm.topk_distill_loss(student_logits, r.top_logprobs,
+                                   r.top_tokens)
+
+A row of logits is read once in a forward and once in a backward pass, in
+its own type (float32, bfloat16, float16); sums are float32. Masked entries
+are -inf (or very low) logits.
+
+GPU tensors run on the kernels, on torch's current stream of their device,
+and raise where the extension is missing; CPU tensors are computed in plain
+torch. Second derivatives are refused.
+"""
+
+from collections import namedtuple
+import math
+
+import hiptorch
+
+MAX_TOP = 128      # alternatives of a row
+MAX_RECORD = 256   # recorded teacher entries of a row
+
+STATS = {"token_logprobs": 0, "topk_distill_loss": 0}
+
+TokenLogprobs = namedtuple(
+    "TokenLogprobs", ["logprobs", "entropy", "top_logprobs", "top_tokens"])
+
+_functions = {}
+
+
+def _check_logits(logits):
+    torch = hiptorch.torch_tensor("logits", logits)
+    code = hiptorch.lm_code(torch, "logits", logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits need a last axis, got {list(logits.shape)}")
+    if logits.shape[-1] >= 1 << 31:
+        raise ValueError("the last axis of logits is too long")
+    return torch, code
+
+
+def _check_temperature(temperature) -> float:
+    t = float(temperature)
+    if not 1e-4 <= t <= 1e4:
+        raise ValueError(f"temperature must be in [1e-4, 1e4], got {t}")
+    return t
+
+
+def _check_ids(torch, name, ids, shape, device):
+    hiptorch.torch_tensor(name, ids)
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{name} must be int64 or int32, got {ids.dtype}")
+    if ids.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got "
+                         f"{list(ids.shape)}")
+    if ids.device != device:
+        raise ValueError(f"{name} are on {ids.device}, logits on {device}")
+    return ids.long().contiguous()
+
+
+def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """ln p(token), the entropy and the ``top`` most likely tokens of rows of
+    logits, p = softmax(logits / temperature).
+
+    logits: [..., v]; tokens: [...] (int64, int32). Returns ``logprobs`` and
+    ``entropy`` [...] in float32, both differentiable, ``top_logprobs``
+    [..., top] in float32 and ``top_tokens`` [..., top] in int64, largest
+    first, of equal logits the lowest token first; neither carries a
+    gradient. top: 0 to 128, at most v.
+
+    A masked token (-inf) is no alternative: a row with fewer than ``top``
+    others ends in (-inf, -1). A row that is masked as a whole has no
+    distribution: ln p is -inf, the entropy 0, the gradient 0. A row whose
+    token is ``ignore_index`` is padding: 0, 0, (-inf, -1) and no gradient.
+    A token outside of [0, v), or a NaN or +inf among the logits, gives NaN.
+    """
+    torch, code = _check_logits(logits)
+    t = _check_temperature(temperature)
+    lead, v = logits.shape[:-1], logits.shape[-1]
+    top = int(top)
+    if not 0 <= top <= min(MAX_TOP, v):
+        raise ValueError(f"top must be in [0, {min(MAX_TOP, v)}], got {top}")
+    tokens = _check_ids(torch, "tokens", tokens, lead, logits.device)
+    if not logits.is_cuda:
+        return _cpu_token_logprobs(torch, logits, tokens, top, t,
+                                   int(ignore_index))
+    out = _function("logprobs", torch).apply(
+        logits, tokens, code, top, 1.0 / t, int(ignore_index))
+    STATS["token_logprobs"] += 1
+    return TokenLogprobs(*out)
+
+
+def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
+                      temperature=1.0, reduction: str = "mean"):
+    """The divergence of a student from a teacher's recorded top logits,
+    T^2 sum_k q_k (ln q_k - ln p[token_k]), with q the softmax of the
+    recorded entries over each other and p the student's softmax over the
+    whole vocabulary, both at temperature T.
+
+    logits: the student's, [..., v]. teacher_logits: [..., k] (float32,
+    bfloat16, float16), logits or log probabilities, k from 1 to 256, without
+    a gradient. teacher_tokens: [..., k] (int64, int32). A row with fewer
+    entries is filled with tokens of -1 or logits of -inf; one with none
+    has no loss and no gradient. A token that is recorded twice counts
+    twice.
+
+    reduction: "mean" (over rows with a record; 0 if there are none), "sum"
+    or "none" ([...]); rows' losses and the result are float32. An entry that the student masks
+    (-inf) gives an infinite loss, with the finite gradient T (p - q) / rows.
+    A token outside of [0, v) but -1, or a NaN or +inf on either side, gives
+    NaN.
+    """
+    torch, code = _check_logits(logits)
+    t = _check_temperature(temperature)
+    lead = logits.shape[:-1]
+    hiptorch.torch_tensor("teacher_logits", teacher_logits)
+    t_code = hiptorch.lm_code(torch, "teacher_logits", teacher_logits)
+    if (teacher_logits.dim() != logits.dim()
+            or teacher_logits.shape[:-1] != lead
+            or not 1 <= teacher_logits.shape[-1] <= MAX_RECORD):
+        raise ValueError(
+            f"teacher_logits must be [{', '.join(map(str, lead))}, k] with k "
+            f"from 1 to {MAX_RECORD}, got {list(teacher_logits.shape)}")
+    if teacher_logits.device != logits.device:
+        raise ValueError(f"teacher_logits are on {teacher_logits.device}, "
+                         f"logits on {logits.device}")
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the teacher gets no gradient: detach its logits")
+    ids = _check_ids(torch, "teacher_tokens", teacher_tokens,
+                     teacher_logits.shape, logits.device)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none', got "
+                         f"{reduction!r}")
+    if not logits.is_cuda:
+        return _cpu_distill(torch, logits, teacher_logits.detach(), ids, t,
+                            reduction)
+    loss = _function("distill", torch).apply(
+        logits, teacher_logits.detach().contiguous(), ids, code, t_code,
+        1.0 / t, reduction)
+    STATS["topk_distill_loss"] += 1
+    return loss
+
+
+# ---------------------------------------------------------------------------
+# GPU tensors
+# ---------------------------------------------------------------------------
+def _function(name, torch):
+    """The autograd function of that name; made at its first use, since
+    importing this module must not import torch."""
+    if not _functions:
+        _make_functions(torch)
+    return _functions[name]
+
+
+def _make_functions(torch):
+    from torch.autograd.function import once_differentiable
+
+    # floats that a row leaves for its backward
+    stats_len = 4
+
+    def workspace(ext, code, rows, v, top, device):
+        need = ext.score_workspace(code, rows, v, top)
+        # from torch's allocator, on the stream that uses it: of a captured
+        # graph, its own
+        return torch.empty(need, dtype=torch.uint8, device=device)
+
+    class TokenLogprobsFunction(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, logits, tokens, code, top, inv_t, ignore):
+            ext = hiptorch.ensure_hiplm()
+            lead, v = logits.shape[:-1], logits.shape[-1]
+            x, stride = hiptorch.rows_view(logits)
+            rows, device = x.shape[0], logits.device
+            f32 = torch.float32
+            logprobs = torch.empty(lead, dtype=f32, device=device)
+            entropy = torch.empty(lead, dtype=f32, device=device)
+            top_lp = torch.empty((*lead, top), dtype=f32, device=device)
+            top_ids = torch.empty((*lead, top), dtype=torch.int64,
+                                  device=device)
+            grad = ctx.needs_input_grad[0]
+            stats = None
+            if grad:
+                stats = torch.empty(rows, stats_len, dtype=f32,
+                                    device=device)
+            if rows:
+                work = workspace(ext, code, rows, v, top, device)
+                with hiptorch.on_device(torch, x) as stream:
+                    ext.token_logprobs(
+                        code, x.data_ptr(), stride, rows, v,
+                        tokens.data_ptr(), ignore, inv_t, top,
+                        logprobs.data_ptr(), entropy.data_ptr(),
+                        top_lp.data_ptr(), top_ids.data_ptr(),
+                        stats.data_ptr() if grad else 0, work.data_ptr(),
+                        stream)
+            ctx.mark_non_differentiable(top_lp, top_ids)
+            ctx.set_materialize_grads(False)
+            if grad:
+                ctx.save_for_backward(logits, tokens, stats)
+                ctx.code, ctx.inv_t = code, inv_t
+            return logprobs, entropy, top_lp, top_ids
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, g_lp, g_h, _top_lp, _top_ids):
+            if g_lp is None and g_h is None:
+                return (None,) * 6
+            logits, tokens, stats = ctx.saved_tensors
+            x, stride = hiptorch.rows_view(logits)
+            rows, v = x.shape
+            dx = torch.empty(logits.shape, dtype=logits.dtype,
+                             device=logits.device)
+            if rows:
+                g_lp = None if g_lp is None else g_lp.contiguous()
+                g_h = None if g_h is None else g_h.contiguous()
+                with hiptorch.on_device(torch, x) as stream:
+                    hiptorch.ensure_hiplm().token_logprobs_bwd(
+                        ctx.code, x.data_ptr(), stride, rows, v,
+                        tokens.data_ptr(), ctx.inv_t, stats.data_ptr(),
+                        0 if g_lp is None else g_lp.data_ptr(),
+                        0 if g_h is None else g_h.data_ptr(),
+                        dx.data_ptr(), stream)
+            return dx, None, None, None, None, None
+
+    class DistillFunction(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, logits, teacher, ids, code, t_code, inv_t,
+                    reduction):
+            ext = hiptorch.ensure_hiplm()
+            lead, v = logits.shape[:-1], logits.shape[-1]
+            x, stride = hiptorch.rows_view(logits)
+            rows, device = x.shape[0], logits.device
+            k = teacher.shape[-1]
+            f32 = torch.float32
+            if not rows:
+                ctx.empty = True
+                ctx.save_for_backward(logits)
+                return torch.zeros(lead if reduction == "none" else (),
+                                   dtype=f32, device=device)
+            ctx.empty = False
+            row_loss = torch.empty(lead, dtype=f32, device=device)
+            q = torch.empty(rows, k, dtype=f32, device=device)
+            stats = torch.empty(rows, stats_len, dtype=f32, device=device)
+            total = None
+            if reduction != "none":
+                # the result, and what it was divided by
+                total = torch.empty(2, dtype=f32, device=device)
+            work = workspace(ext, code, rows, v, 0, device)
+            with hiptorch.on_device(torch, x) as stream:
+                ext.distill(
+                    code, x.data_ptr(), stride, rows, v, t_code,
+                    teacher.data_ptr(), ids.data_ptr(), k, inv_t,
+                    row_loss.data_ptr(), q.data_ptr(), stats.data_ptr(),
+                    0 if total is None else total.data_ptr(),
+                    reduction == "mean", work.data_ptr(), stream)
+            if ctx.needs_input_grad[0]:
+                ctx.save_for_backward(logits, ids, q, stats, total)
+                ctx.code, ctx.inv_t = code, inv_t
+            return row_loss if total is None else total[0].clone()
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            if ctx.empty:
+                (logits,) = ctx.saved_tensors
+                return (torch.zeros_like(logits),) + (None,) * 6
+            logits, ids, q, stats, total = ctx.saved_tensors
+            x, stride = hiptorch.rows_view(logits)
+            rows, v = x.shape
+            grad = grad.contiguous()
+            dx = torch.empty(logits.shape, dtype=logits.dtype,
+                             device=logits.device)
+            with hiptorch.on_device(torch, x) as stream:
+                hiptorch.ensure_hiplm().distill_bwd(
+                    ctx.code, x.data_ptr(), stride, rows, v, ids.data_ptr(),
+                    q.data_ptr(), q.shape[1], ctx.inv_t, stats.data_ptr(),
+                    grad.data_ptr(), 1 if total is None else 0,
+                    0 if total is None else total.data_ptr() + 4,
+                    dx.data_ptr(), stream)
+            return (dx,) + (None,) * 6
+
+    _functions["logprobs"] = TokenLogprobsFunction
+    _functions["distill"] = DistillFunction
+
+
+# ---------------------------------------------------------------------------
+# CPU tensors
+# ---------------------------------------------------------------------------
+def _cpu_log_softmax(torch, logits, t):
+    """ln softmax in float32, and which rows are masked as a whole (their
+    numbers are of no use, but no NaN either). The largest logit is taken off
+    before the division: a lowest value divided would be an infinity."""
+    z = logits.float()
+    empty = (z == -math.inf).all(-1)
+    z = torch.where(empty[..., None], 0.0, z)
+    z = z - z.detach().amax(-1, keepdim=True)
+    return torch.log_softmax(z / t, -1), empty
+
+
+def _cpu_token_logprobs(torch, logits, tokens, top, t, ignore):
+    v = logits.shape[-1]
+    lp, empty = _cpu_log_softmax(torch, logits, t)
+    ignored = tokens == ignore
+    outside = ~ignored & ((tokens < 0) | (tokens >= v))
+    at = tokens.clamp(0, v - 1)[..., None]
+    nan, zero = math.nan, 0.0
+    logprobs = lp.gather(-1, at)[..., 0]
+    logprobs = torch.where(empty, -math.inf, logprobs)
+    entropy = -(lp.exp() * lp.clamp(min=-1e4)).sum(-1)
+    entropy = torch.where(empty, zero, entropy)
+    logprobs, entropy = (
+        torch.where(ignored, zero, torch.where(outside, nan, o))
+        for o in (logprobs, entropy))
+    with torch.no_grad():
+        z = logits.float()
+        z = torch.where(z.isnan() | ignored[..., None], -math.inf, z)
+        values, ids = torch.sort(z, dim=-1, descending=True, stable=True)
+        values, ids = values[..., :top], ids[..., :top]
+        there = values > -math.inf
+        top_lp = torch.where(there, lp.gather(-1, ids), -math.inf)
+        top_ids = torch.where(there, ids, -1)
+    return TokenLogprobs(logprobs, entropy, top_lp, top_ids)
+
+
+def _cpu_distill(torch, logits, teacher, ids, t, reduction):
+    v = logits.shape[-1]
+    lp, empty = _cpu_log_softmax(torch, logits, t)
+    z = teacher.float()
+    there = (ids != -1) & (z != -math.inf)
+    bad = there & (z.isnan() | (z == math.inf) | (ids < 0) | (ids >= v))
+    absent = ~there.any(-1)
+    z = torch.where(there & ~bad, z, -math.inf)
+    lq, _ = _cpu_log_softmax(torch, z, t)
+    # a share of 0 adds nothing, whatever the student gives it
+    there = there & (lq.exp() > 0)
+    lp = torch.where(empty[..., None], lp.detach(), lp)
+    mine = lp.gather(-1, ids.clamp(0, v - 1))
+    mine = torch.where(empty[..., None], -math.inf, mine)
+    mine = torch.where(there, mine, 0.0)
+    loss = (torch.where(there, lq.exp() * lq, 0.0)
+            - torch.where(there, lq.exp() * mine, 0.0)).sum(-1) * (t * t)
+    loss = torch.where(absent, 0.0, loss)
+    loss = torch.where(bad.any(-1), math.nan, loss)
+    if reduction == "none":
+        return loss
+    total = loss.sum()
+    if reduction == "mean":
+        total = total / (~absent).sum().clamp(min=1)
+    return total

@@ -53,6 +53,89 @@ def _ensure_hipgemm():
         _hipgemm = m
     return _hipgemm
 
+# _hiplm (the language-model kernels that hipmx and hiplm call) follows the
+# same rule.
+_hiplm = None
+
+
+def ensure_hiplm():
+    global _hiplm
+    if _hiplm is None:
+        import torch  # noqa: F401  (load torch's HIP runtime first)
+
+        import _hiplm as m
+
+        _hiplm = m
+    return _hiplm
+
+
+# ---------------------------------------------------------------------------
+# what the explicit operators (hipmx, hiplm) share
+# ---------------------------------------------------------------------------
+_lm_codes = {}
+
+
+def LM_CODES(torch) -> dict:
+    """The kernels' code of each type that they take."""
+    if not _lm_codes:
+        _lm_codes.update({torch.float32: 0, torch.bfloat16: 1,
+                          torch.float16: 2})
+    return _lm_codes
+
+
+def torch_tensor(name, x):
+    """torch, where x is a tensor; a TypeError that names it otherwise."""
+    import torch
+
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
+    if x.layout != torch.strided:
+        raise TypeError(f"{name} must be a strided tensor, got {x.layout}")
+    return torch
+
+
+def lm_code(torch, name, x) -> int:
+    code = LM_CODES(torch).get(x.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got "
+                        f"{x.dtype}")
+    return code
+
+
+def rows_view(x):
+    """x as [rows, k] with neighbouring elements in a row, and the distance
+    of its rows: a view where its strides allow one, else a copy."""
+    k = x.shape[-1]
+    rows = 1
+    for d in x.shape[:-1]:
+        rows *= d
+    x2 = x if x.dim() == 2 else x.reshape(rows, k)
+    if k > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    return x2, (x2.stride(0) if rows > 1 else k)
+
+
+class on_device:
+    """Makes x's device the current one while kernels are launched on it, and
+    gives its current stream."""
+
+    __slots__ = ("_torch", "_index", "_before")
+
+    def __init__(self, torch, x):
+        self._torch, self._index = torch, x.device.index
+
+    def __enter__(self):
+        cuda = self._torch.cuda
+        self._before = cuda.current_device()
+        if self._before != self._index:
+            cuda.set_device(self._index)
+        return cuda.current_stream(self._index).cuda_stream
+
+    def __exit__(self, *_):
+        if self._before != self._index:
+            self._torch.cuda.set_device(self._before)
+
+
 # route only when the kernel launch is worth more than its overhead;
 # env-tunable like hipnp's thresholds
 MIN_MM_FLOPS = float(os.environ.get("APP_HIP_TORCH_MIN_FLOPS", 5e7))

@@ -1,0 +1,519 @@
+"""GPU tests of the scoring operators (ops/hiplm.py): the kernels against the
+definitions in 64 bits.
+
+Slack. The kernels work in float32 on the logits' own values. A term e of a
+row's sum is off by its exponent's rounding (3 steps of the exponent y) and
+its own (2 steps), a thread's sum of a row of v elements by v / 256 steps at
+most, their union by 20: relative to the sum at most STEP (v / 256 + 64 + 3
+|y|), y <= 40 where e counts. What is added to or multiplied with that is a
+few steps more.
+"""
+
+import math
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+OPS_DIR = Path(__file__).resolve().parent.parent / "code_interpreter_amd" / "ops"
+sys.path.insert(0, str(OPS_DIR))
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "bfloat16", "float16"]
+STEP = 2.0 ** -24
+INF = math.inf
+
+
+@pytest.fixture(scope="module")
+def lm():
+    torch = pytest.importorskip("torch")
+    if not torch.cuda.is_available():
+        pytest.skip("torch sees no GPU")
+    import hiplm
+
+    return torch, hiplm
+
+
+def relative(v):
+    return STEP * (v / 256 + 200)
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def near(got, want, slack):
+    got = host(got)
+    most = np.finfo(np.float32).max  # results are float32
+    want = np.where(np.abs(want) > most, np.copysign(INF, want), want)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        err = np.where(same, 0, np.abs(got - want) - slack)
+    assert (err <= 0).all(), np.argwhere(~(err <= 0))[:5]
+
+
+def trouble(torch, v, dtype, seed=0):
+    """Rows that are plain, tied, sharp, masked in part or as a whole (by -inf
+    and by the type's lowest value), rising, falling, with a NaN or an
+    infinity; their tokens."""
+    g = torch.Generator().manual_seed(seed + v)
+    dt = getattr(torch, dtype)
+    low = torch.finfo(dt).min
+    x = (torch.randn(18, v, generator=g) * 3).to(dt)
+    x[1] = 2.5
+    x[2, v // 2] = 60
+    x[3, ::2] = -INF
+    x[4, 1:] = -INF
+    x[5] = -INF
+    x[6, : v - v // 5] = low
+    x[7] = low
+    x[8, v // 3] = math.nan
+    x[9, v // 3] = INF
+    x[12] = torch.linspace(-8, 8, v).to(dt)
+    x[13] = torch.linspace(8, -8, v).to(dt)
+    x[14] = (torch.arange(v) % 3).to(dt)
+    x[15] = 0.0
+    x[15, 1::2] = -0.0
+    x[16, : v - v // 7] = -INF
+    x[17] = (x[17].float() * 1000).to(dt)
+    tokens = torch.randint(v, (18,), generator=g)
+    tokens[4] = 0
+    tokens[10] = -100
+    tokens[11] = v
+    return x.cuda(), tokens.cuda()
+
+
+def check_logprobs(torch, hiplm, x, tokens, top, t):
+    import lm_oracle as oracle
+
+    v = x.shape[-1]
+    r = hiplm.token_logprobs(x, tokens, top=top, temperature=t)
+    lp, h, top_lp, top_ids = oracle.token_logprobs(
+        host(x), host(tokens).astype(np.int64), top, t)
+    def slack(a):
+        return relative(v) + 4 * STEP * np.abs(np.where(np.isfinite(a), a, 0))
+
+    near(r.logprobs, lp, slack(lp))
+    # H = ln S - U / S: U's terms are at most 40 S in sum
+    near(r.entropy, h, 42 * relative(v))
+    rows = ~np.isnan(top_lp).any(-1) if top else slice(0)
+    assert np.array_equal(r.top_tokens.cpu().numpy()[rows], top_ids[rows])
+    near(r.top_logprobs, top_lp, slack(top_lp))
+    return r
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v,top", [
+    (1, 1), (2, 2), (5, 3), (63, 20), (256, 128), (1000, 1), (2047, 5),
+    (2049, 64), (8192, 20), (10007, 128), (50001, 20), (131072, 64),
+])
+def test_token_logprobs(lm, dtype, v, top):
+    torch, hiplm = lm
+    x, tokens = trouble(torch, v, dtype)
+    check_logprobs(torch, hiplm, x, tokens, top, 1.0)
+
+
+@pytest.mark.parametrize("t", [0.25, 0.9, 4.0])
+def test_token_logprobs_temperature(lm, t):
+    torch, hiplm = lm
+    for dtype in DTYPES:
+        x, tokens = trouble(torch, 1001, dtype)
+        check_logprobs(torch, hiplm, x, tokens, 7, t)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows", [300, 1100])
+@pytest.mark.parametrize("v,top", [(777, 9), (40000, 33)])
+def test_token_logprobs_many_rows(lm, dtype, rows, v, top):
+    """Enough rows that each is one block's: compared with the same rows a
+    few at a time, which are split, and a few of them with the definition."""
+    torch, hiplm = lm
+    x, tokens = trouble(torch, v, dtype)
+    keep = torch.arange(rows) % 18
+    many = hiplm.token_logprobs(x[keep], tokens[keep], top=top)
+    few = check_logprobs(torch, hiplm, x, tokens, top, 1.0)
+    good = [r for r in range(18) if r not in (8, 9)]
+    for i in good:
+        at = torch.nonzero(keep == i)[:, 0].cuda()
+        assert torch.equal(many.top_tokens[at],
+                           few.top_tokens[i].expand(len(at), top))
+        for a, b in ((many.logprobs, few.logprobs),
+                     (many.entropy, few.entropy)):
+            # the same sums in another order
+            wide = 84 * relative(v) + 8 * STEP * abs(host(b[i]))
+            near(a[at], np.broadcast_to(host(b[i]), (len(at),)),
+                 np.where(np.isfinite(wide), wide, 0))
+
+
+def test_top_of_hard_rows(lm):
+    """Rows that make the choice of alternatives work: all values equal but
+    few, the best in one thread's place, the best in the last part, rising in
+    steps, one cluster."""
+    torch, hiplm = lm
+    v = 70001
+    x = torch.full((7, v), -1.0)
+    x[0, v - 3:] = torch.tensor([1.0, 2.0, 3.0])
+    x[1, 40000:40008] = torch.arange(8).float()
+    x[2, 65000:] = torch.rand(v - 65000)
+    x[3] = torch.div(torch.arange(v), 500, rounding_mode="floor").float()
+    x[4, 1024:1024 + 3000] = 5 + torch.rand(3000)
+    x[5] = (torch.arange(v) * 7919 % v).float()
+    x[6] = torch.finfo(torch.float32).min
+    x[6, ::1000] = 0.5
+    tokens = torch.zeros(7, dtype=torch.long)
+    for dtype in DTYPES:
+        for top in (1, 20, 64, 128):
+            few = x.to(getattr(torch, dtype)).cuda()
+            check_logprobs(torch, hiplm, few, tokens.cuda(), top, 1.0)
+            many = hiplm.token_logprobs(few.repeat(150, 1),
+                                        tokens.repeat(150).cuda(), top=top)
+            one = hiplm.token_logprobs(few, tokens.cuda(), top=top)
+            assert torch.equal(many.top_tokens,
+                               one.top_tokens.repeat(150, 1))
+
+
+def check_grad(torch, got, want, size, v, dtype):
+    """One rounding to the logits' type, and the error of p: of its exponent,
+    and of the row's sum. The hardware's exponential has no subnormal
+    results: a p below 2^-126 is 0. What it is multiplied with is at most
+    (|g_lp| + |g_h| (|ln p| + H)) / t with |g| < 5, H < 12 and t > 0.6, and p
+    |ln p| is at most 88 * 2^-126 there: below 2^-116 in all."""
+    info = torch.finfo(getattr(torch, dtype))
+    slack = (2.0 ** -116 + info.eps / 2 * (np.abs(want) + 50 * relative(v) * size)
+             + 50 * relative(v) * size + info.smallest_normal * info.eps)
+    near(got, want, slack)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [1, 7, 64, 2049, 10007, 65536])
+def test_token_logprobs_gradient(lm, dtype, v):
+    torch, hiplm = lm
+    import lm_oracle as oracle
+
+    x, tokens = trouble(torch, v, dtype)
+    x.requires_grad_(True)
+    g = torch.Generator().manual_seed(v)
+    for t, use in ((1.0, "both"), (0.7, "lp"), (1.3, "h")):
+        r = hiplm.token_logprobs(x, tokens, temperature=t)
+        g_lp, g_h = (torch.randn(18, generator=g).cuda() for _ in range(2))
+        outs, gs = [r.logprobs, r.entropy], [g_lp, g_h]
+        if use == "lp":
+            outs, gs, g_h = outs[:1], gs[:1], torch.zeros(18)
+        if use == "h":
+            outs, gs, g_lp = outs[1:], gs[1:], torch.zeros(18)
+        (got,) = torch.autograd.grad(outs, [x], gs)
+        assert got.dtype == x.dtype and got.shape == x.shape
+        want, size = oracle.token_logprobs_grad(
+            host(x), host(tokens).astype(np.int64), t, host(g_lp), host(g_h))
+        rows = [i for i in range(18) if i not in (8, 9)]
+        check_grad(torch, got[rows], want[rows], size[rows], v, dtype)
+        assert got[8].isnan().any() and got[11].isnan().all()
+
+
+def test_gradient_against_differences(lm):
+    torch, hiplm = lm
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(3, 50, generator=g).cuda()
+    tokens = torch.tensor([4, 0, 49]).cuda()
+    teacher = torch.randn(3, 6, generator=g).cuda()
+    ids = torch.stack([torch.randperm(50, generator=g)[:6]
+                       for _ in range(3)]).cuda()
+
+    def scores(z):
+        r = hiplm.token_logprobs(z, tokens, temperature=0.8)
+        loss = hiplm.topk_distill_loss(z, teacher, ids, temperature=1.5)
+        return (r.logprobs * 0.3 - r.entropy * 0.7).sum() + loss
+
+    z = x.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(scores(z), [z])
+    step = 2.0 ** -6
+    for i, j in ((0, 4), (0, 5), (1, 0), (2, 49), (2, 17)):
+        d = torch.zeros_like(x)
+        d[i, j] = step
+        with torch.no_grad():
+            got = ((scores(x + d) - scores(x - d)) / (2 * step)).item()
+        # the third derivative is below 8, a score is off by some 2^-20
+        assert abs(got - grad[i, j].item()) < 8 * step ** 2 / 6 + 2.0 ** -13
+
+
+@pytest.mark.parametrize("v", [1000, 9001])
+def test_strided_logits(lm, v):
+    torch, hiplm = lm
+    wide = torch.randn(6, 4, v + 24, device="cuda", dtype=torch.bfloat16)
+    tokens = torch.randint(v, (6, 4), device="cuda")
+    views = [wide[..., :v], wide[..., 5:v + 5], wide[..., 1:v + 1]]
+    views.append(wide[..., :v].transpose(0, 1).contiguous().transpose(0, 1))
+    views.append(wide[..., :v].permute(2, 0, 1).contiguous().permute(1, 2, 0))
+    views.append(wide[:1, :, 3:v + 3].expand(6, 4, v))
+    for x in views:
+        a = x.detach().requires_grad_(True)
+        b = x.detach().contiguous().requires_grad_(True)
+        outs = []
+        for z in (a, b):
+            r = hiplm.token_logprobs(z, tokens, top=9)
+            loss = hiplm.topk_distill_loss(z, r.top_logprobs.flip(-1),
+                                           r.top_tokens)
+            total = loss + r.logprobs.mean() + r.entropy.sum()
+            (grad,) = torch.autograd.grad(total, [z])
+            outs.append([*[o.detach() for o in r], loss.detach(), grad])
+        for p, q in zip(*outs):
+            assert torch.equal(p, q)
+
+
+def records(torch, v, k, rows, dtype):
+    g = torch.Generator().manual_seed(100 * v + k)
+    teacher = (torch.randn(rows, k, generator=g) * 2).to(getattr(torch, dtype))
+    ids = torch.randint(v, (rows, k), generator=g)  # repeated ones too
+    ids[1, k // 2:] = -1
+    teacher[2, k // 2:] = -INF
+    ids[3] = -1
+    teacher[4] = -INF
+    ids[7] = ids[7, 0]
+    ids[10] = torch.arange(k) % v
+    ids[12] = v - 1 - torch.arange(k) % v
+    teacher[13] = torch.finfo(teacher.dtype).min
+    ids[11, 0] = v
+    teacher[14, 0] = math.nan
+    return teacher.cuda(), ids.cuda()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dtype,t_dtype", [
+    ("float32", "float32"), ("bfloat16", "float32"), ("float16", "bfloat16"),
+    ("bfloat16", "float16")])
+@pytest.mark.parametrize("v,k", [(1, 1), (9, 4), (2049, 64), (10007, 256),
+                                 (65536, 20)])
+def test_distill(lm, dtype, t_dtype, v, k, reduction):
+    torch, hiplm = lm
+    import lm_oracle as oracle
+
+    t = 1.5
+    x, _ = trouble(torch, v, dtype)
+    teacher, ids = records(torch, v, k, 18, t_dtype)
+    keep = [0, 1, 2, 3, 4, 6, 7, 10, 12, 13, 14, 15, 17]
+    if reduction != "none":  # the one with a NaN in its record
+        keep.remove(14)
+    else:
+        keep += [5, 8, 9, 11, 16]
+    x = x[keep].requires_grad_(True)
+    loss = hiplm.topk_distill_loss(x, teacher[keep], ids[keep],
+                                   temperature=t, reduction=reduction)
+    want, grad, size = oracle.distill(
+        host(x), host(teacher[keep]), host(ids[keep]).astype(np.int64), t,
+        reduction)
+    with np.errstate(invalid="ignore"):
+        spread = (relative(v) + 64 * STEP) * (
+            1 + np.abs(host(x)).max(initial=0, where=host(x) > -1e30)) * 4
+    scale = t * t + np.abs(np.where(np.isfinite(want), want, 0))
+    near(loss, want, spread * scale)
+    (got,) = torch.autograd.grad(loss.sum(), [x])
+    rows = np.isfinite(np.broadcast_to(want, (len(keep),)))
+    check_grad(torch, got[rows], grad[rows], size[rows], v, dtype)
+    # a masked entry in the record: an infinite loss, a finite gradient
+    if reduction == "none":
+        for i, r in enumerate(keep):
+            if want[i] == INF:
+                assert got[i].isfinite().all()
+
+
+def test_distill_weights_rows(lm):
+    torch, hiplm = lm
+    x = torch.randn(5, 300, device="cuda", requires_grad=True)
+    teacher, ids = torch.randn(5, 8).cuda(), torch.randint(300, (5, 8)).cuda()
+    rows = hiplm.topk_distill_loss(x, teacher, ids, reduction="none")
+    g = torch.randn(5, device="cuda")
+    (a,) = torch.autograd.grad(rows, [x], g, retain_graph=True)
+    (b,) = torch.autograd.grad(rows.sum(), [x])  # a gradient of no stride
+    s = hiplm.topk_distill_loss(x, teacher, ids, reduction="sum")
+    (c,) = torch.autograd.grad(s, [x])
+    assert torch.equal(b, c)
+    torch.testing.assert_close(a, b * g[:, None], rtol=1e-6, atol=1e-9)
+    m = hiplm.topk_distill_loss(x, teacher, ids)
+    torch.testing.assert_close(m * 5, s)
+
+
+def test_empty(lm):
+    torch, hiplm = lm
+    x = torch.zeros(0, 3, 9, device="cuda", requires_grad=True)
+    ids = torch.zeros(0, 3, dtype=torch.long, device="cuda")
+    r = hiplm.token_logprobs(x, ids, top=2)
+    assert r.logprobs.shape == (0, 3) and r.top_tokens.shape == (0, 3, 2)
+    (g,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), [x])
+    assert g.shape == x.shape
+    loss = hiplm.topk_distill_loss(
+        x, torch.zeros(0, 3, 2).cuda(),
+        torch.zeros(0, 3, 2, dtype=torch.long).cuda())
+    assert loss.item() == 0
+    (g,) = torch.autograd.grad(loss, [x])
+    assert g.shape == x.shape
+    none = torch.full((4, 3), -1, device="cuda")
+    z = torch.randn(4, 9, device="cuda", requires_grad=True)
+    loss = hiplm.topk_distill_loss(z, torch.zeros(4, 3).cuda(), none)
+    (g,) = torch.autograd.grad(loss, [z])
+    assert loss.item() == 0 and (g == 0).all()
+
+
+def test_second_derivatives_are_refused(lm):
+    torch, hiplm = lm
+    x = torch.randn(2, 9, device="cuda", requires_grad=True)
+    r = hiplm.token_logprobs(x, torch.zeros(2, dtype=torch.long).cuda())
+    (g,) = torch.autograd.grad(r.logprobs.sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_same_bits(lm):
+    torch, hiplm = lm
+    x, tokens = trouble(torch, 50001, "bfloat16")
+    x.requires_grad_(True)
+    outs = []
+    for _ in range(3):
+        r = hiplm.token_logprobs(x, tokens, top=20)
+        loss = hiplm.topk_distill_loss(x[:3], r.top_logprobs[:3],
+                                       r.top_tokens[:3])
+        (g,) = torch.autograd.grad(r.logprobs[:8].sum() + loss, [x])
+        outs.append([o.detach().nan_to_num(nan=7.0)
+                     for o in (*r, loss, g)])
+    for other in outs[1:]:
+        for a, b in zip(outs[0], other):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [2, 700])
+def test_forward_and_backward_in_a_graph(lm, rows):
+    torch, hiplm = lm
+    v, k = 5003, 12
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def inputs():
+        x = torch.randn(rows, v, generator=g, device="cuda")
+        return (x.bfloat16(),
+                torch.randint(v, (rows,), generator=g, device="cuda"))
+
+    def step(x, tokens):
+        r = hiplm.token_logprobs(x, tokens, top=k)
+        loss = hiplm.topk_distill_loss(x, r.top_logprobs.sqrt().nan_to_num(),
+                                       r.top_tokens, temperature=2.0)
+        total = loss + r.entropy.mean() - r.logprobs.mean()
+        return [*r, loss, *torch.autograd.grad(total, [x])]
+
+    sets = [inputs() for _ in range(2)]
+    want = []
+    for x, tokens in sets:
+        out = step(x.clone().requires_grad_(True), tokens)
+        want.append([o.detach().clone() for o in out])
+        del out
+    x, tokens = sets[0][0].clone().requires_grad_(True), sets[0][1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, tokens)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, tokens)
+    got = [o.detach() for o in got]
+    for i in (0, 1, 0, 1):
+        with torch.no_grad():
+            x.copy_(sets[i][0])
+        tokens.copy_(sets[i][1])
+        graph.replay()
+        step(sets[1][0].clone().requires_grad_(True), sets[1][1])  # eager
+        torch.cuda.synchronize()
+        for a, b in zip(got, want[i]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,v,top", [(1, 9, 3), (3, 2049, 128),
+                                        (5, 50001, 20), (1030, 333, 0)])
+def test_kernels_write_their_results_alone(lm, rows, v, top):
+    """The entry points that the wrappers call, into buffers with edges."""
+    torch, hiplm = lm
+    import hiptorch
+
+    ext = hiptorch.ensure_hiplm()
+    stream = torch.cuda.current_stream().cuda_stream
+    edge, kept = 4096, []
+
+    def buffer(size):
+        b = torch.full((2 * edge + size,), 0xA5, dtype=torch.uint8,
+                       device="cuda")
+        kept.append((b, size))
+        return b.data_ptr() + edge
+
+    x = torch.randn(rows, v, device="cuda").bfloat16()
+    tokens = torch.randint(v, (rows,), device="cuda")
+    stats, g = buffer(16 * rows), torch.ones(rows, device="cuda")
+    ext.token_logprobs(1, x.data_ptr(), v, rows, v, tokens.data_ptr(), -100,
+                       1.0, top, buffer(4 * rows), buffer(4 * rows),
+                       buffer(4 * rows * top), buffer(8 * rows * top), stats,
+                       buffer(ext.score_workspace(1, rows, v, top)), stream)
+    dx = buffer(2 * rows * v)
+    ext.token_logprobs_bwd(1, x.data_ptr(), v, rows, v, tokens.data_ptr(), 1.0,
+                           stats, g.data_ptr(), 0, dx, stream)
+    k = 7
+    teacher = torch.randn(rows, k, device="cuda")
+    ids = torch.randint(v, (rows, k), device="cuda")
+    q, total = buffer(4 * rows * k), buffer(8)
+    ext.distill(1, x.data_ptr(), v, rows, v, 0, teacher.data_ptr(),
+                ids.data_ptr(), k, 1.0, buffer(4 * rows), q, stats, total,
+                True, buffer(ext.score_workspace(1, rows, v, 0)), stream)
+    ext.distill_bwd(1, x.data_ptr(), v, rows, v, ids.data_ptr(), q, k, 1.0,
+                    stats, g.data_ptr(), 0, total + 4, buffer(2 * rows * v),
+                    stream)
+    torch.cuda.synchronize()
+    for b, size in kept:
+        assert (b[:edge] == 0xA5).all() and (b[edge + size:] == 0xA5).all()
+
+
+def test_on_another_stream(lm):
+    torch, hiplm = lm
+    x = torch.randn(40, 3001, device="cuda", requires_grad=True)
+    tokens = torch.randint(3001, (40,), device="cuda")
+
+    def step():
+        r = hiplm.token_logprobs(x, tokens, top=5)
+        return [*r, *torch.autograd.grad(r.logprobs.sum(), [x])]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_a_head_records_and_a_student_learns(lm):
+    """The operators in a row, as they would be used."""
+    torch, hiplm = lm
+    import hipmx
+    import lm_oracle as oracle
+
+    g = torch.Generator().manual_seed(4)
+    hidden, vocab, rows = 512, 5003, 70
+    head = hipmx.quantize((torch.randn(vocab, hidden, generator=g) * 0.2)
+                          .bfloat16().cuda())
+    x = torch.randn(rows, hidden, generator=g).bfloat16().cuda()
+    with torch.no_grad():
+        logits = torch.nn.functional.linear(x, head)
+    said = check_logprobs(torch, hiplm, logits, logits.argmax(-1), 16, 1.0)
+    student = torch.randn(rows, vocab, generator=g).cuda().requires_grad_(True)
+    loss = hiplm.topk_distill_loss(student, said.top_logprobs,
+                                   said.top_tokens)
+    (got,) = torch.autograd.grad(loss, [student])
+    want, grad, size = oracle.distill(
+        host(student), host(said.top_logprobs),
+        host(said.top_tokens).astype(np.int64), 1.0, "mean")
+    near(loss, want, 64 * relative(vocab))
+    check_grad(torch, got, grad, size, vocab, "float32")
+    # a student that says what the teacher says loses nothing
+    same = hiplm.topk_distill_loss(
+        torch.full((rows, vocab), -INF).cuda().scatter(
+            1, said.top_tokens, said.top_logprobs),
+        said.top_logprobs, said.top_tokens)
+    assert abs(same.item()) < 64 * relative(vocab)

@@ -1,0 +1,317 @@
+"""GPU tests of microscaled 4-bit quantisation and product (ops/hipmx.py).
+
+The kernels' codes have to be those of the definition, bit for bit. Products
+of codes are exact in float32, so a result is off by what its sum in float32
+and its one rounding cost.
+"""
+
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+OPS_DIR = Path(__file__).resolve().parent.parent / "code_interpreter_amd" / "ops"
+sys.path.insert(0, str(OPS_DIR))
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "bfloat16", "float16"]
+
+
+@pytest.fixture(scope="module")
+def mx():
+    torch = pytest.importorskip("torch")
+    if not torch.cuda.is_available():
+        pytest.skip("torch sees no GPU")
+    import hipmx
+
+    return torch, hipmx
+
+
+def values(torch, q):
+    """What codes stand for, in 64 bits, on the host."""
+    import lm_oracle as oracle
+
+    return oracle.values(q.codes.cpu().numpy(), q.scales.cpu().numpy(),
+                         q.shape[-1])
+
+
+def same_codes(torch, hipmx, x):
+    """The kernel's codes of x against those of the plain form on the host,
+    which is tested against the definition element by element."""
+    q, want = hipmx.quantize(x), hipmx.quantize(x.cpu())
+    assert torch.equal(q.scales.cpu(), want.scales)
+    # a negative number that rounds to 0 may keep its sign or not
+    a, b = q.codes.cpu(), want.codes
+    for shift in (0, 4):
+        p, r = (a >> shift) & 15, (b >> shift) & 15
+        assert torch.equal(torch.where(p == 8, 0, p), torch.where(r == 8, 0, r))
+    return q
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 32), (3, 31), (5, 33),
+                                   (7, 100), (64, 4096), (333, 1000),
+                                   (2, 3, 65), (70000, 8)])
+def test_quantize_codes(mx, dtype, shape):
+    torch, hipmx = mx
+    g = torch.Generator().manual_seed(sum(shape))
+    x = torch.randn(*shape, generator=g) * torch.exp(
+        4 * torch.randn(*shape, generator=g))
+    x = x.clamp(-6e4, 6e4).to(getattr(torch, dtype)).cuda()
+    q = same_codes(torch, hipmx, x)
+    for out in DTYPES:
+        v = q.dequantize(getattr(torch, out))
+        want = torch.from_numpy(values(torch, q)).to(getattr(torch, out))
+        assert torch.equal(v.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_every_16_bit_pattern(mx, dtype):
+    torch, hipmx = mx
+    bits = torch.arange(65536, dtype=torch.int32)
+    if dtype == "float32":
+        x = (bits << 16).view(torch.float32)
+    else:
+        x = torch.where(bits > 32767, bits - 65536, bits).to(
+            torch.int16).view(getattr(torch, dtype))
+    g = torch.Generator().manual_seed(5)
+    # in order (blocks of near values) and mixed (blocks of far ones, most
+    # with a NaN among them), and mixed without NaN
+    fine = x[torch.isfinite(x.float())]
+    for t in (x, x[torch.randperm(65536, generator=g)],
+              fine[torch.randperm(fine.numel(), generator=g)]):
+        same_codes(torch, hipmx, t.reshape(1, -1).cuda())
+
+
+def test_quantize_strided(mx):
+    torch, hipmx = mx
+    base = torch.randn(40, 200, device="cuda", dtype=torch.bfloat16)
+    for x in (base[:, 3:103], base[::3], base.t(), base[:, ::2], base[5:6],
+              base[0].expand(4, 200), base[:, 7]):
+        same_codes(torch, hipmx, x)
+
+
+def test_empty(mx):
+    torch, hipmx = mx
+    q = hipmx.quantize(torch.zeros(0, 40, device="cuda"))
+    assert q.dequantize().shape == (0, 40)
+    w = hipmx.quantize(torch.randn(5, 40, device="cuda"))
+    assert hipmx.linear(torch.zeros(2, 0, 40, device="cuda"), w).shape == (2, 0, 5)
+
+
+def operands(torch, hipmx, m, n, k, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp(
+        torch.randn(1, k, generator=g))
+    w = torch.randn(n, k, generator=g) * 0.05
+    bias = torch.randn(n, generator=g)
+    dt = getattr(torch, dtype)
+    return (x.to(dt).cuda(), hipmx.quantize(w.cuda()), bias.to(dt).cuda())
+
+
+def check_linear(torch, hipmx, y, x, w, bias):
+    """y against the product of the values in 64 bits. In float32 a sum of k
+    products in any order is off by at most k 2^-24 of the sum of their
+    magnitudes; the result is off by half a step more."""
+    q = x if isinstance(x, hipmx.MXFP4Tensor) else hipmx.quantize(x)
+    a = torch.from_numpy(values(torch, q)).cuda()
+    b = torch.from_numpy(values(torch, w)).cuda()
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    k = a.shape[-1]
+    info = torch.finfo(y.dtype)
+    slack = ((k + 2) * 2.0 ** -24 * size * (1 + info.eps)
+             + info.eps / 2 * want.abs() + info.smallest_normal * info.eps)
+    err = (y.double() - want).abs()
+    assert (err <= slack).all(), (err - slack).max().item()
+
+
+SHAPES = [
+    (1, 1, 1), (1, 16, 32), (1, 17, 33), (1, 512, 4096), (2, 100, 2056),
+    (15, 64, 512), (16, 64, 544), (17, 65, 1000), (33, 48, 96), (48, 33, 64),
+    (49, 128, 16384), (64, 1000, 777), (64, 16, 8192), (65, 64, 32),
+    (65, 200, 1056), (127, 129, 255), (128, 128, 256), (129, 300, 300),
+    (300, 257, 480), (1000, 96, 2048), (513, 4097, 288), (2049, 2050, 520),
+]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear(mx, m, n, k, dtype):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, n, k, dtype, m + n + k)
+    y = hipmx.linear(x, w, bias)
+    assert y.shape == (m, n) and y.dtype == x.dtype
+    check_linear(torch, hipmx, y, x, w, bias)
+    check_linear(torch, hipmx, hipmx.linear(x, w), x, w, None)
+    # an operand that comes quantised gives the same sums
+    p = hipmx.linear(hipmx.quantize(x), w, bias, dtype=x.dtype)
+    check_linear(torch, hipmx, p, x, w, bias)
+    # and the same call the same bits
+    assert torch.equal(hipmx.linear(x, w, bias), y)
+
+
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 512), (4100, 4200, 264),
+                                   (256, 16384, 1024)])
+def test_linear_large(mx, m, n, k):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, n, k, "bfloat16", 1)
+    check_linear(torch, hipmx, hipmx.linear(x, w, bias), x, w, bias)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_tells_rows_and_columns_apart(mx, m):
+    torch, hipmx = mx
+    # a weight of one element a row, each of another size and place
+    n = k = 320
+    w = torch.zeros(n, k, device="cuda")
+    at = (torch.arange(n, device="cuda") * 7) % k
+    w[torch.arange(n), at] = 2.0 ** (torch.arange(n, device="cuda") % 9 - 4)
+    x = torch.zeros(m, k, device="cuda")
+    x[torch.arange(m), (torch.arange(m) * 11) % k] = 3.0
+    y = hipmx.linear(x, hipmx.quantize(w))
+    assert torch.equal(y, (x.double() @ w.double().T).float())
+
+
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_linear_nan_stays_in_its_row(mx, m):
+    torch, hipmx = mx
+    x, w, _ = operands(torch, hipmx, m, 100, 96, "float32")
+    x[m // 2, 40] = float("inf")
+    y = hipmx.linear(x, w)
+    bad = y.isnan()
+    assert bad[m // 2].all() and bad.sum() == 100
+    w.scales[7, 2] = 255
+    x[m // 2, 40] = 0.0
+    bad = hipmx.linear(x, w).isnan()
+    assert bad[:, 7].all() and bad.sum() == m
+
+
+@pytest.mark.parametrize("m", [1, 24, 200])
+def test_linear_scales_at_the_ends(mx, m):
+    torch, hipmx = mx
+    # large weights against small activations: the products are ordinary
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randn(m, 128, generator=g) * 2.0 ** -100).cuda()
+    w = hipmx.quantize((torch.randn(70, 128, generator=g) * 2.0 ** 100).cuda())
+    y = hipmx.linear(x, w)
+    check_linear(torch, hipmx, y, x, w, None)
+    assert hipmx.linear(torch.zeros_like(x), w).abs().max() == 0
+
+
+def test_linear_inputs_of_other_strides(mx):
+    torch, hipmx = mx
+    base = torch.randn(90, 400, device="cuda", dtype=torch.bfloat16)
+    w = hipmx.quantize(torch.randn(50, 90, device="cuda"))
+    for x in (base.t(), base.t()[:3], base.t()[::7], base.t()[3]):
+        y = hipmx.linear(x, w)
+        assert torch.equal(y, hipmx.linear(x.contiguous(), w))
+    wide = torch.randn(30, 200, device="cuda")
+    for x in (wide[:, 5:95], wide[:2, 1:91]):
+        assert torch.equal(hipmx.linear(x, w),
+                           hipmx.linear(x.contiguous(), w))
+    bias = torch.randn(100, device="cuda")[::2]
+    y = hipmx.linear(wide[:, :90], w, bias)
+    assert torch.equal(y, hipmx.linear(wide[:, :90], w, bias.contiguous()))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 5, 40), (3, 17, 64), (40, 37, 100),
+                                   (70, 37, 64), (129, 131, 288),
+                                   (4097, 4100, 32)])
+def test_linear_writes_its_results_alone(mx, m, n, k):
+    torch, hipmx = mx
+    import hiptorch
+
+    # the entry point that the wrapper calls, into the middle of a buffer
+    ext = hiptorch.ensure_hiplm()
+    x, w, _ = operands(torch, hipmx, m, n, k, "bfloat16")
+    edge = 4096
+    out = torch.full((edge + m * n + edge,), 7.0, dtype=torch.bfloat16,
+                     device="cuda")
+    need = ext.mx_linear_workspace(m, n, k, False)
+    work = torch.full((edge + need + edge,), 9, dtype=torch.uint8,
+                      device="cuda")
+    ext.mx_linear(1, x.data_ptr(), k, 0, 0, w.codes.data_ptr(),
+                  w.scales.data_ptr(), 0, out.data_ptr() + 2 * edge, m, n, k,
+                  work.data_ptr() + edge, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    y = out[edge:edge + m * n].view(m, n)
+    assert torch.equal(y, hipmx.linear(x, w))
+    assert (out[:edge] == 7).all() and (out[edge + m * n:] == 7).all()
+    assert (work[:edge] == 9).all() and (work[edge + need:] == 9).all()
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 200])
+def test_linear_in_a_graph(mx, m):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, 300, 16384, "bfloat16")
+    other = operands(torch, hipmx, m, 300, 16384, "bfloat16", 9)[0]
+    want = [hipmx.linear(t, w, bias) for t in (x, other)]
+    still = x.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hipmx.linear(still, w, bias)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):  # two graphs, alive together
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = hipmx.linear(still, w, bias)
+        graphs.append((g, y))
+    for i in (0, 1, 0, 1):
+        still.copy_((x, other)[i])
+        for g, _ in graphs:
+            g.replay()
+        hipmx.linear(other, w, bias)  # eager work in between
+        torch.cuda.synchronize()
+        for _, y in graphs:
+            assert torch.equal(y, want[i])
+
+
+def test_linear_on_another_stream(mx):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, 130, 300, 512, "bfloat16")
+    want = hipmx.linear(x, w, bias)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = hipmx.linear(x, w, bias)
+        b = hipmx.linear(a[:, :256], hipmx.quantize(a[:40, :256]))
+    side.synchronize()
+    assert torch.equal(a, want)
+    c = hipmx.linear(want[:, :256], hipmx.quantize(want[:40, :256]))
+    assert torch.equal(b, c)
+
+
+def test_torch_linear_dispatches(mx):
+    torch, hipmx = mx
+    import hiptorch
+
+    x, w, bias = operands(torch, hipmx, 5, 64, 96, "bfloat16")
+    want = hipmx.linear(x, w, bias)
+    before = hipmx.STATS["linear"]
+    assert torch.equal(torch.nn.functional.linear(x, w, bias), want)
+    assert hiptorch.install(mode="require")
+    try:
+        assert torch.equal(torch.nn.functional.linear(x, w, bias), want)
+    finally:
+        hiptorch.uninstall()
+    assert hipmx.STATS["linear"] == before + 2
+
+
+def test_mixed_devices_are_refused(mx):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, 5, 64, 96, "bfloat16")
+    with pytest.raises(ValueError, match="weight on"):
+        hipmx.linear(x.cpu(), w)
+    with pytest.raises(ValueError, match="bias must be"):
+        hipmx.linear(x, w, bias.cpu())
+    with pytest.raises(ValueError, match="different devices"):
+        hipmx.MXFP4Tensor(w.codes, w.scales.cpu(), 96)
+    moved = w.to("cpu")
+    assert torch.equal(moved.dequantize(), w.dequantize().cpu())
