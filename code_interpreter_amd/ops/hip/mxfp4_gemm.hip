@@ -43,14 +43,19 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* row, int at,
   return s;
 }
 
+template <LmType T>
+struct Out {
+  using type = typename std::conditional<
+      T == LmType::F32, float,
+      typename std::conditional<T == LmType::BF16, __bf16, _Float16>::type>::
+      type;
+};
+
 // outputs n .. n + 3 of a row
 template <LmType T>
 __device__ __forceinline__ void store4(void* y, int64_t at, const float* f,
                                        int valid) {
-  using E = typename std::conditional<
-      T == LmType::F32, float,
-      typename std::conditional<T == LmType::BF16, __bf16, _Float16>::type>::
-      type;
+  using E = typename Out<T>::type;
   using E4 = E __attribute__((ext_vector_type(4)));
   E* p = (E*)y + at;
   if (valid >= 4) {
@@ -73,24 +78,98 @@ __device__ __forceinline__ float bias_at(const void* bias, int64_t i) {
 // ---------------------------------------------------------------------------
 // tiles: many tokens
 // ---------------------------------------------------------------------------
+// Before the product, one launch quantises the tokens and lays out both
+// operands' scales by steps of 256 elements of k: [step][row][8], 1 behind a
+// row's end. Rows' scales for a step are then neighbours in memory, where in
+// a row's own order a wave would touch a cache line for every row.
+constexpr int kPrepareThreads = 256;
+constexpr int kPrepareRows = 32;  // of a block that quantises one step
+constexpr int kLayRows = kPrepareThreads, kLaySteps = 8;  // of one that does not
+
+__device__ __forceinline__ void lay_out_scales(const uint8_t* from,
+                                               uint2* to, int64_t rows,
+                                               int nb, int steps, int blk) {
+  const int parts = (steps + kLaySteps - 1) / kLaySteps;
+  const int64_t row = (int64_t)(blk / parts) * kLayRows + threadIdx.x;
+  const int t0 = blk % parts * kLaySteps;
+  if (row >= rows) return;
+  const uint8_t* p = from + row * nb;
+  for (int t = t0; t < min(steps, t0 + kLaySteps); t++)
+    to[t * rows + row] = {load_scales(p, t * 8, nb),
+                          load_scales(p, t * 8 + 4, nb)};
+}
+
+// blocks [0, x_blocks): x to codes and laid out scales, or (packed) its
+// scales laid out; the others: the weight's scales laid out. A quantising
+// block takes 32 rows of one step, so that its scales are 256 bytes in order.
+template <LmType T, bool kPacked>
+__global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
+    const char* __restrict__ x, int64_t stride,
+    const uint8_t* __restrict__ xs, uint32_t* __restrict__ codes,
+    uint8_t* __restrict__ xst, int64_t m, int64_t k, int x_blocks,
+    const uint8_t* __restrict__ ws, uint2* __restrict__ wst, int64_t n,
+    int nb, int steps) {
+  if ((int)blockIdx.x >= x_blocks) {
+    lay_out_scales(ws, wst, n, nb, steps, blockIdx.x - x_blocks);
+    return;
+  }
+  if constexpr (kPacked) {
+    lay_out_scales(xs, (uint2*)xst, m, nb, steps, blockIdx.x);
+  } else {
+    constexpr int kGroups = kPrepareRows * 32 / kPrepareThreads;
+    const int t = blockIdx.x % steps;
+    const int64_t row0 = (int64_t)(blockIdx.x / steps) * kPrepareRows +
+                         (threadIdx.x >> 5);
+    const int col = threadIdx.x & 31;  // of the step's groups of 8 elements
+    const int blk = t * 8 + (col >> 2);
+    u32x4 w[kGroups], w2[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; i++) {
+      const int64_t row = row0 + i * (kPrepareThreads / 32);
+      if (row < m)
+        load8<T>(x + row * stride * Size<T>::value,
+                 (int64_t)t * 256 + col * kPer, k, w[i], w2[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kGroups; i++) {
+      const int64_t row = row0 + i * (kPrepareThreads / 32);
+      if (row >= m) break;
+      uint32_t byte = block_scale<T>(w[i], w2[i]);
+      if (blk < nb)
+        codes[(row * nb + t * 8) * 4 + col] =
+            byte == 255 ? 0u : encode<T>(w[i], w2[i], scale_value(byte));
+      if ((col & 3) == 0)
+        xst[(t * m + row) * 8 + (col >> 2)] =
+            blk < nb ? (uint8_t)byte : 0x7F;
+    }
+  }
+}
+
 // A block of WM x WN waves makes BM tokens x BN outputs; a wave FM x FN
 // tiles of 32 x 32. A step takes 256 elements of k, 128 bytes of a row, into
 // one of two buffers of shared memory by asynchronous loads of 16 bytes a
-// lane, while the other one is read. In shared memory the 8 units of 16
-// bytes of row r stand at their index ^ (r & 7), so that 8 lanes that read
-// the same unit of 8 rows touch all of the banks once.
+// lane. In shared memory the 8 units of 16 bytes of row r stand at their
+// index ^ (r / 2 & 7), so that 16 lanes that read the same unit of 16 rows
+// touch all of the 64 banks once.
+//
+// A step is 4 instructions deep in k. While the matrix units work on one of
+// them the next one's operands are read; the last one's time covers the
+// barrier, the first reads of the next step's buffer and the start of the
+// loads of the one after.
 template <LmType T, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(WM* WN * 64) void tile_kernel(
-    const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs,
-    const uint8_t* __restrict__ wc, const uint8_t* __restrict__ ws,
+__global__ __launch_bounds__(WM* WN * 64, 1) void tile_kernel(
+    const uint8_t* __restrict__ xc, const uint2* __restrict__ xs,
+    const uint8_t* __restrict__ wc, const uint2* __restrict__ ws,
     const void* __restrict__ bias, void* __restrict__ y, int64_t m, int64_t n,
     int nb, int tiles_m, int tiles_n) {
+#ifdef __HIP_DEVICE_COMPILE__  // buffer descriptors are no type on the host
   constexpr int kWaves = WM * WN;
   constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
   constexpr int kRow = 128;
   constexpr int kBuf = (BM + BN) * kRow;
   constexpr int kLoadsX = BM / 8 / kWaves, kLoadsW = BN / 8 / kWaves;
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "");
+  static_assert(kWaves % 2 == 0, "");
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   // A chiplet gets every eighth block; it is given neighbouring tiles, in
@@ -115,135 +194,240 @@ __global__ __launch_bounds__(WM* WN * 64) void tile_kernel(
   // a row behind it is not stored
   const uint8_t* xb = xc + m0 * row_bytes;
   const uint8_t* wb = wc + n0 * row_bytes;
+  const int unit = (lane & 7) ^ (((wave & 1) * 4 + (lane >> 4)) & 7);
   uint32_t xo[kLoadsX], wo[kLoadsW];
 #pragma unroll
   for (int i = 0; i < kLoadsX; i++) {
     int64_t r = (i * kWaves + wave) * 8 + (lane >> 3);
-    xo[i] = (uint32_t)(min(r, m - 1 - m0) * row_bytes);
+    xo[i] = (uint32_t)(min(r, m - 1 - m0) * row_bytes) + unit * 16;
   }
 #pragma unroll
   for (int i = 0; i < kLoadsW; i++) {
     int64_t r = (i * kWaves + wave) * 8 + (lane >> 3);
-    wo[i] = (uint32_t)(min(r, n - 1 - n0) * row_bytes);
+    wo[i] = (uint32_t)(min(r, n - 1 - n0) * row_bytes) + unit * 16;
   }
-  const int unit = (lane & 7) ^ (lane >> 3);
-  const int steps = (nb + 7) / 8;
-  const int rest = nb - (steps - 1) * 8;  // blocks of the last step, 1 to 8
+  const int full = nb / 8, rest = nb % 8;  // steps; blocks behind them
+  const int steps = full + (rest != 0);
+  // in the last, short step a unit behind the row's end is read as its last
+  const int back = rest && unit >= rest ? (unit - rest + 1) * 16 : 0;
 
-  auto stage = [&](int t) {
-    char* to = smem + (t & 1) * kBuf + wave * 1024;
-    const uint32_t u =
-        (uint32_t)(t == steps - 1 ? min(unit, rest - 1) : unit) * 16;
-    const uint8_t* xt = xb + (int64_t)t * kRow;
-    const uint8_t* wt = wb + (int64_t)t * kRow;
-#pragma unroll
-    for (int i = 0; i < kLoadsW; i++)
-      __builtin_amdgcn_global_load_lds((global_void*)(wt + wo[i] + u),
-                                       (lds_void*)(to + i * kWaves * 1024),
-                                       16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kLoadsX; i++)
-      __builtin_amdgcn_global_load_lds(
-          (global_void*)(xt + xo[i] + u),
-          (lds_void*)(to + BN * kRow + i * kWaves * 1024), 16, 0, 0);
+  // The tile's rows as buffers: an asynchronous load is then one instruction,
+  // with the row in a register of the lane and the step in a scalar one.
+  auto buffer = [](const void* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void*)p, 0, (int)min(bytes, (int64_t)0xFFFFFFFF), 0x00020000);
+  };
+  const auto xr = buffer(xb, min(m - m0, (int64_t)BM) * row_bytes);
+  const auto wr = buffer(wb, min(n - n0, (int64_t)BN) * row_bytes);
+  // step t into buffer `into`
+  auto load = [&](int t, int into, auto rsrc, uint32_t at, int to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rsrc, (lds_void*)(smem + into * kBuf + to + wave * 1024), 16,
+        (int)at - (t == full ? back : 0), t * kRow, 0, 0);
+  };
+  auto load_w = [&](int t, int into, int i) {
+    load(t, into, wr, wo[i], i * kWaves * 1024);
+  };
+  auto load_x = [&](int t, int into, int i) {
+    load(t, into, xr, xo[i], BN * kRow + i * kWaves * 1024);
   };
 
-  const uint8_t* xsr[FM];
-  const uint8_t* wsr[FN];
+  // scales: the lower lanes take a step's blocks 0 to 3, the upper 4 to 7
+  uint32_t xso[FM], wso[FN];
 #pragma unroll
   for (int i = 0; i < FM; i++)
-    xsr[i] = xs + min(m0 + (wm * FM + i) * 32 + l31, m - 1) * nb;
+    xso[i] = (uint32_t)(min((int64_t)(wm * FM + i) * 32 + l31, m - 1 - m0) * 8) +
+             4 * h;
 #pragma unroll
   for (int i = 0; i < FN; i++)
-    wsr[i] = ws + min(n0 + (wn * FN + i) * 32 + l31, n - 1) * nb;
-
-  v16f acc[FN][FM] = {};
+    wso[i] = (uint32_t)(min((int64_t)(wn * FN + i) * 32 + l31, n - 1 - n0) * 8) +
+             4 * h;
   uint32_t sx[FM], sw[FN];
-  auto scales = [&](int t, uint32_t* dx, uint32_t* dw) {
-#pragma unroll
-    for (int i = 0; i < FM; i++) dx[i] = load_scales(xsr[i], t * 8 + 4 * h, nb);
-#pragma unroll
-    for (int i = 0; i < FN; i++) dw[i] = load_scales(wsr[i], t * 8 + 4 * h, nb);
+  auto scale_x = [&](int t, int i) {
+    return *(const uint32_t*)((const char*)(xs + (int64_t)t * m + m0) +
+                              xso[i]);
+  };
+  auto scale_w = [&](int t, int i) {
+    return *(const uint32_t*)((const char*)(ws + (int64_t)t * n + n0) +
+                              wso[i]);
   };
 
-  // Instruction s multiplies blocks s (lower lanes) and 4 + s (upper ones)
-  // of the step. Behind the row's end codes and scales are made 0 and 1.
-  auto multiply = [&](int t, auto last) {
+  v16f acc[FN][FM] = {};
+  struct Operands {
+    u32x4 w[FN], x[FM];
+  };
+  // what instruction s of a step takes: blocks s (lower lanes) and 4 + s
+  const int at0 = (wn * FN * 32 + l31) * kRow;
+  const int at1 = (BN + wm * FM * 32 + l31) * kRow;
+  // operand i of them: FN of the weights, then FM of the tokens
+  auto read = [&](int t, int s, int i, Operands& o) {
     const char* from = smem + (t & 1) * kBuf;
-    auto one = [&](auto step) {
+    const int u = ((s + 4 * h) ^ (lane >> 1 & 7)) * 16;
+    if (i < FN)
+      o.w[i] = *(const u32x4*)(from + at0 + i * 32 * kRow + u);
+    else
+      o.x[i - FN] = *(const u32x4*)(from + at1 + (i - FN) * 32 * kRow + u);
+  };
+  auto product = [&](auto step, const Operands& o, int i, int j) {
+    constexpr int s = decltype(step)::value;
+    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+        operand(o.w[i]), operand(o.x[j]), acc[i][j], 4, 4, s, (int)sw[i], s,
+        (int)sx[j]);
+  };
+
+  // all of this wave's loads have landed, and its reads are done
+  auto settle = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  std::integral_constant<int, 0> s0;
+  std::integral_constant<int, 1> s1;
+  std::integral_constant<int, 2> s2;
+  std::integral_constant<int, 3> s3;
+
+  // The products of one instruction's depth, with `between(slot)` behind
+  // each: what is read and loaded for later then goes out piece by piece
+  // while the matrix units work, instead of holding up the products. The
+  // compiler would gather it; the barriers for its scheduler keep the order.
+  constexpr int kSlots = FN * FM;
+  auto multiply = [&](auto step, const Operands& o, auto between) {
+#pragma unroll
+    for (int slot = 0; slot < kSlots; slot++) {
+      product(step, o, slot / FM, slot % FM);
+      __builtin_amdgcn_sched_barrier(0);
+      between(slot);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // piece by piece: those of `count` that fall to this of the slots
+  auto spread = [](int slot, int count, auto piece) {
+#pragma unroll
+    for (int i = 0; i < count; i++)
+      if (i * kSlots / count == slot) piece(i);
+  };
+  // operands are read early in a part, one a slot
+  constexpr int kReads = FN + FM;
+  auto read_early = [&](int slot, int t, int s, Operands& o) {
+#pragma unroll
+    for (int i = 0; i < kReads; i++)
+      if (i * kSlots / (2 * kReads) == slot) read(t, s, i, o);
+  };
+
+  // Step t's tokens and step t + 1's weights are under way while step t - 1
+  // is worked on.
+#pragma unroll
+  for (int i = 0; i < kLoadsW; i++) load_w(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < kLoadsX; i++) load_x(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < FM; i++) sx[i] = scale_x(0, i);
+#pragma unroll
+  for (int i = 0; i < FN; i++) sw[i] = scale_w(0, i);
+  settle();
+#pragma unroll
+  for (int i = 0; i < kLoadsW; i++) load_w(min(1, steps - 1), 1, i);
+  Operands a, b;
+#pragma unroll
+  for (int i = 0; i < kReads; i++) read(0, 0, i, a);
+  for (int t = 0; t < full; t++) {
+    // No branches in here, which the compiler would gather the products
+    // behind: where there is no next step, or none after it, the last one is
+    // read and loaded again, into a buffer that is free.
+    const int ahead = min(t + 1, steps - 1), next = min(t + 2, steps - 1);
+    uint32_t nx[FM], nw[FN];
+    multiply(s0, a, [&](int slot) {
+      read_early(slot, t, 1, b);
+      spread(slot, kLoadsX, [&](int i) { load_x(ahead, (t + 1) & 1, i); });
+    });
+    multiply(s1, b, [&](int slot) {
+      read_early(slot, t, 2, a);
+      spread(slot, FM, [&](int i) { nx[i] = scale_x(ahead, i); });
+      spread(slot, FN, [&](int i) { nw[i] = scale_w(ahead, i); });
+    });
+    multiply(s2, a, [&](int slot) { read_early(slot, t, 3, b); });
+    settle();  // every wave's part of step t + 1 is there, step t is read
+    multiply(s3, b, [&](int slot) {
+      read_early(slot, t + 1, 0, a);
+      spread(slot, kLoadsW, [&](int i) { load_w(next, t & 1, i); });
+    });
+#pragma unroll
+    for (int i = 0; i < FM; i++) sx[i] = nx[i];
+#pragma unroll
+    for (int i = 0; i < FN; i++) sw[i] = nw[i];
+  }
+  if (rest) {  // codes behind the row's end are made 0; their scales are 1
+    // where there was no whole step, the tokens' part has landed in settle()
+    auto last = [&](auto step) {
       constexpr int s = decltype(step)::value;
-      if (decltype(last)::value && s >= rest) return;
-      const int at = ((s + 4 * h) ^ (lane & 7)) * 16 + l31 * kRow;
-      const bool in = !decltype(last)::value || s + 4 * h < rest;
-      v8i a[FN], b[FM];
+      if (s >= rest) return;
+      const bool in = s + 4 * h < rest;
 #pragma unroll
-      for (int i = 0; i < FN; i++) {
-        u32x4 w = *(const u32x4*)(from + (wn * FN + i) * 32 * kRow + at);
-        a[i] = operand(in ? w : u32x4{0, 0, 0, 0});
-      }
-#pragma unroll
-      for (int i = 0; i < FM; i++) {
-        u32x4 w =
-            *(const u32x4*)(from + (BN + (wm * FM + i) * 32) * kRow + at);
-        b[i] = operand(in ? w : u32x4{0, 0, 0, 0});
+      for (int i = 0; i < kReads; i++) {
+        read(full, s, i, a);
+        u32x4& w = i < FN ? a.w[i] : a.x[i - FN];
+        w = in ? w : u32x4{0, 0, 0, 0};
       }
 #pragma unroll
       for (int i = 0; i < FN; i++)
 #pragma unroll
-        for (int j = 0; j < FM; j++)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              a[i], b[j], acc[i][j], 4, 4, s, (int)sw[i], s, (int)sx[j]);
+        for (int j = 0; j < FM; j++) product(step, a, i, j);
     };
-    one(std::integral_constant<int, 0>{});
-    one(std::integral_constant<int, 1>{});
-    one(std::integral_constant<int, 2>{});
-    one(std::integral_constant<int, 3>{});
-  };
-
-  stage(0);
-  scales(0, sx, sw);
-  for (int t = 0; t < steps; t++) {
-    // this wave's loads of step t have landed; then every wave's have, and
-    // every wave is through with step t - 1, whose buffer is filled next
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    uint32_t nx[FM], nw[FN];
-    if (t + 1 < steps) {
-      stage(t + 1);
-      scales(t + 1, nx, nw);
-      multiply(t, std::false_type{});
-#pragma unroll
-      for (int i = 0; i < FM; i++) sx[i] = nx[i];
-#pragma unroll
-      for (int i = 0; i < FN; i++) sw[i] = nw[i];
-    } else if (rest == 8) {
-      multiply(t, std::false_type{});
-    } else {
-      multiply(t, std::true_type{});
-    }
+    last(s0);
+    last(s1);
+    last(s2);
+    last(s3);
   }
 
+  // A lane holds 4 neighbouring outputs of one token at a time: stored from
+  // there, rows would go out in pieces of 8 or 16 bytes. They pass through
+  // shared memory, 32 tokens of a wave at a time, and go out 16 bytes a lane
+  // along the rows.
+  using E = typename Out<T>::type;
+  using E4 = E __attribute__((ext_vector_type(4)));
+  constexpr int kOutRow = FN * 32 * (int)sizeof(E);
+  constexpr int kPad = kOutRow + 16;
+  constexpr int kLanes = kOutRow / 16;  // of a row
+  constexpr int kPer16 = 16 / (int)sizeof(E);
+  static_assert(kWaves * 32 * kPad + BN * 4 <= 2 * kBuf, "");
+  float* sb = (float*)smem;
+  char* out = smem + BN * 4 + wave * 32 * kPad;
+  settle();
+  for (int i = threadIdx.x; i < BN; i += kWaves * 64)
+    sb[i] = bias && n0 + i < n ? bias_at<T>(bias, n0 + i) : 0.f;
+  __syncthreads();
+  const int col = (lane % kLanes) * kPer16;
+  const int64_t c0 = n0 + wn * FN * 32 + col;
 #pragma unroll
-  for (int i = 0; i < FN; i++)
+  for (int j = 0; j < FM; j++) {
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int64_t col = n0 + (wn * FN + i) * 32 + 8 * g + 4 * h;
-      const int valid = (int)min((int64_t)4, n - col);
-      if (valid <= 0) continue;
-      float add[4] = {};
-      if (bias)
-        for (int r = 0; r < 4; r++)
-          if (r < valid) add[r] = bias_at<T>(bias, col + r);
+    for (int i = 0; i < FN; i++)
 #pragma unroll
-      for (int j = 0; j < FM; j++) {
-        const int64_t row = m0 + (wm * FM + j) * 32 + l31;
-        if (row >= m) continue;
-        float f[4];
+      for (int g = 0; g < 4; g++) {
+        const int at = i * 32 + 8 * g + 4 * h;
+        const v4f add = *(const v4f*)(sb + wn * FN * 32 + at);
+        E4 v;
 #pragma unroll
-        for (int r = 0; r < 4; r++) f[r] = acc[i][j][4 * g + r] + add[r];
-        store4<T>(y, row * n + col, f, valid);
+        for (int r = 0; r < 4; r++) v[r] = (E)(acc[i][j][4 * g + r] + add[r]);
+        *(E4*)(out + l31 * kPad + at * (int)sizeof(E)) = v;
+      }
+    const int64_t row0 = m0 + (wm * FM + j) * 32;
+#pragma unroll
+    for (int p = 0; p < 32; p += 64 / kLanes) {
+      const int r = p + lane / kLanes;
+      const u32x4 v = *(const u32x4*)(out + r * kPad + col * (int)sizeof(E));
+      if (row0 + r >= m) continue;
+      E* to = (E*)y + (row0 + r) * n + c0;
+      if (c0 + kPer16 <= n) {
+        *(raw16*)to = v;
+      } else {
+        const E* e = (const E*)(out + r * kPad) + col;
+        for (int q = 0; q < kPer16 && c0 + q < n; q++) to[q] = e[q];
       }
     }
+  }
+#endif
 }
 
 // ---------------------------------------------------------------------------
@@ -402,8 +586,8 @@ bool fuses(int64_t m, int64_t nb) {
 }
 
 template <LmType T, int WM, int WN, int FM, int FN>
-void run_tile(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
-              const uint8_t* ws, const void* bias, void* y, int64_t m,
+void run_tile(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
+              const uint2* ws, const void* bias, void* y, int64_t m,
               int64_t n, int nb, hipStream_t stream) {
   constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
   int64_t tm = (m + BM - 1) / BM, tn = (n + BN - 1) / BN;
@@ -415,6 +599,62 @@ void run_tile(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
   HIP_CHECK(hipGetLastError());
 }
 
+// what the tiles' workspace holds: x's codes, its scales by steps, the
+// weight's
+struct TileSpace {
+  int64_t codes, xs, ws;
+};
+
+int64_t round16(int64_t v) { return (v + 15) & ~(int64_t)15; }
+
+TileSpace tile_space(int64_t m, int64_t n, int64_t nb, bool packed) {
+  int64_t steps = (nb + 7) / 8;
+  return {packed ? 0 : m * nb * kMxBytes, round16(m * steps * 8),
+          n * steps * 8};
+}
+
+template <LmType T>
+void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
+               const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
+               const void* bias, void* y, int64_t m, int64_t n, int64_t k,
+               void* scratch, hipStream_t stream) {
+  const int64_t nb = mx_blocks(k), steps = (nb + 7) / 8;
+  TileSpace space = tile_space(m, n, nb, x == nullptr);
+  uint8_t* codes = (uint8_t*)scratch;
+  uint8_t* xst = codes + space.codes;
+  uint2* wst = (uint2*)(xst + space.xs);
+  auto lay_blocks = [&](int64_t rows) {
+    return (rows + kLayRows - 1) / kLayRows *
+           ((steps + kLaySteps - 1) / kLaySteps);
+  };
+  const int64_t w_blocks = lay_blocks(n);
+  const int64_t x_blocks =
+      x ? (m + kPrepareRows - 1) / kPrepareRows * steps : lay_blocks(m);
+  // a token tile's offsets into the codes are 32 bits
+  if (x_blocks + w_blocks >= (int64_t)1 << 31 || nb * kMxBytes >= 1 << 23)
+    throw std::runtime_error("product too large for one launch");
+  const dim3 grid((unsigned)(x_blocks + w_blocks));
+  if (x)
+    prepare_kernel<T, false><<<grid, kPrepareThreads, 0, stream>>>(
+        (const char*)x, stride, nullptr, (uint32_t*)codes, xst, m, k,
+        (int)x_blocks, ws, wst, n, (int)nb, (int)steps);
+  else
+    prepare_kernel<T, true><<<grid, kPrepareThreads, 0, stream>>>(
+        nullptr, 0, xs, nullptr, xst, m, k, (int)x_blocks, ws, wst, n,
+        (int)nb, (int)steps);
+  HIP_CHECK(hipGetLastError());
+  if (x) xc = codes;
+  auto* xs2 = (const uint2*)xst;
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
+  const int64_t mid = ((m + 127) / 128) * ((n + 127) / 128);
+  if (big >= 256)
+    run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
+  else if (mid >= 256)
+    run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
+  else
+    run_tile<T, 2, 2, 1, 1>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
+}
+
 template <LmType T>
 void run_linear(const void* x, int64_t stride, const uint8_t* xc,
                 const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
@@ -422,7 +662,7 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
                 void* scratch, hipStream_t stream) {
   const int64_t nb = mx_blocks(k);
   const bool fused = x && fuses(m, nb);
-  if (x && !fused) {
+  if (m <= kFewTokens && x && !fused) {
     uint8_t* codes = (uint8_t*)scratch;
     uint8_t* scales = codes + m * nb * kMxBytes;
     launch_mx_quantize(T, x, stride, codes, scales, m, k, stream);
@@ -457,19 +697,17 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
     fused ? by_mt(std::false_type{}) : by_mt(std::true_type{});
     return;
   }
-  if (((m + 255) / 256) * ((n + 255) / 256) >= 256)
-    run_tile<T, 2, 4, 4, 2>(xc, xs, wc, ws, bias, y, m, n, (int)nb, stream);
-  else if (((m + 127) / 128) * ((n + 127) / 128) >= 256)
-    run_tile<T, 2, 2, 2, 2>(xc, xs, wc, ws, bias, y, m, n, (int)nb, stream);
-  else
-    run_tile<T, 2, 2, 1, 1>(xc, xs, wc, ws, bias, y, m, n, (int)nb, stream);
+  run_tiles<T>(x, stride, xc, xs, wc, ws, bias, y, m, n, k, scratch, stream);
 }
 
 }  // namespace
 
-int64_t mx_linear_workspace(int64_t m, int64_t, int64_t k, bool packed) {
+int64_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, bool packed) {
   const int64_t nb = mx_blocks(k);
-  return packed || fuses(m, nb) ? 0 : m * nb * (kMxBytes + 1);
+  if (m <= kFewTokens)
+    return packed || fuses(m, nb) ? 0 : m * nb * (kMxBytes + 1);
+  TileSpace space = tile_space(m, n, nb, packed);
+  return space.codes + space.xs + space.ws;
 }
 
 void launch_mx_linear(LmType t, const void* x, int64_t stride,
