@@ -33,12 +33,56 @@ namespace {
     return nullptr;                                \
   }
 
-using ull = unsigned long long;
+// The arguments of a call in their order; the first that is not what is asked
+// for leaves an exception.
+class Args {
+ public:
+  Args(PyObject* const* args, Py_ssize_t n, Py_ssize_t want)
+      : args_(args), good_(n == want) {
+    if (!good_)
+      PyErr_Format(PyExc_TypeError, "%zd arguments wanted, got %zd", want, n);
+  }
+  int64_t integer() {
+    if (!good_) return 0;
+    const long long v = PyLong_AsLongLong(*args_++);
+    good_ = !(v == -1 && PyErr_Occurred());
+    return v;
+  }
+  template <class P = void>
+  P* pointer() {
+    if (!good_) return nullptr;
+    const unsigned long long v = PyLong_AsUnsignedLongLong(*args_++);
+    good_ = !(v == ~0ull && PyErr_Occurred());
+    return (P*)v;
+  }
+  float real() {
+    if (!good_) return 0;
+    const double v = PyFloat_AsDouble(*args_++);
+    good_ = !(v == -1 && PyErr_Occurred());
+    return (float)v;
+  }
+  LmType type() {
+    const int64_t v = integer();
+    if (good_ && (v < 0 || v > 2)) {
+      PyErr_SetString(PyExc_RuntimeError, "bad dtype code");
+      good_ = false;
+    }
+    return (LmType)v;
+  }
+  int within(int64_t low, int64_t high, const char* what) {
+    const int64_t v = integer();
+    if (good_ && (v < low || v > high)) {
+      PyErr_SetString(PyExc_RuntimeError, what);
+      good_ = false;
+    }
+    return (int)v;
+  }
+  bool good() const { return good_; }
 
-LmType lm_type(int code) {
-  if (code < 0 || code > 2) throw std::runtime_error("bad dtype code");
-  return (LmType)code;
-}
+ private:
+  PyObject* const* args_;
+  bool good_;
+};
 
 PyObject* py_is_available(PyObject*, PyObject*) {
   int count = 0;
@@ -47,186 +91,211 @@ PyObject* py_is_available(PyObject*, PyObject*) {
   Py_RETURN_TRUE;
 }
 
-PyObject* py_mx_quantize(PyObject*, PyObject* args) {
-  int dt;
-  ull x, codes, scales, stream;
-  long long stride, rows, k;
-  if (!PyArg_ParseTuple(args, "iKLKKLLK", &dt, &x, &stride, &codes, &scales,
-                        &rows, &k, &stream))
-    return nullptr;
+PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 8);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer();
+  auto* codes = a.pointer<uint8_t>();
+  auto* scales = a.pointer<uint8_t>();
+  const int64_t rows = a.integer(), k = a.integer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
   NOGIL_BEGIN
-  launch_mx_quantize(t, (const void*)x, stride, (uint8_t*)codes,
-                     (uint8_t*)scales, rows, k, (hipStream_t)stream);
+  launch_mx_quantize(t, x, stride, codes, scales, rows, k, stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_mx_dequantize(PyObject*, PyObject* args) {
-  int dt;
-  ull codes, scales, out, stream;
-  long long rows, k;
-  if (!PyArg_ParseTuple(args, "iKKKLLK", &dt, &codes, &scales, &out, &rows,
-                        &k, &stream))
-    return nullptr;
+PyObject* py_mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 7);
+  const LmType t = a.type();
+  auto* codes = a.pointer<uint8_t>();
+  auto* scales = a.pointer<uint8_t>();
+  void* out = a.pointer();
+  const int64_t rows = a.integer(), k = a.integer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
   NOGIL_BEGIN
-  launch_mx_dequantize(t, (const uint8_t*)codes, (const uint8_t*)scales,
-                       (void*)out, rows, k, (hipStream_t)stream);
+  launch_mx_dequantize(t, codes, scales, out, rows, k, stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_mx_linear_workspace(PyObject*, PyObject* args) {
-  long long m, n, k;
-  int packed;
-  if (!PyArg_ParseTuple(args, "LLLp", &m, &n, &k, &packed)) return nullptr;
-  return PyLong_FromLongLong(mx_linear_workspace(m, n, k, packed));
+PyObject* py_mx_linear_workspace(PyObject*, PyObject* const* args,
+                                 Py_ssize_t n) {
+  Args a(args, n, 4);
+  const int64_t m = a.integer(), cols = a.integer(), k = a.integer();
+  const bool packed = a.integer() != 0;
+  if (!a.good()) return nullptr;
+  return PyLong_FromLongLong(mx_linear_workspace(m, cols, k, packed));
 }
 
-PyObject* py_mx_linear(PyObject*, PyObject* args) {
-  int dt;
-  ull x, xc, xs, wc, ws, bias, y, work, stream;
-  long long stride, m, n, k;
-  if (!PyArg_ParseTuple(args, "iKLKKKKKKLLLKK", &dt, &x, &stride, &xc, &xs,
-                        &wc, &ws, &bias, &y, &m, &n, &k, &work, &stream))
-    return nullptr;
+PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 14);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer();
+  auto* xc = a.pointer<uint8_t>();
+  auto* xs = a.pointer<uint8_t>();
+  auto* wc = a.pointer<uint8_t>();
+  auto* ws = a.pointer<uint8_t>();
+  const void* bias = a.pointer();
+  void* y = a.pointer();
+  const int64_t m = a.integer(), cols = a.integer(), k = a.integer();
+  void* work = a.pointer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
   NOGIL_BEGIN
-  launch_mx_linear(t, (const void*)x, stride, (const uint8_t*)xc,
-                   (const uint8_t*)xs, (const uint8_t*)wc,
-                   (const uint8_t*)ws, (const void*)bias, (void*)y, m, n, k,
-                   (void*)work, (hipStream_t)stream);
+  launch_mx_linear(t, x, stride, xc, xs, wc, ws, bias, y, m, cols, k, work,
+                   stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_score_workspace(PyObject*, PyObject* args) {
-  int dt, top;
-  long long rows, v;
-  if (!PyArg_ParseTuple(args, "iLLi", &dt, &rows, &v, &top)) return nullptr;
-  WRAP_BEGIN
-  return PyLong_FromLongLong(score_workspace(lm_type(dt), rows, v, top));
-  WRAP_END
+PyObject* py_score_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 4);
+  const LmType t = a.type();
+  const int64_t rows = a.integer(), v = a.integer();
+  const int top = a.within(0, kMaxTop, "bad top");
+  if (!a.good()) return nullptr;
+  return PyLong_FromLongLong(score_workspace(t, rows, v, top));
 }
 
-PyObject* py_token_logprobs(PyObject*, PyObject* args) {
-  int dt, top;
-  ull x, tokens, lp, entropy, top_lp, top_ids, stats, work, stream;
-  long long stride, rows, v, ignore;
-  float inv_t;
-  if (!PyArg_ParseTuple(args, "iKLLLKLfiKKKKKKK", &dt, &x, &stride, &rows, &v,
-                        &tokens, &ignore, &inv_t, &top, &lp, &entropy,
-                        &top_lp, &top_ids, &stats, &work, &stream))
-    return nullptr;
+PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 16);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
+  auto* tokens = a.pointer<int64_t>();
+  const int64_t ignore = a.integer();
+  const float inv_t = a.real();
+  const int top = a.within(0, kMaxTop, "bad top");
+  auto* logprobs = a.pointer<float>();
+  auto* entropy = a.pointer<float>();
+  auto* top_lp = a.pointer<float>();
+  auto* top_ids = a.pointer<int64_t>();
+  auto* stats = a.pointer<RowStats>();
+  void* work = a.pointer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
-  if (top < 0 || top > kMaxTop) throw std::runtime_error("bad top");
   NOGIL_BEGIN
-  launch_token_logprobs(t, (const void*)x, stride, rows, v,
-                        (const int64_t*)tokens, ignore, inv_t, top,
-                        (float*)lp, (float*)entropy, (float*)top_lp,
-                        (int64_t*)top_ids, (RowStats*)stats, (void*)work,
-                        (hipStream_t)stream);
+  launch_token_logprobs(t, x, stride, rows, v, tokens, ignore, inv_t, top,
+                        logprobs, entropy, top_lp, top_ids, stats, work,
+                        stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_token_logprobs_bwd(PyObject*, PyObject* args) {
-  int dt;
-  ull x, tokens, stats, g_lp, g_h, dx, stream;
-  long long stride, rows, v;
-  float inv_t;
-  if (!PyArg_ParseTuple(args, "iKLLLKfKKKKK", &dt, &x, &stride, &rows, &v,
-                        &tokens, &inv_t, &stats, &g_lp, &g_h, &dx, &stream))
-    return nullptr;
+PyObject* py_token_logprobs_bwd(PyObject*, PyObject* const* args,
+                                Py_ssize_t n) {
+  Args a(args, n, 12);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
+  auto* tokens = a.pointer<int64_t>();
+  const float inv_t = a.real();
+  auto* stats = a.pointer<RowStats>();
+  auto* g_lp = a.pointer<float>();
+  auto* g_h = a.pointer<float>();
+  void* dx = a.pointer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
   NOGIL_BEGIN
-  launch_token_logprobs_bwd(t, (const void*)x, stride, rows, v,
-                            (const int64_t*)tokens, inv_t,
-                            (const RowStats*)stats, (const float*)g_lp,
-                            (const float*)g_h, (void*)dx,
-                            (hipStream_t)stream);
+  launch_token_logprobs_bwd(t, x, stride, rows, v, tokens, inv_t, stats, g_lp,
+                            g_h, dx, stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_distill(PyObject*, PyObject* args) {
-  int dt, tt, k, mean;
-  ull x, teacher, ids, row_loss, q, stats, total, work, stream;
-  long long stride, rows, v;
-  float inv_t;
-  if (!PyArg_ParseTuple(args, "iKLLLiKKifKKKKpKK", &dt, &x, &stride, &rows,
-                        &v, &tt, &teacher, &ids, &k, &inv_t, &row_loss, &q,
-                        &stats, &total, &mean, &work, &stream))
-    return nullptr;
+PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 18);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
+  const LmType tt = a.type();
+  const void* teacher = a.pointer();
+  auto* ids = a.pointer<int64_t>();
+  const int k = a.within(1, kMaxRecord, "bad record length");
+  const float inv_t = a.real();
+  auto* row_loss = a.pointer<float>();
+  auto* q = a.pointer<float>();
+  auto* stats = a.pointer<RowStats>();
+  auto* total = a.pointer<float>();
+  auto* count = a.pointer<float>();
+  const bool mean = a.integer() != 0;
+  void* work = a.pointer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt), u = lm_type(tt);
-  if (k < 1 || k > kMaxRecord) throw std::runtime_error("bad record length");
   NOGIL_BEGIN
-  launch_distill(t, (const void*)x, stride, rows, v, u, (const void*)teacher,
-                 (const int64_t*)ids, k, inv_t, (float*)row_loss, (float*)q,
-                 (RowStats*)stats, (float*)total, mean, (void*)work,
-                 (hipStream_t)stream);
+  launch_distill(t, x, stride, rows, v, tt, teacher, ids, k, inv_t, row_loss,
+                 q, stats, total, count, mean, work, stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
 
-PyObject* py_distill_bwd(PyObject*, PyObject* args) {
-  int dt, k;
-  ull x, ids, q, stats, grad, count, dx, stream;
-  long long stride, rows, v, grad_stride;
-  float inv_t;
-  if (!PyArg_ParseTuple(args, "iKLLLKKifKKLKKK", &dt, &x, &stride, &rows, &v,
-                        &ids, &q, &k, &inv_t, &stats, &grad, &grad_stride,
-                        &count, &dx, &stream))
-    return nullptr;
+PyObject* py_distill_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 15);
+  const LmType t = a.type();
+  const void* x = a.pointer();
+  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
+  auto* ids = a.pointer<int64_t>();
+  auto* q = a.pointer<float>();
+  const int k = a.within(1, kMaxRecord, "bad record length");
+  const float inv_t = a.real();
+  auto* stats = a.pointer<RowStats>();
+  auto* grad = a.pointer<float>();
+  const int64_t grad_stride = a.integer();
+  auto* count = a.pointer<float>();
+  void* dx = a.pointer();
+  auto stream = (hipStream_t)a.pointer();
+  if (!a.good()) return nullptr;
   WRAP_BEGIN
-  LmType t = lm_type(dt);
-  if (k < 1 || k > kMaxRecord) throw std::runtime_error("bad record length");
   NOGIL_BEGIN
-  launch_distill_bwd(t, (const void*)x, stride, rows, v, (const int64_t*)ids,
-                     (const float*)q, k, inv_t, (const RowStats*)stats,
-                     (const float*)grad, grad_stride, (const float*)count,
-                     (void*)dx, (hipStream_t)stream);
+  launch_distill_bwd(t, x, stride, rows, v, ids, q, k, inv_t, stats, grad,
+                     grad_stride, count, dx, stream);
   NOGIL_END
   Py_RETURN_NONE;
   WRAP_END
 }
+
+#define FAST(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL
 
 PyMethodDef methods[] = {
     {"is_available", py_is_available, METH_NOARGS, "GPU present?"},
-    {"mx_quantize", py_mx_quantize, METH_VARARGS,
+    {"mx_quantize", FAST(py_mx_quantize),
      "mx_quantize(dtype, x, stride, codes, scales, rows, k, stream)"},
-    {"mx_dequantize", py_mx_dequantize, METH_VARARGS,
+    {"mx_dequantize", FAST(py_mx_dequantize),
      "mx_dequantize(dtype, codes, scales, out, rows, k, stream)"},
-    {"mx_linear_workspace", py_mx_linear_workspace, METH_VARARGS,
+    {"mx_linear_workspace", FAST(py_mx_linear_workspace),
      "mx_linear_workspace(m, n, k, packed) -> bytes"},
-    {"mx_linear", py_mx_linear, METH_VARARGS,
+    {"mx_linear", FAST(py_mx_linear),
      "mx_linear(dtype, x, stride, xcodes, xscales, wcodes, wscales, bias, y, "
      "m, n, k, workspace, stream)"},
-    {"score_workspace", py_score_workspace, METH_VARARGS,
+    {"score_workspace", FAST(py_score_workspace),
      "score_workspace(dtype, rows, v, top) -> bytes"},
-    {"token_logprobs", py_token_logprobs, METH_VARARGS,
+    {"token_logprobs", FAST(py_token_logprobs),
      "token_logprobs(dtype, x, stride, rows, v, tokens, ignore, inv_t, top, "
      "logprobs, entropy, top_lp, top_ids, stats, workspace, stream)"},
-    {"token_logprobs_bwd", py_token_logprobs_bwd, METH_VARARGS,
+    {"token_logprobs_bwd", FAST(py_token_logprobs_bwd),
      "token_logprobs_bwd(dtype, x, stride, rows, v, tokens, inv_t, stats, "
      "g_logprobs, g_entropy, dx, stream)"},
-    {"distill", py_distill, METH_VARARGS,
+    {"distill", FAST(py_distill),
      "distill(dtype, x, stride, rows, v, teacher_dtype, teacher, ids, k, "
-     "inv_t, row_loss, q, stats, total, mean, workspace, stream)"},
-    {"distill_bwd", py_distill_bwd, METH_VARARGS,
+     "inv_t, row_loss, q, stats, total, count, mean, workspace, stream)"},
+    {"distill_bwd", FAST(py_distill_bwd),
      "distill_bwd(dtype, x, stride, rows, v, ids, q, k, inv_t, stats, grad, "
      "grad_stride, count, dx, stream)"},
     {nullptr, nullptr, 0, nullptr},

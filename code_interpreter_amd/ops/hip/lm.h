@@ -59,13 +59,14 @@ void launch_token_logprobs_bwd(LmType t, const void* x, int64_t stride,
                                hipStream_t stream);
 
 // teacher: [rows][k] recorded logits and ids, an id of -1 or a logit of
-// -inf where a row has fewer. row_loss [rows], q [rows][k]; mean (may be
-// null): {sum or mean over rows with a record, their number}
+// -inf where a row has fewer. row_loss [rows], q [rows][k]. total (may be
+// null): the sum, or the mean over rows with a record; count: what the sum
+// was divided by
 void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
                     int64_t v, LmType tt, const void* teacher,
                     const int64_t* ids, int k, float inv_t, float* row_loss,
-                    float* q, RowStats* stats, float* total, bool mean,
-                    void* ws, hipStream_t stream);
+                    float* q, RowStats* stats, float* total, float* count,
+                    bool mean, void* ws, hipStream_t stream);
 void launch_distill_bwd(LmType t, const void* x, int64_t stride,
                         int64_t rows, int64_t v, const int64_t* ids,
                         const float* q, int k, float inv_t,

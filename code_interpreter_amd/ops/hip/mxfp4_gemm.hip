@@ -434,13 +434,52 @@ __global__ __launch_bounds__(WM* WN * 64, 1) void tile_kernel(
 // few tokens
 // ---------------------------------------------------------------------------
 // The weights are read once, from memory into registers, and bound the time;
-// 16 * MT tokens are held against them. A block makes 16 * NT outputs of all
-// tokens: its 8 waves take turns along k, 512 elements a turn, a lane 4
-// neighbouring blocks (64 bytes) of one row, and add up through shared
-// memory at the end, in a fixed order. The tokens come from memory as codes
-// (packed), or are quantised by each block into its shared memory, which
-// saves a launch and costs the more the more tokens there are.
-template <LmType T, int MT, int NT, bool kPacked>
+// 16 * MT tokens are held against them. A block makes 16 outputs of all
+// tokens: its 8 waves take turns along k, 512 elements a turn, and add up
+// through shared memory at the end, in a fixed order. The loads of two turns
+// are under way before the first is worked on. The tokens come from memory
+// as codes (packed), or are quantised by each block into its shared memory,
+// which saves a launch and costs the more the more tokens there are.
+//
+// Instruction j of a turn takes blocks 4 j + q from the lanes 16 q .. 16 q +
+// 15, so that 4 lanes load 64 bytes in a row. A lane holds the 16 scales of
+// its row's turn, and shifts the one for instruction j to the word's front.
+using raw16b = uint32_t __attribute__((ext_vector_type(4), aligned(1)));
+
+// bytes of a token's codes and scales in shared memory
+__host__ __device__ constexpr int few_codes(int nb) { return (nb | 1) * 16; }
+__host__ __device__ constexpr int few_scales(int nb) {
+  return ((nb + 15) / 16 | 1) * 16;
+}
+
+struct Turn {
+  u32x4 c[4], s;
+};
+
+// blocks [at, at + 16) of a row of nb, from memory or shared memory; behind
+// its end codes of 0 and scales of 1
+template <bool kScales>
+__device__ __forceinline__ void load_turn(const uint8_t* codes,
+                                          const uint8_t* scales, int at,
+                                          int nb, int q, Turn& to) {
+  if (at + 16 <= nb) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      to.c[j] = *(const u32x4*)(codes + (int64_t)(at + 4 * j + q) * 16);
+    if constexpr (kScales) to.s = *(const raw16b*)(scales + at);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int blk = at + 4 * j + q;
+    to.c[j] = blk < nb ? *(const u32x4*)(codes + (int64_t)blk * 16)
+                       : u32x4{0, 0, 0, 0};
+    if constexpr (kScales)
+      to.s[j] = (blk < nb ? (uint32_t)scales[blk] : 0x7Fu) << (8 * q);
+  }
+}
+
+template <LmType T, int MT, bool kPacked>
 __global__ __launch_bounds__(512) void few_kernel(
     const void* __restrict__ x, int64_t stride,
     const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs,
@@ -451,39 +490,20 @@ __global__ __launch_bounds__(512) void few_kernel(
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l15 = lane & 15, q = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int turns = (nb + 15) / 16;
 
-  const uint8_t* wrow[NT];
-  const uint8_t* srow[NT];
-#pragma unroll
-  for (int i = 0; i < NT; i++) {
-    int64_t r = min(n0 + i * 16 + l15, n - 1);
-    wrow[i] = wc + r * nb * kMxBytes;
-    srow[i] = ws + r * nb;
-  }
-  struct Turn {
-    u32x4 c[NT][4];
-    uint32_t s[NT];
-  };
-  auto load = [&](int turn, Turn& to) {
-    const int at = turn * 16 + 4 * q;
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        to.c[i][j] = at + j < nb
-                         ? *(const u32x4*)(wrow[i] + (int64_t)(at + j) * 16)
-                         : u32x4{0, 0, 0, 0};
-      to.s[i] = load_scales(srow[i], at, nb);
-    }
-  };
-  Turn next;
-  if (wave < turns) load(wave, next);
+  const int64_t r = min(n0 + l15, n - 1);
+  const uint8_t* wrow = wc + r * nb * kMxBytes;
+  const uint8_t* srow = ws + r * nb;
+  Turn next, after;
+  if (wave < turns) load_turn<true>(wrow, srow, wave * 16, nb, q, next);
+  if (wave + kWaves < turns)
+    load_turn<true>(wrow, srow, (wave + kWaves) * 16, nb, q, after);
 
-  // codes of a token stand (nb + 1) * 16 bytes apart: 8 lanes that read the
-  // same unit of 8 tokens touch all banks once
-  const int crow = (nb + 1) * 16, sstride = ((nb + 3) & ~3) + 4;
+  // In shared memory tokens stand an odd number of 16-byte units apart: 16
+  // lanes that read the same unit of 16 tokens touch all banks once.
+  const int crow = few_codes(nb), sstride = few_scales(nb);
   uint8_t* lds_s = (uint8_t*)smem + m * crow;
   if constexpr (!kPacked) {
     const uint32_t per_row = (uint32_t)nb * 4, groups = per_row * m;
@@ -497,73 +517,52 @@ __global__ __launch_bounds__(512) void few_kernel(
           byte == 255 ? 0u : encode<T>(w, w2, scale_value(byte));
       if ((g & 3) == 0) lds_s[row * sstride + (col >> 2)] = (uint8_t)byte;
     }
-    // scales of 1 up to the end of a row's last whole word
-    for (uint32_t g = threadIdx.x; g < 4u * m; g += 512) {
-      const uint32_t col = nb + (g & 3);
-      if (col < (uint32_t)sstride) lds_s[(g >> 2) * sstride + col] = 0x7F;
+    // scales of 1 up to the end of a row's last turn
+    for (uint32_t g = threadIdx.x; g < 16u * m; g += 512) {
+      const int col = nb + (int)(g & 15);
+      if (col < turns * 16) lds_s[(g >> 4) * sstride + col] = 0x7F;
     }
     __syncthreads();
   }
 
-  v4f acc[NT][MT] = {};
+  v4f acc[MT] = {};
   for (int turn = wave; turn < turns; turn += kWaves) {
     Turn now = next;
-    if (turn + kWaves < turns) load(turn + kWaves, next);
-    const int at = turn * 16 + 4 * q;
+    next = after;
+    if (turn + 2 * kWaves < turns)
+      load_turn<true>(wrow, srow, (turn + 2 * kWaves) * 16, nb, q, after);
 #pragma unroll
-    for (int j = 0; j < MT; j++) {
-      const int token = min(j * 16 + l15, m - 1);
-      u32x4 c[4];
-      uint32_t s;
+    for (int i = 0; i < MT; i++) {
+      const int token = min(i * 16 + l15, m - 1);
+      Turn tok;
       if constexpr (kPacked) {
-        const uint8_t* p = xc + ((int64_t)token * nb + at) * 16;
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-          c[b] = at + b < nb ? *(const u32x4*)(p + b * 16)
-                             : u32x4{0, 0, 0, 0};
-        s = load_scales(xs + (int64_t)token * nb, at, nb);
+        load_turn<true>(xc + (int64_t)token * nb * 16, xs + (int64_t)token * nb,
+                        turn * 16, nb, q, tok);
       } else {
-        const char* p = smem + token * crow + at * 16;
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-          c[b] = at + b < nb ? *(const u32x4*)(p + b * 16)
-                             : u32x4{0, 0, 0, 0};
-        s = at < nb ? *(const uint32_t*)(lds_s + token * sstride + at) : kUnit;
+        load_turn<false>((const uint8_t*)smem + token * crow, nullptr,
+                         turn * 16, nb, q, tok);
+        tok.s = *(const u32x4*)(lds_s + token * sstride + turn * 16);
       }
 #pragma unroll
-      for (int i = 0; i < NT; i++) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            operand(now.c[i][0]), operand(c[0]), acc[i][j], 4, 4, 0,
-            (int)now.s[i], 0, (int)s);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            operand(now.c[i][1]), operand(c[1]), acc[i][j], 4, 4, 1,
-            (int)now.s[i], 1, (int)s);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            operand(now.c[i][2]), operand(c[2]), acc[i][j], 4, 4, 2,
-            (int)now.s[i], 2, (int)s);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            operand(now.c[i][3]), operand(c[3]), acc[i][j], 4, 4, 3,
-            (int)now.s[i], 3, (int)s);
-      }
+      for (int j = 0; j < 4; j++)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            operand(now.c[j]), operand(tok.c[j]), acc[i], 4, 4, 0,
+            (int)(now.s[j] >> (8 * q)), 0, (int)(tok.s[j] >> (8 * q)));
     }
   }
 
   __syncthreads();  // the tokens' place is taken by the partial sums
-  v4f* part = (v4f*)smem;  // [wave][NT][MT][64]
+  v4f* part = (v4f*)smem;  // [wave][MT][64]
 #pragma unroll
-  for (int i = 0; i < NT; i++)
-#pragma unroll
-    for (int j = 0; j < MT; j++)
-      part[((wave * NT + i) * MT + j) * 64 + lane] = acc[i][j];
+  for (int i = 0; i < MT; i++) part[(wave * MT + i) * 64 + lane] = acc[i];
   __syncthreads();
-  for (int e = threadIdx.x; e < NT * MT * 64; e += 512) {
-    const int j = (e >> 6) % MT, i = (e >> 6) / MT;
-    const int token = j * 16 + (e & 15);
-    const int64_t col = n0 + i * 16 + 4 * ((e & 63) >> 4);
+  for (int e = threadIdx.x; e < MT * 64; e += 512) {
+    const int token = (e >> 6) * 16 + (e & 15);
+    const int64_t col = n0 + 4 * ((e & 63) >> 4);
     const int valid = (int)min((int64_t)4, n - col);
     if (token >= m || valid <= 0) continue;
     v4f sum = part[e];
-    for (int w = 1; w < kWaves; w++) sum += part[w * NT * MT * 64 + e];
+    for (int w = 1; w < kWaves; w++) sum += part[w * MT * 64 + e];
     float f[4];
     for (int r = 0; r < 4; r++)
       f[r] = sum[r] + (bias && r < valid ? bias_at<T>(bias, col + r) : 0.f);
@@ -575,10 +574,11 @@ __global__ __launch_bounds__(512) void few_kernel(
 // launching
 // ---------------------------------------------------------------------------
 constexpr int kFewTokens = 64;
-constexpr int64_t kFusedLds = 64 << 10;
+constexpr int64_t kFusedLds = 150 << 10;
 
 int64_t few_lds(int64_t m, int64_t nb) {
-  return m * ((nb + 1) * 16 + ((nb + 3) & ~3) + 4);
+  return nb > 1 << 14 ? 1 << 30
+                      : m * (few_codes((int)nb) + few_scales((int)nb));
 }
 
 bool fuses(int64_t m, int64_t nb) {
@@ -672,12 +672,11 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
   if (m <= kFewTokens) {
     auto go = [&](auto mt, auto packed) {
       constexpr int MT = decltype(mt)::value;
-      constexpr int NT = 1;
       constexpr bool P = decltype(packed)::value;
       int64_t lds = std::max<int64_t>(P ? 0 : few_lds(m, nb),
-                                      (int64_t)8 * NT * MT * 64 * 16);
-      few_kernel<T, MT, NT, P>
-          <<<dim3((unsigned)((n + 16 * NT - 1) / (16 * NT))), 512, lds,
+                                      (int64_t)8 * MT * 64 * 16);
+      few_kernel<T, MT, P>
+          <<<dim3((unsigned)((n + 15) / 16)), 512, lds,
              stream>>>(x, stride, xc, xs, wc, ws, bias, y, (int)m, n, k,
                        (int)nb);
       HIP_CHECK(hipGetLastError());

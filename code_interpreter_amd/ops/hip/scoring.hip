@@ -30,6 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLow = -16384.f;  // 2^kLow is 0
 constexpr int kThreads = 256;
+constexpr int kMaxKeys = 4096;  // of a row's parts together, 32 KB
 constexpr int kWaves = kThreads / 64;
 
 // 16 bytes at any element's address: the hardware takes vector loads and
@@ -165,12 +166,20 @@ __device__ __forceinline__ Triple join(Triple a, Triple b, float c) {
   return {m, x.s + y.s, x.u + y.u};
 }
 
-__device__ Triple join_wave(Triple a, float c) {
+__device__ __forceinline__ float wave_sum(float a) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1)
-    a = join(a, {__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.u, d)},
-             c);
+  for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
   return a;
+}
+__device__ __forceinline__ float wave_max(float a) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) a = fmaxf(a, __shfl_xor(a, d));
+  return a;
+}
+
+__device__ __forceinline__ Triple join_wave(Triple a, float c) {
+  a = under(a, wave_max(a.m), c);
+  return {a.m, wave_sum(a.s), wave_sum(a.u)};
 }
 
 // order-preserving bits of a value above, the complement of its index
@@ -192,91 +201,148 @@ __device__ __forceinline__ uint32_t key_index(uint64_t key) {
 // ---------------------------------------------------------------------------
 // alternatives
 // ---------------------------------------------------------------------------
-constexpr int kCap = 2048;  // candidates that are ranked at a time
+constexpr int kCap = 2048;  // candidates that are held at a time
 
 struct TopShared {
-  uint64_t keys[kCap];   // the best so far, then candidates
+  // the best so far, then candidates; a pair more than there can be
+  alignas(16) uint64_t keys[kCap + 2];
   uint64_t best[kMaxTop];
   uint64_t wave_key[kWaves];
-  float thread_max[kThreads];
-  float least;           // candidates are larger than this
-  int have;              // entries of the best so far
-  int count;             // entries of keys
+  float bound[kWaves];
+  float least;    // a candidate is larger than this
+  int count;      // entries of keys
+  int flag[3];    // whether a chunk has candidates, by its number mod 3
 };
 
 // keys[0 .. n) -> the k best, sorted, at keys[0 ..), by counting for each
-// key how many are larger: keys are all different
-__device__ void rank_keys(TopShared& sh, int n, int k) {
+// key how many are larger: keys are all different. Returns their number.
+__device__ int rank_keys(TopShared& sh, int n, int k) {
+  using Pair = uint64_t __attribute__((ext_vector_type(2)));
+  if (threadIdx.x == 0) sh.keys[n] = 0;  // the last pair's other half
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    uint64_t key = sh.keys[i];
+    const uint64_t key = sh.keys[i];
     int rank = 0;
-    for (int j = 0; j < n; j++) rank += sh.keys[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+      const Pair o = *(const Pair*)&sh.keys[j];
+      rank += (o[0] > key) + (o[1] > key);
+    }
     if (rank < k) sh.best[rank] = key;
   }
   __syncthreads();
-  int have = min(n, k);
+  const int have = min(n, k);
   for (int i = threadIdx.x; i < have; i += kThreads) sh.keys[i] = sh.best[i];
   if (threadIdx.x == 0) {
-    sh.have = sh.count = have;
+    sh.count = have;
     if (have == k) sh.least = key_value(sh.best[k - 1]);
   }
   __syncthreads();
+  return have;
 }
 
-// Takes the candidates of a chunk that the block holds in registers: words
-// w[0 .. U) of each thread, thread t's word i at element base + (i * 256 +
-// t) * kVec. Chunks come in the order of their indexes, so that an element
-// must be larger than the last of the k best so far to displace it.
+// The k best of a row's elements, from chunks that the block holds in
+// registers: words w[0 .. U) of each thread, thread t's word i at element
+// base + (i * 256 + t) * kVec. Chunks come in the order of their indexes, so
+// that an element must be larger than the last of the k best so far to
+// displace it; few of a later chunk are. Candidates are gathered and ranked
+// when there are 3 k + 32 or more, or at the end: ranking raises the bar for
+// what follows, and costs the square of their number.
 //
-// The k-th largest of the threads' own maxima is a lower bound of the
-// chunk's k-th largest element. At most k - 1 threads hold larger elements
-// than it, so few pass it but where many are equal. Where the candidates
-// still do not fit, the k best are taken one by one.
+// For the first chunk, and where candidates do not fit: in each of the 4
+// waves ceil(k / 4) threads hold an element that is not below the
+// ceil(k / 4)-th largest of the threads' own maxima. So the least of the four
+// is a lower bound of the chunk's k-th largest element. Not many elements
+// pass it but where many are equal. Where the candidates still do not fit,
+// the k best are taken one by one.
 template <LmType T, int U>
-__device__ void take_candidates(TopShared& sh, const u32x4* w, int64_t base,
-                                float thread_max, int k) {
+struct Top {
   using E = Elem<T>;
-  const int tid = threadIdx.x;
-  float least = sh.least;
-  auto append = [&](float floor_) {
-    if (thread_max > least && thread_max >= floor_) {
-#pragma unroll
-      for (int i = 0; i < U; i++)
-#pragma unroll
-        for (int j = 0; j < E::kVec; j++) {
-          float x = E::get(w[i], j);
-          if (x > least && x >= floor_) {
-            int at = atomicAdd(&sh.count, 1);
-            if (at < kCap)
-              sh.keys[at] = make_key(
-                  x, (uint32_t)(base + (i * kThreads + tid) * E::kVec + j));
-          }
-        }
+  TopShared& sh;
+  const int k;
+  int have = 0, count = 0, chunk = 0;  // equal in all threads
+  float least = -INFINITY;
+
+  __device__ Top(TopShared& sh, int k) : sh(sh), k(k) {
+    if (threadIdx.x == 0) {
+      sh.count = 0;
+      sh.least = least;
+      sh.flag[0] = sh.flag[1] = sh.flag[2] = 0;
     }
+    __syncthreads();
+  }
+
+  // elements larger than `least` and not less than `bound` to the keys
+  __device__ void append(const u32x4* w, int64_t base, float thread_max,
+                         float bound) {
+    if (!(thread_max > least && thread_max >= bound)) return;
+    uint32_t which = 0;  // of the thread's elements
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++) {
+        const float x = E::get(w[i], j);
+        which |= (uint32_t)((x > least) & (x >= bound)) << (i * E::kVec + j);
+      }
+    int at = atomicAdd(&sh.count, __popc(which));
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+      for (int j = 0; j < E::kVec; j++) {
+        if (!(which >> (i * E::kVec + j) & 1)) continue;
+        if (at < kCap)
+          sh.keys[at] = make_key(
+              E::get(w[i], j),
+              (uint32_t)(base + (i * kThreads + threadIdx.x) * E::kVec + j));
+        at++;
+      }
+  }
+
+  __device__ void merge(int n) {
+    have = count = rank_keys(sh, n, k);
+    least = sh.least;
+  }
+
+  // The ceil(k / 4)-th largest of a wave's lanes' maxima, by the bits of its
+  // order from the top: each is set where enough lanes stay at or above it.
+  // kBits of them give 16-bit types exactly, and a lower bound for the rest.
+  __device__ float bound_of_wave(float lane_max) const {
+    constexpr int kBits = 20;
+    const uint32_t order = (uint32_t)(make_key(lane_max, 0) >> 32);
+    const int r = (k + kWaves - 1) / kWaves;
+    uint32_t found = 0;
+#pragma unroll
+    for (int bit = 31; bit > 31 - kBits; bit--) {
+      const uint32_t with = found | 1u << bit;
+      if (__popcll(__ballot(order >= with)) >= r) found = with;
+    }
+    // no number's order is below that of -inf
+    return key_value((uint64_t)max(found, 0x007FFFFFu) << 32);
+  }
+
+  __device__ void take_bounded(const u32x4* w, int64_t base,
+                               float thread_max) {
+    const int tid = threadIdx.x;
+    const float mine = bound_of_wave(thread_max);
+    if ((tid & 63) == 0) sh.bound[tid >> 6] = mine;
+    __syncthreads();
+    float bound = sh.bound[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; i++) bound = fminf(bound, sh.bound[i]);
+    append(w, base, thread_max, bound);
     __syncthreads();
     int n = sh.count;
     __syncthreads();
-    if (n > kCap && tid == 0) sh.count = sh.have;
-    return n;
-  };
-  int n = kCap + 1;
-  if (sh.have == k) n = append(-INFINITY);
-  if (n > kCap) {
-    sh.thread_max[tid] = thread_max;
-    __syncthreads();
-    // of equal maxima the threads' order decides: one thread has rank k - 1
-    int rank = 0;
-    for (int j = 0; j < kThreads; j++) {
-      float o = sh.thread_max[j];
-      rank += o > thread_max || (o == thread_max && j < tid);
+    if (n > kCap) {
+      if (tid == 0) sh.count = have;
+      __syncthreads();
+      n = one_by_one(w, base);
     }
-    __syncthreads();
-    if (rank == k - 1) sh.thread_max[0] = thread_max;
-    __syncthreads();
-    n = append(sh.thread_max[0]);
+    merge(n);
   }
-  if (n > kCap) {
-    __syncthreads();  // sh.count is back at sh.have
+
+  __device__ int one_by_one(const u32x4* w, int64_t base) {
+    const int tid = threadIdx.x;
     uint64_t last = ~0ull;
     for (int r = 0; r < k; r++) {
       uint64_t mine = 0;
@@ -284,14 +350,14 @@ __device__ void take_candidates(TopShared& sh, const u32x4* w, int64_t base,
       for (int i = 0; i < U; i++)
 #pragma unroll
         for (int j = 0; j < E::kVec; j++) {
-          float x = E::get(w[i], j);
-          uint64_t key = make_key(
+          const float x = E::get(w[i], j);
+          const uint64_t key = make_key(
               x, (uint32_t)(base + (i * kThreads + tid) * E::kVec + j));
           if (x > least && key < last && key > mine) mine = key;
         }
 #pragma unroll
       for (int d = 32; d; d >>= 1) {
-        uint64_t o = __shfl_xor((unsigned long long)mine, d);
+        const uint64_t o = __shfl_xor((unsigned long long)mine, d);
         mine = o > mine ? o : mine;
       }
       if ((tid & 63) == 0) sh.wave_key[tid >> 6] = mine;
@@ -305,21 +371,56 @@ __device__ void take_candidates(TopShared& sh, const u32x4* w, int64_t base,
       last = best;
     }
     __syncthreads();
-    n = sh.count;
+    return sh.count;
   }
-  rank_keys(sh, n, k);
-}
+
+  __device__ void take(const u32x4* w, int64_t base, float thread_max) {
+    const int now = chunk % 3;
+    chunk++;
+    if (__any(thread_max > least) && (threadIdx.x & 63) == 0) sh.flag[now] = 1;
+    __syncthreads();
+    // the flag of the chunk after the next: it is set behind another barrier
+    if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
+    if (!sh.flag[now]) return;
+    if (have < k) {
+      if (count > have) merge(count);
+      return take_bounded(w, base, thread_max);
+    }
+    append(w, base, thread_max, -INFINITY);
+    __syncthreads();
+    const int n = sh.count;
+    if (n < 3 * k + 32) {
+      count = n;
+      return;
+    }
+    __syncthreads();
+    if (n <= kCap) return merge(n);
+    if (threadIdx.x == 0) sh.count = count;
+    __syncthreads();
+    merge(count);  // what was there before this chunk
+    take_bounded(w, base, thread_max);
+  }
+
+  __device__ void finish() {
+    __syncthreads();
+    if (count > have) merge(count);
+  }
+};
 
 // ---------------------------------------------------------------------------
 // one pass over a row, or over one of `splits` parts of it
 // ---------------------------------------------------------------------------
+struct NoTop {
+  __device__ NoTop(int&, int) {}
+};
+
 struct Part {
   Triple t;
   float pad;
 };
 
 template <LmType T, int U, bool kEntropy, bool kTop>
-__global__ __launch_bounds__(kThreads) void score_kernel(
+__global__ __launch_bounds__(kThreads, 4) void score_kernel(
     const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
     int splits, int64_t part_len, float c, int k, Part* __restrict__ parts,
     uint64_t* __restrict__ part_keys) {
@@ -334,13 +435,7 @@ __global__ __launch_bounds__(kThreads) void score_kernel(
   const typename E::type* src = x + row * stride;
   const int tid = threadIdx.x;
 
-  if constexpr (kTop) {
-    if (tid == 0) {
-      sh.have = sh.count = 0;
-      sh.least = -INFINITY;
-    }
-    __syncthreads();
-  }
+  typename std::conditional<kTop, Top<T, U>, NoTop>::type best(sh, k);
 
   Triple t = {-INFINITY, 0.f, 0.f};
   u32x4 next[U];
@@ -378,10 +473,7 @@ __global__ __launch_bounds__(kThreads) void score_kernel(
       }
     t.s += s;
     t.u += u;
-    if constexpr (kTop) {
-      if (__syncthreads_or(chunk_max > sh.least))
-        take_candidates<T, U>(sh, w, base, chunk_max, k);
-    }
+    if constexpr (kTop) best.take(w, base, chunk_max);
   }
 
   t = join_wave(t, c);
@@ -392,8 +484,9 @@ __global__ __launch_bounds__(kThreads) void score_kernel(
     parts[blockIdx.x].t = t;
   }
   if constexpr (kTop) {
+    best.finish();
     for (int i = tid; i < k; i += kThreads)
-      part_keys[(int64_t)blockIdx.x * k + i] = i < sh.have ? sh.keys[i] : 0;
+      part_keys[(int64_t)blockIdx.x * k + i] = i < best.have ? sh.keys[i] : 0;
   }
 }
 
@@ -408,23 +501,17 @@ __device__ Triple join_parts(const Part* parts, int splits, float c) {
 // ---------------------------------------------------------------------------
 // token log probabilities
 // ---------------------------------------------------------------------------
-// a wave a row: what needs no alternatives
+// a row's log probability, entropy and what its backward needs, by one
+// thread
 template <LmType T>
-__global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
-    const typename Elem<T>::type* __restrict__ x, int64_t stride,
-    int64_t rows, int64_t v, const int64_t* __restrict__ tokens,
-    int64_t ignore, float inv_t, float c, const Part* __restrict__ parts,
-    int splits, float* __restrict__ logprobs, float* __restrict__ entropy,
-    RowStats* __restrict__ stats) {
-  int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  Triple t = join_parts(parts + row * splits, splits, c);
-  if (threadIdx.x & 63) return;
-  int64_t token = tokens[row];
-  bool ignored = token == ignore;
-  bool outside = !ignored && (token < 0 || token >= v);
-  bool empty = t.m == -INFINITY && t.s == 0.f;
-  float log2_sum = log2f(t.s);
+__device__ void write_row(int64_t row, const typename Elem<T>::type* x,
+                          int64_t stride, int64_t v, const Triple& t,
+                          float log2_sum, int64_t token, int64_t ignore,
+                          float inv_t, float* logprobs, float* entropy,
+                          RowStats* stats) {
+  const bool ignored = token == ignore;
+  const bool outside = !ignored && (token < 0 || token >= v);
+  const bool empty = t.m == -INFINITY && t.s == 0.f;
   float lp, h;
   if (ignored) {
     lp = h = 0.f;
@@ -434,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
     lp = -INFINITY;
     h = 0.f;
   } else {
-    float xt = Elem<T>::load(x + row * stride + token);
+    const float xt = Elem<T>::load(x + row * stride + token);
     lp = (xt - t.m) * inv_t - log2_sum * kLn2;
     h = (log2_sum - t.u / t.s) * kLn2;
     if (!(t.s == t.s)) lp = NAN;
@@ -446,58 +533,100 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
                   ignored || (empty && !outside) ? 0.f : 1.f};
 }
 
-// a block a row: joins the parts' sorted lists of alternatives.
-// Of `splits` lists each element in place ceil(k / splits) or before: there
-// are k of them, so the least of these places' keys is a lower bound of the
-// k-th best; so is any list's own k-th. What passes both is ranked.
+// a wave a row, without alternatives
+template <LmType T>
+__global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride,
+    int64_t rows, int64_t v, const int64_t* __restrict__ tokens,
+    int64_t ignore, float inv_t, float c, const Part* __restrict__ parts,
+    int splits, float* __restrict__ logprobs, float* __restrict__ entropy,
+    RowStats* __restrict__ stats) {
+  int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const Triple t = join_parts(parts + row * splits, splits, c);
+  if ((threadIdx.x & 63) == 0)
+    write_row<T>(row, x, stride, v, t, log2f(t.s), tokens[row], ignore, inv_t,
+                 logprobs, entropy, stats);
+}
+
+// the r-th largest of the lanes' keys, 0 counting as none
+__device__ uint64_t rth_of_wave(uint64_t key, int lanes, int r) {
+  int not_less = 0;
+  for (int j = 0; j < lanes; j++) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)key, j);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(key >> 32), j);
+    not_less += ((uint64_t)hi << 32 | lo) >= key;
+  }
+  unsigned long long best = not_less >= r ? key : 0;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const unsigned long long o = __shfl_xor(best, d);
+    best = o > best ? o : best;
+  }
+  return best;
+}
+
+// A block a row, with alternatives: joins the parts' sorted lists. Where r
+// lists have a key of at least b in place p, there are r p such keys: so the
+// ceil(k / p)-th largest of the lists' keys in place p is a lower bound of
+// the k-th best key of all. Each wave finds the bound of another p; few keys
+// pass the largest of them, and these are ranked.
+template <LmType T>
 __global__ __launch_bounds__(kThreads) void top_rows_kernel(
-    const uint64_t* __restrict__ part_keys, const Part* __restrict__ parts,
-    int splits, int k, const int64_t* __restrict__ tokens, int64_t ignore,
-    float inv_t, float c, float* __restrict__ top_lp,
-    int64_t* __restrict__ top_ids) {
-  extern __shared__ uint64_t keys[];  // splits * k
-  __shared__ uint64_t best[kMaxTop];
-  __shared__ unsigned long long bound_all, bound_any;
+    const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
+    const int64_t* __restrict__ tokens, int64_t ignore, float inv_t, float c,
+    const Part* __restrict__ parts, const uint64_t* __restrict__ part_keys,
+    int splits, int k, float* __restrict__ logprobs,
+    float* __restrict__ entropy, float* __restrict__ top_lp,
+    int64_t* __restrict__ top_ids, RowStats* __restrict__ stats) {
+  constexpr int kMine = kMaxKeys / kThreads;
+  __shared__ uint64_t keys[kMaxKeys];
+  __shared__ uint64_t best[kMaxTop], bounds[kWaves];
   __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const uint64_t* src = part_keys + row * splits * k;
-  if (tid == 0) {
-    bound_all = ~0ull;
-    bound_any = 0;
-    count = 0;
-  }
+  const int all = splits * k;
+  uint64_t mine[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    mine[i] = tid + i * kThreads < all ? src[tid + i * kThreads] : 0;
+  // splits is 64 at most: a list a lane
+  const int place = min(k, (k + splits - 1) / splits << (tid >> 6));
+  const uint64_t bound_of_wave =
+      rth_of_wave(lane < splits ? src[lane * k + place - 1] : 0, splits,
+                  (k + place - 1) / place);
+  const Triple t = join_parts(parts + row * splits, splits, c);
+  const int64_t token = tokens[row];
+  if (lane == 0) bounds[tid >> 6] = bound_of_wave;
+  if (tid == 0) count = 0;
   if (tid < k) best[tid] = 0;
   __syncthreads();
-  const int place = (k + splits - 1) / splits - 1;
-  for (int i = tid; i < splits; i += kThreads) {
-    atomicMin(&bound_all, (unsigned long long)src[(int64_t)i * k + place]);
-    atomicMax(&bound_any, (unsigned long long)src[(int64_t)i * k + k - 1]);
-  }
-  __syncthreads();
-  uint64_t bound = bound_all > bound_any ? bound_all : bound_any;
-  if (!bound) bound = 1;  // none is no alternative
-  for (int i = tid; i < splits * k; i += kThreads) {
-    uint64_t key = src[i];
-    if (key >= bound) keys[atomicAdd(&count, 1)] = key;
-  }
+  uint64_t bound = 1;  // none is no alternative
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) bound = max(bound, bounds[i]);
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    if (mine[i] >= bound) keys[atomicAdd(&count, 1)] = mine[i];
   __syncthreads();
   const int n = count;
   for (int i = tid; i < n; i += kThreads) {
-    uint64_t key = keys[i];
+    const uint64_t key = keys[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; j++) rank += keys[j] > key;
     if (rank < k) best[rank] = key;
   }
+  const float log2_sum = log2f(t.s);
+  if (tid == 0)
+    write_row<T>(row, x, stride, v, t, log2_sum, token, ignore, inv_t,
+                 logprobs, entropy, stats);
   __syncthreads();
-  Triple t = join_parts(parts + row * splits, splits, c);
-  const float log_sum = log2f(t.s) * kLn2;
-  const bool ignored = tokens[row] == ignore;
-  for (int i = tid; i < k; i += kThreads) {
-    uint64_t key = ignored ? 0 : best[i];
-    top_lp[row * k + i] =
-        key ? (key_value(key) - t.m) * inv_t - log_sum : -INFINITY;
-    top_ids[row * k + i] = key ? (int64_t)key_index(key) : -1;
+  if (tid < k) {
+    const uint64_t key = token == ignore ? 0 : best[tid];
+    top_lp[row * k + tid] =
+        key ? (key_value(key) - t.m) * inv_t - log2_sum * kLn2 : -INFINITY;
+    top_ids[row * k + tid] = key ? (int64_t)key_index(key) : -1;
   }
 }
 
@@ -571,33 +700,22 @@ __device__ float load_any(LmType t, const void* p, int64_t i) {
   }
 }
 
-__device__ float wave_sum(float a) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
-  return a;
-}
-__device__ float wave_max(float a) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) a = fmaxf(a, __shfl_xor(a, d));
-  return a;
-}
+// a row by a wave: the teacher's softmax over its record, and
+// T^2 sum q (ln q - ln p). Returns (in every lane) the loss, and whether the
+// row has a record.
+struct RowLoss {
+  float loss;
+  bool there;
+};
 
-// a wave a row: the teacher's softmax over its record, and
-// T^2 sum q (ln q - ln p)
 template <LmType T>
-__global__ __launch_bounds__(kThreads) void distill_rows_kernel(
-    const typename Elem<T>::type* __restrict__ x, int64_t stride,
-    int64_t rows, int64_t v, LmType tt, const void* __restrict__ teacher,
-    const int64_t* __restrict__ ids, int k, float inv_t, float c,
-    const Part* __restrict__ parts, int splits, float* __restrict__ row_loss,
-    float* __restrict__ q, RowStats* __restrict__ stats) {
+__device__ RowLoss distill_row(
+    int64_t row, const typename Elem<T>::type* x, int64_t stride, int64_t v,
+    LmType tt, const void* teacher, const int64_t* ids, int k, float inv_t,
+    float c, const Part* parts, int splits, float* row_loss, float* q,
+    RowStats* stats) {
   constexpr int kMine = kMaxRecord / 64;
-  int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= rows) return;
   const int lane = threadIdx.x & 63;
-  Triple t = join_parts(parts + row * splits, splits, c);
-  const bool empty = t.m == -INFINITY && t.s == 0.f;
-  const float log2_sum = log2f(t.s);
   float z[kMine];
   int64_t id[kMine];
   float top = -INFINITY;
@@ -613,6 +731,13 @@ __global__ __launch_bounds__(kThreads) void distill_rows_kernel(
     top = fmaxf(top, z[i]);
   }
   bad = __any(bad);
+  float xs[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    xs[i] = id[i] != -1 && !bad ? Elem<T>::load(x + row * stride + id[i]) : 0.f;
+  const Triple t = join_parts(parts + row * splits, splits, c);
+  const bool empty = t.m == -INFINITY && t.s == 0.f;
+  const float log2_sum = log2f(t.s);
   top = wave_max(top);
   const bool absent = top == -INFINITY && !bad;
   float sum = 0.f;
@@ -629,29 +754,76 @@ __global__ __launch_bounds__(kThreads) void distill_rows_kernel(
     if (id[i] != -1 && !bad) {
       float lq = (z[i] - top) * c - log2_q;
       share = exp2_raw(lq);
-      float lp = empty ? -INFINITY
-                       : (Elem<T>::load(x + row * stride + id[i]) - t.m) * c -
-                             log2_sum;
+      float lp = empty ? -INFINITY : (xs[i] - t.m) * c - log2_sum;
       if (share > 0.f) loss = fmaf(share, lq - lp, loss);
     }
     if (at < k) q[row * k + at] = share;
   }
   loss = wave_sum(loss) * (kLn2 / (inv_t * inv_t));
+  loss = absent ? 0.f : bad ? NAN : loss;
   if (lane == 0) {
-    row_loss[row] = absent ? 0.f : bad ? NAN : loss;
-    stats[row] = {bad ? NAN : t.m, log2_sum, 0.f,
+    row_loss[row] = loss;
+    // in the entropy's place: whether the row counts in the mean
+    stats[row] = {bad ? NAN : t.m, log2_sum, absent ? 0.f : 1.f,
                   absent || (empty && !bad) ? 0.f : 1.f};
-    // a row counts in the mean where it has a record
-    stats[row].entropy = absent ? 0.f : 1.f;
+  }
+  return {loss, !absent};
+}
+
+// The waves' sums, in their order, by the block's first thread.
+__device__ void write_total(double s, double n, int mean, float* total,
+                            float* count) {
+  __shared__ double wave_s[16], wave_n[16];
+  const int waves = blockDim.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    wave_s[threadIdx.x >> 6] = s;
+    wave_n[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < waves; i++) {
+    s += wave_s[i];
+    n += wave_n[i];
+  }
+  const double by = mean && n > 1 ? n : 1;
+  *total = (float)(s / by);
+  *count = (float)by;
+}
+
+// kWhole: one block for all rows, which also adds them up
+template <LmType T, bool kWhole>
+__global__ __launch_bounds__(kWhole ? 1024 : kThreads) void
+distill_rows_kernel(
+    const typename Elem<T>::type* __restrict__ x, int64_t stride,
+    int64_t rows, int64_t v, LmType tt, const void* __restrict__ teacher,
+    const int64_t* __restrict__ ids, int k, float inv_t, float c,
+    const Part* __restrict__ parts, int splits, float* __restrict__ row_loss,
+    float* __restrict__ q, RowStats* __restrict__ stats, int mean,
+    float* __restrict__ total, float* __restrict__ count) {
+  const int64_t first =
+      (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  if constexpr (kWhole) {
+    double s = 0, n = 0;
+    for (int64_t row = first; row < rows; row += 16) {
+      const RowLoss r =
+          distill_row<T>(row, x, stride, v, tt, teacher, ids, k, inv_t, c,
+                         parts, splits, row_loss, q, stats);
+      s += r.loss;
+      n += r.there;
+    }
+    write_total(s, n, mean, total, count);
+  } else {
+    if (first < rows)
+      distill_row<T>(first, x, stride, v, tt, teacher, ids, k, inv_t, c, parts,
+                     splits, row_loss, q, stats);
   }
 }
 
 // sum or mean of the rows' losses, in a fixed order, in 64 bits; one block
 __global__ __launch_bounds__(1024) void distill_total_kernel(
     const float* __restrict__ row_loss, const RowStats* __restrict__ stats,
-    int64_t rows, int mean, float* __restrict__ total) {
-  __shared__ double wave_s[16];
-  __shared__ double wave_n[16];
+    int64_t rows, int mean, float* __restrict__ total,
+    float* __restrict__ count) {
   double s = 0, n = 0;
   for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     s += row_loss[i];
@@ -662,19 +834,7 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(
     s += __shfl_xor(s, d);
     n += __shfl_xor(n, d);
   }
-  if ((threadIdx.x & 63) == 0) {
-    wave_s[threadIdx.x >> 6] = s;
-    wave_n[threadIdx.x >> 6] = n;
-  }
-  __syncthreads();
-  if (threadIdx.x) return;
-  for (int i = 1; i < 16; i++) {
-    s += wave_s[i];
-    n += wave_n[i];
-  }
-  double by = mean && n > 1 ? n : 1;
-  total[0] = (float)(s / by);
-  total[1] = (float)by;
+  write_total(s, n, mean, total, count);
 }
 
 // dx_j = g T (p_j - sum of q at j). The block writes p_j of its chunk, and
@@ -752,7 +912,6 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
 // are kWant blocks, into parts of whole chunks.
 constexpr int64_t kWant = 1024;
 constexpr int64_t kMaxSplits = 64;
-constexpr int64_t kMaxKeys = 4096;  // that top_rows_kernel joins, 32 KB
 
 struct Plan {
   int unroll;        // words of 16 bytes a thread holds at a time
@@ -769,7 +928,7 @@ Plan plan_of(LmType t, int64_t rows, int64_t v, int top) {
   int64_t chunks = (v + chunk - 1) / chunk;
   int64_t splits = std::min(std::min(chunks, kMaxSplits),
                             std::max<int64_t>(1, kWant / rows));
-  if (top) splits = std::min(splits, kMaxKeys / top);
+  if (top) splits = std::min<int64_t>(splits, kMaxKeys / top);
   p.part_len = (chunks + splits - 1) / splits * chunk;
   p.splits = (v + p.part_len - 1) / p.part_len;
   return p;
@@ -844,19 +1003,17 @@ void launch_token_logprobs(LmType t, const void* x, int64_t stride,
   run_score<true>(t, x, stride, rows, v, p, c, top, parts, keys, stream);
   by_type(t, [&](auto type) {
     constexpr LmType T = decltype(type)::value;
-    logprobs_rows_kernel<T>
-        <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
-           stream>>>((const typename Elem<T>::type*)x, stride, rows, v,
-                     tokens, ignore, inv_t, c, parts, (int)p.splits, logprobs,
-                     entropy, stats);
+    auto* xt = (const typename Elem<T>::type*)x;
+    if (top)
+      top_rows_kernel<T><<<dim3((unsigned)rows), kThreads, 0, stream>>>(
+          xt, stride, v, tokens, ignore, inv_t, c, parts, keys, (int)p.splits,
+          top, logprobs, entropy, top_lp, top_ids, stats);
+    else
+      logprobs_rows_kernel<T>
+          <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
+             stream>>>(xt, stride, rows, v, tokens, ignore, inv_t, c, parts,
+                       (int)p.splits, logprobs, entropy, stats);
   });
-  if (top) {
-    top_rows_kernel<<<dim3((unsigned)rows), kThreads,
-                      (size_t)p.splits * top * 8, stream>>>(
-        keys, parts, (int)p.splits, top, tokens, ignore, inv_t, c, top_lp,
-        top_ids);
-    HIP_CHECK(hipGetLastError());
-  }
 }
 
 void launch_token_logprobs_bwd(LmType t, const void* x, int64_t stride,
@@ -882,23 +1039,30 @@ void launch_token_logprobs_bwd(LmType t, const void* x, int64_t stride,
 void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
                     int64_t v, LmType tt, const void* teacher,
                     const int64_t* ids, int k, float inv_t, float* row_loss,
-                    float* q, RowStats* stats, float* total, bool mean,
-                    void* ws, hipStream_t stream) {
+                    float* q, RowStats* stats, float* total, float* count,
+                    bool mean, void* ws, hipStream_t stream) {
   Plan p = plan_of(t, rows, v, 0);
   const float c = inv_t * kLog2e;
   Part* parts = (Part*)ws;
+  // up to 4 rows a wave a launch less is the shorter way
+  const bool whole = total && rows <= 64;
   run_score<false>(t, x, stride, rows, v, p, c, 0, parts, nullptr, stream);
   by_type(t, [&](auto type) {
     constexpr LmType T = decltype(type)::value;
-    distill_rows_kernel<T>
-        <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
-           stream>>>((const typename Elem<T>::type*)x, stride, rows, v, tt,
-                     teacher, ids, k, inv_t, c, parts, (int)p.splits,
-                     row_loss, q, stats);
+    auto go = [&](auto w) {
+      constexpr bool W = decltype(w)::value;
+      distill_rows_kernel<T, W>
+          <<<dim3(W ? 1 : (unsigned)((rows + kWaves - 1) / kWaves)),
+             W ? 1024 : kThreads, 0, stream>>>(
+              (const typename Elem<T>::type*)x, stride, rows, v, tt, teacher,
+              ids, k, inv_t, c, parts, (int)p.splits, row_loss, q, stats, mean,
+              total, count);
+    };
+    whole ? go(std::true_type{}) : go(std::false_type{});
   });
-  if (total) {
+  if (total && !whole) {
     distill_total_kernel<<<1, 1024, 0, stream>>>(row_loss, stats, rows, mean,
-                                                 total);
+                                                 total, count);
     HIP_CHECK(hipGetLastError());
   }
 }

@@ -36,14 +36,15 @@ TokenLogprobs = namedtuple(
 _functions = {}
 
 
-def _check_logits(logits):
-    torch = hiptorch.torch_tensor("logits", logits)
-    code = hiptorch.lm_code(torch, "logits", logits)
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits need a last axis, got {list(logits.shape)}")
-    if logits.shape[-1] >= 1 << 31:
+def _check_logits(logits) -> int:
+    hiptorch.check_tensor("logits", logits)
+    code = hiptorch.check_dtype("logits", logits.dtype)
+    shape = logits.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"logits need a last axis, got {list(shape)}")
+    if shape[-1] >= 1 << 31:
         raise ValueError("the last axis of logits is too long")
-    return torch, code
+    return code
 
 
 def _check_temperature(temperature) -> float:
@@ -54,15 +55,17 @@ def _check_temperature(temperature) -> float:
 
 
 def _check_ids(torch, name, ids, shape, device):
-    hiptorch.torch_tensor(name, ids)
-    if ids.dtype not in (torch.int64, torch.int32):
+    hiptorch.check_tensor(name, ids)
+    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
         raise TypeError(f"{name} must be int64 or int32, got {ids.dtype}")
     if ids.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got "
                          f"{list(ids.shape)}")
     if ids.device != device:
         raise ValueError(f"{name} are on {ids.device}, logits on {device}")
-    return ids.long().contiguous()
+    if ids.dtype != torch.int64:
+        ids = ids.long()
+    return ids.contiguous()
 
 
 def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
@@ -82,7 +85,8 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
     token is ``ignore_index`` is padding: 0, 0, (-inf, -1) and no gradient.
     A token outside of [0, v), or a NaN or +inf among the logits, gives NaN.
     """
-    torch, code = _check_logits(logits)
+    torch = hiptorch.lm_torch()
+    code = _check_logits(logits)
     t = _check_temperature(temperature)
     lead, v = logits.shape[:-1], logits.shape[-1]
     top = int(top)
@@ -92,10 +96,16 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
     if not logits.is_cuda:
         return _cpu_token_logprobs(torch, logits, tokens, top, t,
                                    int(ignore_index))
-    out = _function("logprobs", torch).apply(
-        logits, tokens, code, top, 1.0 / t, int(ignore_index))
+    f32 = torch.float32
+    top_lp = logits.new_empty((*lead, top), dtype=f32)
+    top_ids = tokens.new_empty((*lead, top))
+    args = (logits, tokens, top_lp, top_ids, code, 1.0 / t, int(ignore_index))
+    if logits.requires_grad and torch.is_grad_enabled():
+        logprobs, entropy = _function("logprobs", torch).apply(*args)
+    else:
+        logprobs, entropy, _ = _logprobs(torch, *args, False)
     STATS["token_logprobs"] += 1
-    return TokenLogprobs(*out)
+    return TokenLogprobs(logprobs, entropy, top_lp, top_ids)
 
 
 def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
@@ -118,33 +128,38 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
     A token outside of [0, v) but -1, or a NaN or +inf on either side, gives
     NaN.
     """
-    torch, code = _check_logits(logits)
+    torch = hiptorch.lm_torch()
+    code = _check_logits(logits)
     t = _check_temperature(temperature)
     lead = logits.shape[:-1]
-    hiptorch.torch_tensor("teacher_logits", teacher_logits)
-    t_code = hiptorch.lm_code(torch, "teacher_logits", teacher_logits)
-    if (teacher_logits.dim() != logits.dim()
-            or teacher_logits.shape[:-1] != lead
-            or not 1 <= teacher_logits.shape[-1] <= MAX_RECORD):
+    hiptorch.check_tensor("teacher_logits", teacher_logits)
+    t_code = hiptorch.check_dtype("teacher_logits", teacher_logits.dtype)
+    t_shape = teacher_logits.shape
+    if (len(t_shape) != len(lead) + 1 or t_shape[:-1] != lead
+            or not 1 <= t_shape[-1] <= MAX_RECORD):
         raise ValueError(
             f"teacher_logits must be [{', '.join(map(str, lead))}, k] with k "
-            f"from 1 to {MAX_RECORD}, got {list(teacher_logits.shape)}")
+            f"from 1 to {MAX_RECORD}, got {list(t_shape)}")
     if teacher_logits.device != logits.device:
         raise ValueError(f"teacher_logits are on {teacher_logits.device}, "
                          f"logits on {logits.device}")
-    if teacher_logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError("the teacher gets no gradient: detach its logits")
-    ids = _check_ids(torch, "teacher_tokens", teacher_tokens,
-                     teacher_logits.shape, logits.device)
+    if teacher_logits.requires_grad:
+        if torch.is_grad_enabled():
+            raise ValueError("the teacher gets no gradient: detach its logits")
+        teacher_logits = teacher_logits.detach()
+    ids = _check_ids(torch, "teacher_tokens", teacher_tokens, t_shape,
+                     logits.device)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got "
                          f"{reduction!r}")
     if not logits.is_cuda:
-        return _cpu_distill(torch, logits, teacher_logits.detach(), ids, t,
-                            reduction)
-    loss = _function("distill", torch).apply(
-        logits, teacher_logits.detach().contiguous(), ids, code, t_code,
-        1.0 / t, reduction)
+        return _cpu_distill(torch, logits, teacher_logits, ids, t, reduction)
+    args = (logits, teacher_logits.contiguous(), ids, code, t_code, 1.0 / t,
+            reduction)
+    if logits.requires_grad and torch.is_grad_enabled():
+        loss = _function("distill", torch).apply(*args)
+    else:
+        loss, _ = _distill(torch, *args)
     STATS["topk_distill_loss"] += 1
     return loss
 
@@ -152,6 +167,64 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
 # ---------------------------------------------------------------------------
 # GPU tensors
 # ---------------------------------------------------------------------------
+# Scratch comes from torch's allocator, on the stream that uses it: of a
+# captured graph, its own.
+_STATS_BYTES = 16  # what a row leaves for its backward
+
+
+def _logprobs(torch, logits, tokens, top_lp, top_ids, code, inv_t, ignore,
+              grad):
+    """(log probabilities, entropies, what the backward needs or None)."""
+    ext = hiptorch.ensure_hiplm()
+    x, stride = hiptorch.rows_view(logits)
+    rows, v = x.shape
+    top = top_ids.shape[-1]
+    lead = logits.shape[:-1]
+    logprobs = top_lp.new_empty(lead)
+    entropy = top_lp.new_empty(lead)
+    stats = top_lp.new_empty((rows, _STATS_BYTES // 4)) if grad else None
+    if rows:
+        work = x.new_empty((ext.score_workspace(code, rows, v, top),),
+                           dtype=torch.uint8)
+        with hiptorch.on_device(x) as stream:
+            ext.token_logprobs(
+                code, x.data_ptr(), stride, rows, v, tokens.data_ptr(),
+                ignore, inv_t, top, logprobs.data_ptr(), entropy.data_ptr(),
+                top_lp.data_ptr(), top_ids.data_ptr(),
+                stats.data_ptr() if grad else 0, work.data_ptr(), stream)
+    return logprobs, entropy, stats
+
+
+def _distill(torch, logits, teacher, ids, code, t_code, inv_t, reduction):
+    """(the loss, what the backward needs: the rows' numbers, the teacher's
+    shares, what the loss was divided by and the rows' losses, one behind the
+    other; None without rows)."""
+    ext = hiptorch.ensure_hiplm()
+    x, stride = hiptorch.rows_view(logits)
+    rows, v = x.shape
+    k = teacher.shape[-1]
+    f32 = torch.float32
+    whole = reduction != "none"
+    loss = x.new_empty(() if whole else logits.shape[:-1], dtype=f32)
+    if not rows:
+        return loss.zero_(), None
+    kept = loss.new_empty((rows * (_STATS_BYTES // 4 + k)
+                           + (1 + rows if whole else 0),))
+    stats = kept.data_ptr()
+    q = stats + rows * _STATS_BYTES
+    count = q + rows * k * 4
+    work = x.new_empty((ext.score_workspace(code, rows, v, 0),),
+                       dtype=torch.uint8)
+    with hiptorch.on_device(x) as stream:
+        ext.distill(
+            code, x.data_ptr(), stride, rows, v, t_code, teacher.data_ptr(),
+            ids.data_ptr(), k, inv_t,
+            count + 4 if whole else loss.data_ptr(), q, stats,
+            loss.data_ptr() if whole else 0, count if whole else 0,
+            reduction == "mean", work.data_ptr(), stream)
+    return loss, kept
+
+
 def _function(name, torch):
     """The autograd function of that name; made at its first use, since
     importing this module must not import torch."""
@@ -163,129 +236,82 @@ def _function(name, torch):
 def _make_functions(torch):
     from torch.autograd.function import once_differentiable
 
-    # floats that a row leaves for its backward
-    stats_len = 4
+    # what makes a second derivative an error costs time on every call, and
+    # is needed only where a graph of the backward is asked for
+    def once(backward):
+        slow = once_differentiable(backward)
 
-    def workspace(ext, code, rows, v, top, device):
-        need = ext.score_workspace(code, rows, v, top)
-        # from torch's allocator, on the stream that uses it: of a captured
-        # graph, its own
-        return torch.empty(need, dtype=torch.uint8, device=device)
+        def run(ctx, *grads):
+            if torch.is_grad_enabled():
+                return slow(ctx, *grads)
+            return backward(ctx, *grads)
+
+        return staticmethod(run)
 
     class TokenLogprobsFunction(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, logits, tokens, code, top, inv_t, ignore):
-            ext = hiptorch.ensure_hiplm()
-            lead, v = logits.shape[:-1], logits.shape[-1]
-            x, stride = hiptorch.rows_view(logits)
-            rows, device = x.shape[0], logits.device
-            f32 = torch.float32
-            logprobs = torch.empty(lead, dtype=f32, device=device)
-            entropy = torch.empty(lead, dtype=f32, device=device)
-            top_lp = torch.empty((*lead, top), dtype=f32, device=device)
-            top_ids = torch.empty((*lead, top), dtype=torch.int64,
-                                  device=device)
-            grad = ctx.needs_input_grad[0]
-            stats = None
-            if grad:
-                stats = torch.empty(rows, stats_len, dtype=f32,
-                                    device=device)
-            if rows:
-                work = workspace(ext, code, rows, v, top, device)
-                with hiptorch.on_device(torch, x) as stream:
-                    ext.token_logprobs(
-                        code, x.data_ptr(), stride, rows, v,
-                        tokens.data_ptr(), ignore, inv_t, top,
-                        logprobs.data_ptr(), entropy.data_ptr(),
-                        top_lp.data_ptr(), top_ids.data_ptr(),
-                        stats.data_ptr() if grad else 0, work.data_ptr(),
-                        stream)
-            ctx.mark_non_differentiable(top_lp, top_ids)
+        def forward(ctx, logits, tokens, top_lp, top_ids, code, inv_t,
+                    ignore):
+            logprobs, entropy, stats = _logprobs(
+                torch, logits, tokens, top_lp, top_ids, code, inv_t, ignore,
+                True)
             ctx.set_materialize_grads(False)
-            if grad:
-                ctx.save_for_backward(logits, tokens, stats)
-                ctx.code, ctx.inv_t = code, inv_t
-            return logprobs, entropy, top_lp, top_ids
+            ctx.save_for_backward(logits, tokens, stats)
+            ctx.code, ctx.inv_t = code, inv_t
+            return logprobs, entropy
 
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, g_lp, g_h, _top_lp, _top_ids):
+        @once
+        def backward(ctx, g_lp, g_h):
+            none = (None,) * 6
             if g_lp is None and g_h is None:
-                return (None,) * 6
+                return (None, *none)
             logits, tokens, stats = ctx.saved_tensors
             x, stride = hiptorch.rows_view(logits)
             rows, v = x.shape
-            dx = torch.empty(logits.shape, dtype=logits.dtype,
-                             device=logits.device)
+            dx = x.new_empty(logits.shape)
             if rows:
                 g_lp = None if g_lp is None else g_lp.contiguous()
                 g_h = None if g_h is None else g_h.contiguous()
-                with hiptorch.on_device(torch, x) as stream:
-                    hiptorch.ensure_hiplm().token_logprobs_bwd(
+                with hiptorch.on_device(x) as stream:
+                    _hiplm().token_logprobs_bwd(
                         ctx.code, x.data_ptr(), stride, rows, v,
                         tokens.data_ptr(), ctx.inv_t, stats.data_ptr(),
                         0 if g_lp is None else g_lp.data_ptr(),
                         0 if g_h is None else g_h.data_ptr(),
                         dx.data_ptr(), stream)
-            return dx, None, None, None, None, None
+            return (dx, *none)
 
     class DistillFunction(torch.autograd.Function):
         @staticmethod
         def forward(ctx, logits, teacher, ids, code, t_code, inv_t,
                     reduction):
-            ext = hiptorch.ensure_hiplm()
-            lead, v = logits.shape[:-1], logits.shape[-1]
-            x, stride = hiptorch.rows_view(logits)
-            rows, device = x.shape[0], logits.device
-            k = teacher.shape[-1]
-            f32 = torch.float32
-            if not rows:
-                ctx.empty = True
-                ctx.save_for_backward(logits)
-                return torch.zeros(lead if reduction == "none" else (),
-                                   dtype=f32, device=device)
-            ctx.empty = False
-            row_loss = torch.empty(lead, dtype=f32, device=device)
-            q = torch.empty(rows, k, dtype=f32, device=device)
-            stats = torch.empty(rows, stats_len, dtype=f32, device=device)
-            total = None
-            if reduction != "none":
-                # the result, and what it was divided by
-                total = torch.empty(2, dtype=f32, device=device)
-            work = workspace(ext, code, rows, v, 0, device)
-            with hiptorch.on_device(torch, x) as stream:
-                ext.distill(
-                    code, x.data_ptr(), stride, rows, v, t_code,
-                    teacher.data_ptr(), ids.data_ptr(), k, inv_t,
-                    row_loss.data_ptr(), q.data_ptr(), stats.data_ptr(),
-                    0 if total is None else total.data_ptr(),
-                    reduction == "mean", work.data_ptr(), stream)
-            if ctx.needs_input_grad[0]:
-                ctx.save_for_backward(logits, ids, q, stats, total)
-                ctx.code, ctx.inv_t = code, inv_t
-            return row_loss if total is None else total[0].clone()
+            loss, kept = _distill(torch, logits, teacher, ids, code, t_code,
+                                  inv_t, reduction)
+            ctx.save_for_backward(logits, ids, kept)
+            ctx.code, ctx.inv_t, ctx.whole = code, inv_t, reduction != "none"
+            return loss
 
-        @staticmethod
-        @once_differentiable
+        @once
         def backward(ctx, grad):
-            if ctx.empty:
-                (logits,) = ctx.saved_tensors
-                return (torch.zeros_like(logits),) + (None,) * 6
-            logits, ids, q, stats, total = ctx.saved_tensors
-            x, stride = hiptorch.rows_view(logits)
-            rows, v = x.shape
-            grad = grad.contiguous()
-            dx = torch.empty(logits.shape, dtype=logits.dtype,
-                             device=logits.device)
-            with hiptorch.on_device(torch, x) as stream:
-                hiptorch.ensure_hiplm().distill_bwd(
-                    ctx.code, x.data_ptr(), stride, rows, v, ids.data_ptr(),
-                    q.data_ptr(), q.shape[1], ctx.inv_t, stats.data_ptr(),
-                    grad.data_ptr(), 1 if total is None else 0,
-                    0 if total is None else total.data_ptr() + 4,
-                    dx.data_ptr(), stream)
+            logits, ids, kept = ctx.saved_tensors
+            dx = logits.new_empty(logits.shape)
+            if kept is not None:
+                x, stride = hiptorch.rows_view(logits)
+                rows, v = x.shape
+                k = ids.shape[-1]
+                grad = grad.contiguous()
+                stats = kept.data_ptr()
+                q = stats + rows * _STATS_BYTES
+                with hiptorch.on_device(x) as stream:
+                    _hiplm().distill_bwd(
+                        ctx.code, x.data_ptr(), stride, rows, v,
+                        ids.data_ptr(), q, k, ctx.inv_t, stats,
+                        grad.data_ptr(), 0 if ctx.whole else 1,
+                        q + rows * k * 4 if ctx.whole else 0, dx.data_ptr(),
+                        stream)
             return (dx,) + (None,) * 6
 
+    _hiplm = hiptorch.ensure_hiplm
     _functions["logprobs"] = TokenLogprobsFunction
     _functions["distill"] = DistillFunction
 

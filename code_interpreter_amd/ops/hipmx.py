@@ -45,11 +45,9 @@ class MXFP4Tensor:
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes, scales, k: int):
-        import torch
-
-        if not (isinstance(codes, torch.Tensor)
-                and isinstance(scales, torch.Tensor)):
-            raise TypeError("codes and scales must be tensors")
+        torch = hiptorch.lm_torch()
+        hiptorch.check_tensor("codes", codes)
+        hiptorch.check_tensor("scales", scales)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales must be uint8, got "
                             f"{codes.dtype} and {scales.dtype}")
@@ -68,9 +66,11 @@ class MXFP4Tensor:
         codes = codes.contiguous()
         if codes.data_ptr() % 16:
             codes = codes.clone()
-        self.codes = codes
-        self.scales = scales.contiguous()
-        self.shape = torch.Size((*lead, k))
+        self._set(codes, scales.contiguous(), torch.Size((*lead, k)))
+
+    def _set(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, shape
+        return self
 
     @property
     def device(self):
@@ -107,43 +107,42 @@ class MXFP4Tensor:
 def quantize(x) -> MXFP4Tensor:
     """x ([..., k], float32, bfloat16 or float16) in microscaled 4-bit form.
     The result is data: it carries no gradient."""
-    torch = hiptorch.torch_tensor("x", x)
-    code = hiptorch.lm_code(torch, "x", x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x needs a last axis, got {list(x.shape)}")
-    lead, k = x.shape[:-1], x.shape[-1]
+    torch = hiptorch.lm_torch()
+    hiptorch.check_tensor("x", x)
+    code = hiptorch.check_dtype("x", x.dtype)
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"x needs a last axis, got {list(shape)}")
+    lead, k = shape[:-1], shape[-1]
     nb = _blocks(k)
     if not x.is_cuda:
         return MXFP4Tensor(*_cpu_quantize(torch, x.detach()), k)
     ext = hiptorch.ensure_hiplm()
     x2, stride = hiptorch.rows_view(x)
     rows = x2.shape[0]
-    codes = torch.empty((*lead, nb * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, nb), dtype=torch.uint8, device=x.device)
+    u8 = torch.uint8
+    codes = x.new_empty((*lead, nb * 16), dtype=u8)
+    scales = x.new_empty((*lead, nb), dtype=u8)
     if rows:
-        with hiptorch.on_device(torch, x) as stream:
+        with hiptorch.on_device(x) as stream:
             ext.mx_quantize(code, x2.data_ptr(), stride, codes.data_ptr(),
                             scales.data_ptr(), rows, k, stream)
     STATS["quantize"] += 1
-    return MXFP4Tensor(codes, scales, k)
+    return MXFP4Tensor.__new__(MXFP4Tensor)._set(codes, scales, shape)
 
 
 def _dequantize(q: MXFP4Tensor, dtype=None):
-    import torch
-
+    torch = hiptorch.lm_torch()
     dtype = torch.bfloat16 if dtype is None else dtype
-    code = hiptorch.LM_CODES(torch).get(dtype)
-    if code is None:
-        raise TypeError("dtype must be float32, bfloat16 or float16, "
-                        f"got {dtype}")
+    code = hiptorch.check_dtype("dtype", dtype)
     if not q.codes.is_cuda:
         return _cpu_dequantize(torch, q).to(dtype)
     ext = hiptorch.ensure_hiplm()
     k = q.shape[-1]
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = q.codes.new_empty(q.shape, dtype=dtype)
     rows = out.numel() // k
     if rows:
-        with hiptorch.on_device(torch, out) as stream:
+        with hiptorch.on_device(out) as stream:
             ext.mx_dequantize(code, q.codes.data_ptr(), q.scales.data_ptr(),
                               out.data_ptr(), rows, k, stream)
     STATS["dequantize"] += 1
@@ -160,57 +159,55 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
     result is rounded once. There is no backward: tensors that require a
     gradient are refused while gradients are enabled.
     """
-    import torch
-
+    torch = hiptorch.lm_torch()
     if not isinstance(weight, MXFP4Tensor):
         raise TypeError("weight must be an MXFP4Tensor, got "
                         f"{type(weight).__name__}")
     if len(weight.shape) != 2:
         raise ValueError(f"weight must be [n, k], got {list(weight.shape)}")
+    n, k = weight.shape
+    wcodes = weight.codes
     packed = isinstance(input, MXFP4Tensor)
     if packed:
         dtype = torch.bfloat16 if dtype is None else dtype
-        code = hiptorch.LM_CODES(torch).get(dtype)
-        if code is None:
-            raise TypeError("dtype must be float32, bfloat16 or float16, "
-                            f"got {dtype}")
+        code = hiptorch.check_dtype("dtype", dtype)
+        data = input.codes
     else:
-        hiptorch.torch_tensor("input", input)
-        code = hiptorch.lm_code(torch, "input", input)
+        hiptorch.check_tensor("input", input)
+        code = hiptorch.check_dtype("input", input.dtype)
         if dtype is not None and dtype != input.dtype:
             raise TypeError("dtype is for an MXFP4Tensor input: a tensor's "
                             "own type is the result's")
         dtype = input.dtype
-        if input.dim() < 1:
-            raise ValueError("input needs a last axis")
-    n, k = weight.shape
-    if input.shape[-1] != k:
-        raise ValueError(f"input {list(input.shape)} and weight "
+        data = input
+    shape = input.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"input {list(shape)} and weight "
                          f"{list(weight.shape)} differ in their last axis")
-    device = weight.codes.device
-    if input.device != device:
-        raise ValueError(f"input is on {input.device}, weight on {device}")
+    if data.device != wcodes.device:
+        raise ValueError(f"input is on {data.device}, weight on "
+                         f"{wcodes.device}")
     if bias is not None:
-        hiptorch.torch_tensor("bias", bias)
-        if bias.dtype != dtype or bias.shape != (n,) or bias.device != device:
+        hiptorch.check_tensor("bias", bias)
+        if (bias.dtype != dtype or bias.shape != (n,)
+                or bias.device != wcodes.device):
             raise ValueError(
-                f"bias must be [{n}], {dtype}, on {device}, got "
+                f"bias must be [{n}], {dtype}, on {wcodes.device}, got "
                 f"{list(bias.shape)}, {bias.dtype}, on {bias.device}")
-    if torch.is_grad_enabled() and (
-        (not packed and input.requires_grad)
-        or (bias is not None and bias.requires_grad)
-    ):
-        raise RuntimeError("hipmx.linear has no backward: call it under "
-                           "torch.no_grad(), or detach its inputs")
-    lead = input.shape[:-1]
-    if not weight.codes.is_cuda:
+    if ((not packed and input.requires_grad)
+            or (bias is not None and bias.requires_grad)):
+        if torch.is_grad_enabled():
+            raise RuntimeError("hipmx.linear has no backward: call it under "
+                               "torch.no_grad(), or detach its inputs")
+    lead = shape[:-1]
+    if not wcodes.is_cuda:
         q = input if packed else quantize(input)
         y = _cpu_dequantize(torch, q) @ _cpu_dequantize(torch, weight).T
         if bias is not None:
             y = y + bias.detach().float()
         return y.to(dtype)
     ext = hiptorch.ensure_hiplm()
-    y = torch.empty((*lead, n), dtype=dtype, device=device)
+    y = wcodes.new_empty((*lead, n), dtype=dtype)
     m = 1
     for d in lead:
         m *= d
@@ -218,7 +215,7 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
         return y
     if packed:
         x_ptr = stride = 0
-        xc, xs = input.codes.data_ptr(), input.scales.data_ptr()
+        xc, xs = data.data_ptr(), input.scales.data_ptr()
     else:
         x2, stride = hiptorch.rows_view(input)
         x_ptr, xc, xs = x2.data_ptr(), 0, 0
@@ -227,15 +224,16 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
         bias = bias.contiguous()
         b_ptr = bias.data_ptr()
     need = ext.mx_linear_workspace(m, n, k, packed)
-    # from torch's allocator, on the stream that uses it: of a captured
-    # graph, its own
-    work = None
+    w_ptr = 0
     if need:
-        work = torch.empty(need, dtype=torch.uint8, device=device)
-    with hiptorch.on_device(torch, y) as stream:
-        ext.mx_linear(code, x_ptr, stride, xc, xs, weight.codes.data_ptr(),
+        # from torch's allocator, on the stream that uses it: of a captured
+        # graph, its own
+        work = wcodes.new_empty((need,))
+        w_ptr = work.data_ptr()
+    with hiptorch.on_device(y) as stream:
+        ext.mx_linear(code, x_ptr, stride, xc, xs, wcodes.data_ptr(),
                       weight.scales.data_ptr(), b_ptr, y.data_ptr(), m, n, k,
-                      0 if work is None else work.data_ptr(), stream)
+                      w_ptr, stream)
     STATS["linear"] += 1
     return y
 

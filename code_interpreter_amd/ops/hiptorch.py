@@ -70,70 +70,80 @@ def ensure_hiplm():
 
 
 # ---------------------------------------------------------------------------
-# what the explicit operators (hipmx, hiplm) share
+# what the explicit operators (hipmx, hiplm) share; kept short, since for one
+# token's worth of work the host's part is the longer one
 # ---------------------------------------------------------------------------
-_lm_codes = {}
+_lm_codes = {}  # the kernels' code of each type that they take
+_raw = {}       # torch's own handles of the current device and stream
 
 
-def LM_CODES(torch) -> dict:
-    """The kernels' code of each type that they take."""
-    if not _lm_codes:
-        _lm_codes.update({torch.float32: 0, torch.bfloat16: 1,
-                          torch.float16: 2})
-    return _lm_codes
-
-
-def torch_tensor(name, x):
-    """torch, where x is a tensor; a TypeError that names it otherwise."""
+def lm_torch():
+    """torch, with the tables above filled."""
     import torch
 
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
-    if x.layout != torch.strided:
-        raise TypeError(f"{name} must be a strided tensor, got {x.layout}")
+    if not _raw:
+        _lm_codes.update({torch.float32: 0, torch.bfloat16: 1,
+                          torch.float16: 2})
+        _raw["tensor"] = torch.Tensor
+        _raw["strided"] = torch.strided
+        _raw["set"] = torch.cuda.set_device
+        # the public calls make an object each time: these are their cores
+        _raw["device"] = getattr(torch._C, "_cuda_getDevice",
+                                 torch.cuda.current_device)
+        _raw["stream"] = getattr(
+            torch._C, "_cuda_getCurrentRawStream",
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
     return torch
 
 
-def lm_code(torch, name, x) -> int:
-    code = LM_CODES(torch).get(x.dtype)
+def check_tensor(name, x):
+    """A TypeError that names x where it is no strided tensor."""
+    if not isinstance(x, _raw["tensor"]):
+        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
+    if x.layout is not _raw["strided"]:
+        raise TypeError(f"{name} must be a strided tensor, got {x.layout}")
+
+
+def check_dtype(name, dtype) -> int:
+    code = _lm_codes.get(dtype)
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got "
-                        f"{x.dtype}")
+                        f"{dtype}")
     return code
 
 
 def rows_view(x):
     """x as [rows, k] with neighbouring elements in a row, and the distance
     of its rows: a view where its strides allow one, else a copy."""
-    k = x.shape[-1]
-    rows = 1
-    for d in x.shape[:-1]:
-        rows *= d
-    x2 = x if x.dim() == 2 else x.reshape(rows, k)
-    if k > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    return x2, (x2.stride(0) if rows > 1 else k)
+    if x.dim() != 2:
+        k = x.shape[-1]
+        x = x.reshape(x.numel() // k, k)
+    stride, inner = x.stride()
+    rows, k = x.shape
+    if inner != 1 and k > 1:
+        x = x.contiguous()
+        stride = k
+    return x, (stride if rows > 1 else k)
 
 
 class on_device:
     """Makes x's device the current one while kernels are launched on it, and
     gives its current stream."""
 
-    __slots__ = ("_torch", "_index", "_before")
+    __slots__ = ("_index", "_before")
 
-    def __init__(self, torch, x):
-        self._torch, self._index = torch, x.device.index
+    def __init__(self, x):
+        self._index = x.get_device()
 
     def __enter__(self):
-        cuda = self._torch.cuda
-        self._before = cuda.current_device()
-        if self._before != self._index:
-            cuda.set_device(self._index)
-        return cuda.current_stream(self._index).cuda_stream
+        before = self._before = _raw["device"]()
+        if before != self._index:
+            _raw["set"](self._index)
+        return _raw["stream"](self._index)
 
     def __exit__(self, *_):
         if self._before != self._index:
-            self._torch.cuda.set_device(self._before)
+            _raw["set"](self._before)
 
 
 # route only when the kernel launch is worth more than its overhead;

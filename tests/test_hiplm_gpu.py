@@ -460,7 +460,7 @@ def test_kernels_write_their_results_alone(lm, rows, v, top):
     q, total = buffer(4 * rows * k), buffer(8)
     ext.distill(1, x.data_ptr(), v, rows, v, 0, teacher.data_ptr(),
                 ids.data_ptr(), k, 1.0, buffer(4 * rows), q, stats, total,
-                True, buffer(ext.score_workspace(1, rows, v, 0)), stream)
+                total + 4, True, buffer(ext.score_workspace(1, rows, v, 0)), stream)
     ext.distill_bwd(1, x.data_ptr(), v, rows, v, ids.data_ptr(), q, k, 1.0,
                     stats, g.data_ptr(), 0, total + 4, buffer(2 * rows * v),
                     stream)

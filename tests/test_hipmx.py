@@ -177,7 +177,7 @@ def test_parts_are_checked_and_shared():
             hipmx.MXFP4Tensor(*bad)
     with pytest.raises(TypeError, match="uint8"):
         hipmx.MXFP4Tensor(q.codes.int(), q.scales, 40)
-    with pytest.raises(TypeError, match="tensors"):
+    with pytest.raises(TypeError, match="codes must be a tensor"):
         hipmx.MXFP4Tensor(q.codes.numpy(), q.scales, 40)
     # parts cut out of larger ones
     big = torch.zeros(3, 64, dtype=torch.uint8)
