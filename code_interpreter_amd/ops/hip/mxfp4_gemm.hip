@@ -94,9 +94,15 @@ __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
   const int t0 = blk % parts * kLaySteps;
   if (row >= rows) return;
   const uint8_t* p = from + row * nb;
-  for (int t = t0; t < min(steps, t0 + kLaySteps); t++)
-    to[t * rows + row] = {load_scales(p, t * 8, nb),
-                          load_scales(p, t * 8 + 4, nb)};
+  uint2 v[kLaySteps];
+#pragma unroll
+  for (int i = 0; i < kLaySteps; i++)
+    if (t0 + i < steps)
+      v[i] = {load_scales(p, (t0 + i) * 8, nb),
+              load_scales(p, (t0 + i) * 8 + 4, nb)};
+#pragma unroll
+  for (int i = 0; i < kLaySteps; i++)
+    if (t0 + i < steps) to[(t0 + i) * rows + row] = v[i];
 }
 
 // blocks [0, x_blocks): x to codes and laid out scales, or (packed) its
@@ -185,7 +191,8 @@ __global__ __launch_bounds__(WM* WN * 64, 1) void tile_kernel(
   const int64_t m0 = (int64_t)(group * 8 + (id % per) % high) * BM;
   const int64_t n0 = (int64_t)((id % per) / high) * BN;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int l31 = lane & 31, h = lane >> 5;
   const int64_t row_bytes = (int64_t)nb * kMxBytes;
@@ -431,10 +438,191 @@ __global__ __launch_bounds__(WM* WN * 64, 1) void tile_kernel(
 }
 
 // ---------------------------------------------------------------------------
+// small tiles: where there are too few large ones to fill the chip
+// ---------------------------------------------------------------------------
+// The time is the memory's answer, not the products': so a block keeps the
+// loads of kStages - 1 steps under way, in a ring of buffers, and small tiles
+// make many blocks. 4 waves make a tile of 32 WM tokens x 32 WN outputs; of
+// the 4 instructions of a step WK waves take a share each, and their sums are
+// added in a fixed order at the end. Rows stand in shared memory as for the
+// large tiles; the scales of a step come the same way, 4 bytes a lane.
+template <LmType T, int WM, int WN, int WK, int kStages>
+__global__ __launch_bounds__(256) void small_kernel(
+    const uint8_t* __restrict__ xc, const uint2* __restrict__ xs,
+    const uint8_t* __restrict__ wc, const uint2* __restrict__ ws,
+    const void* __restrict__ bias, void* __restrict__ y, int64_t m, int64_t n,
+    int nb, int tiles_m, int tiles_n) {
+#ifdef __HIP_DEVICE_COMPILE__  // buffer descriptors are no type on the host
+  static_assert(WM * WN * WK == 4, "");
+  constexpr int BM = WM * 32, BN = WN * 32;
+  constexpr int kRow = 128;
+  constexpr int kScales = (BM + BN) * kRow;  // behind the rows
+  constexpr int kBuf = kScales + 1024;
+  constexpr int kLoads = (BM + BN) / 32;  // of a wave, 8 rows each
+  constexpr int kPerStep = kLoads + 1;    // with one of scales
+  constexpr int kWait = (kStages - 2) * kPerStep;
+  static_assert(kWait < 64, "");
+  constexpr int kOut = BN + 4;  // floats between tokens in the epilogue
+  static_assert(WK * BM * kOut * 4 <= kStages * kBuf, "");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+
+  int id = blockIdx.x;
+  {  // neighbouring tiles to one chiplet, columns of 8 tiles of tokens
+    const int all = tiles_m * tiles_n, q = all / 8, r = all % 8;
+    const int xcd = id % 8, idx = id / 8;
+    id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  }
+  const int per = 8 * tiles_n, group = id / per;
+  const int high = min(8, tiles_m - group * 8);
+  const int64_t m0 = (int64_t)(group * 8 + (id % per) % high) * BM;
+  const int64_t n0 = (int64_t)((id % per) / high) * BN;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
+  const int l31 = lane & 31, h = lane >> 5;
+  const int64_t row_bytes = (int64_t)nb * kMxBytes;
+  const int full = nb / 8, rest = nb % 8;
+  const int steps = full + (rest != 0);
+
+  auto buffer = [](const void* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void*)p, 0, (int)min(bytes, (int64_t)0xFFFFFFFF), 0x00020000);
+  };
+  const auto wr = buffer(wc + n0 * row_bytes,
+                         min(n - n0, (int64_t)BN) * row_bytes);
+  const auto xr = buffer(xc + m0 * row_bytes,
+                         min(m - m0, (int64_t)BM) * row_bytes);
+  // rows of the weight first, then of the tokens; 8 of one operand a load
+  const int unit = (lane & 7) ^ (((wave & 1) * 4 + (lane >> 4)) & 7);
+  const int back = rest && unit >= rest ? (unit - rest + 1) * 16 : 0;
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; i++) {
+    const int64_t r = (i * 4 + wave) * 8 + (lane >> 3);
+    const int64_t at = i * 32 < BN ? min(r, n - 1 - n0)
+                                   : min(r - BN, m - 1 - m0);
+    off[i] = (uint32_t)(at * row_bytes) + unit * 16;
+  }
+  // scales: words 2 r, 2 r + 1 of row r. A wave behind the last word loads
+  // the first ones once more, to a place that is not read. Rows behind the
+  // operand's last one get some other row's, or 0: they are not stored.
+  constexpr int kScaleWaves = (BM + BN) * 2 / 64;
+  const int word0 = (wave % kScaleWaves) * 64;
+  const bool of_x = word0 >= BN * 2;
+  const auto sr = of_x ? buffer(xs, m * steps * 8) : buffer(ws, n * steps * 8);
+  const int sstep = (int)(of_x ? m : n) * 8;
+  const int soff = (int)(of_x ? m0 : n0) * 8 +
+                   (word0 + lane - (of_x ? BN * 2 : 0)) * 4;
+
+  auto stage = [&](int t, int into) {
+    char* to = smem + into * kBuf;
+    const int less = t == full ? back : 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      lds_void* at = (lds_void*)(to + (i * 4 + wave) * 1024);
+      if (i * 32 < BN)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            wr, at, 16, (int)off[i] - less, t * kRow, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            xr, at, 16, (int)off[i] - less, t * kRow, 0, 0);
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        sr, (lds_void*)(to + kScales + wave * 256), 4, soff, t * sstep, 0, 0);
+  };
+
+  v16f acc = {};
+  const int aw = (wn * 32 + l31) * kRow, ax = (BN + wm * 32 + l31) * kRow;
+  const int sw = kScales + (wn * 32 + l31) * 8 + 4 * h;
+  const int sx = kScales + (BN + wm * 32 + l31) * 8 + 4 * h;
+  auto multiply = [&](int at, auto last) {
+    const char* from = smem + at * kBuf;
+    // a wave's instructions are wk * 4 / WK and those behind it: their scales
+    // are shifted to the front of the word
+    const uint32_t s0 = *(const uint32_t*)(from + sw) >> (wk * 4 / WK * 8);
+    const uint32_t s1 = *(const uint32_t*)(from + sx) >> (wk * 4 / WK * 8);
+    auto one = [&](auto step) {
+      constexpr int s = decltype(step)::value;
+      const int blk = wk * 4 / WK + s;
+      if (decltype(last)::value && blk >= rest) return;
+      const int u = ((blk + 4 * h) ^ (lane >> 1 & 7)) * 16;
+      u32x4 w = *(const u32x4*)(from + aw + u);
+      u32x4 x = *(const u32x4*)(from + ax + u);
+      if (decltype(last)::value && blk + 4 * h >= rest)
+        w = x = u32x4{0, 0, 0, 0};
+      acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          operand(w), operand(x), acc, 4, 4, s, (int)s0, s, (int)s1);
+    };
+    one(std::integral_constant<int, 0>{});
+    if constexpr (WK < 4) one(std::integral_constant<int, 1>{});
+    if constexpr (WK < 2) {
+      one(std::integral_constant<int, 2>{});
+      one(std::integral_constant<int, 3>{});
+    }
+  };
+
+  // Behind the last step the last one is loaded again, into buffers that are
+  // free, so that the number of loads under way is always the same.
+#pragma unroll
+  for (int t = 0; t < kStages - 1; t++) stage(min(t, steps - 1), t);
+  auto arrive = [] {
+    // this wave's loads of a step have landed; behind the barrier every
+    // wave's, and the step before is read
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((kWait & 15) | 7 << 4 | 15 << 8 |
+                               (kWait >> 4) << 14);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  int now = 0, into = kStages - 1;
+  for (int t = 0; t < full; t++) {
+    arrive();
+    stage(min(t + kStages - 1, steps - 1), into);
+    multiply(now, std::false_type{});
+    now = now + 1 == kStages ? 0 : now + 1;
+    into = into + 1 == kStages ? 0 : into + 1;
+  }
+  if (rest) {
+    arrive();
+    multiply(now, std::true_type{});
+  }
+
+  // the waves' sums as [wk][token][output]
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  float* sums = (float*)smem;
+  float* mine = sums + (wk * BM + wm * 32 + l31) * kOut + wn * 32 + 4 * h;
+#pragma unroll
+  for (int g = 0; g < 4; g++)
+    *(v4f*)(mine + 8 * g) = v4f{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2],
+                                acc[4 * g + 3]};
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < BM * BN / 1024; i++) {
+    const int e = (i * 256 + threadIdx.x) * 4;
+    const int64_t row = m0 + e / BN, col = n0 + e % BN;
+    const int valid = (int)min((int64_t)4, n - col);
+    if (row >= m || valid <= 0) continue;
+    v4f sum = *(const v4f*)(sums + e / BN * kOut + e % BN);
+#pragma unroll
+    for (int k = 1; k < WK; k++)
+      sum += *(const v4f*)(sums + (k * BM + e / BN) * kOut + e % BN);
+    float f[4];
+    for (int r = 0; r < 4; r++)
+      f[r] = sum[r] + (bias && r < valid ? bias_at<T>(bias, col + r) : 0.f);
+    store4<T>(y, row * n + col, f, valid);
+  }
+#endif
+}
+
+// ---------------------------------------------------------------------------
 // few tokens
 // ---------------------------------------------------------------------------
 // The weights are read once, from memory into registers, and bound the time;
-// 16 * MT tokens are held against them. A block makes 16 outputs of all
+// up to 16 tokens are held against them. A block makes 16 outputs of all
 // tokens: its 8 waves take turns along k, 512 elements a turn, and add up
 // through shared memory at the end, in a fixed order. The loads of two turns
 // are under way before the first is worked on. The tokens come from memory
@@ -479,7 +667,7 @@ __device__ __forceinline__ void load_turn(const uint8_t* codes,
   }
 }
 
-template <LmType T, int MT, bool kPacked>
+template <LmType T, bool kPacked>
 __global__ __launch_bounds__(512) void few_kernel(
     const void* __restrict__ x, int64_t stride,
     const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs,
@@ -507,15 +695,28 @@ __global__ __launch_bounds__(512) void few_kernel(
   uint8_t* lds_s = (uint8_t*)smem + m * crow;
   if constexpr (!kPacked) {
     const uint32_t per_row = (uint32_t)nb * 4, groups = per_row * m;
-    for (uint32_t g = threadIdx.x; g < groups; g += 512) {
-      const uint32_t row = g / per_row, col = g - row * per_row;
-      u32x4 w, w2;
-      load8<T>((const char*)x + row * stride * Size<T>::value,
-               (int64_t)col * kPer, k, w, w2);
-      uint32_t byte = block_scale<T>(w, w2);
-      *(uint32_t*)(smem + row * crow + col * 4) =
-          byte == 255 ? 0u : encode<T>(w, w2, scale_value(byte));
-      if ((g & 3) == 0) lds_s[row * sstride + (col >> 2)] = (uint8_t)byte;
+    constexpr int kGroups = 4;  // loads under way
+    for (uint32_t g0 = threadIdx.x; g0 < groups; g0 += 512 * kGroups) {
+      u32x4 w[kGroups], w2[kGroups];
+      uint32_t row[kGroups], col[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; i++) {
+        const uint32_t g = g0 + i * 512;
+        row[i] = g / per_row;
+        col[i] = g - row[i] * per_row;
+        if (g < groups)
+          load8<T>((const char*)x + row[i] * stride * Size<T>::value,
+                   (int64_t)col[i] * kPer, k, w[i], w2[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kGroups; i++) {
+        if (g0 + i * 512 >= groups) break;  // whole blocks: a multiple of 4
+        const uint32_t byte = block_scale<T>(w[i], w2[i]);
+        *(uint32_t*)(smem + row[i] * crow + col[i] * 4) =
+            byte == 255 ? 0u : encode<T>(w[i], w2[i], scale_value(byte));
+        if ((col[i] & 3) == 0)
+          lds_s[row[i] * sstride + (col[i] >> 2)] = (uint8_t)byte;
+      }
     }
     // scales of 1 up to the end of a row's last turn
     for (uint32_t g = threadIdx.x; g < 16u * m; g += 512) {
@@ -525,64 +726,71 @@ __global__ __launch_bounds__(512) void few_kernel(
     __syncthreads();
   }
 
-  v4f acc[MT] = {};
+  v4f acc = {};
+  const int token = min(l15, m - 1);
   for (int turn = wave; turn < turns; turn += kWaves) {
     Turn now = next;
     next = after;
     if (turn + 2 * kWaves < turns)
       load_turn<true>(wrow, srow, (turn + 2 * kWaves) * 16, nb, q, after);
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-      const int token = min(i * 16 + l15, m - 1);
-      Turn tok;
-      if constexpr (kPacked) {
-        load_turn<true>(xc + (int64_t)token * nb * 16, xs + (int64_t)token * nb,
-                        turn * 16, nb, q, tok);
-      } else {
-        load_turn<false>((const uint8_t*)smem + token * crow, nullptr,
-                         turn * 16, nb, q, tok);
-        tok.s = *(const u32x4*)(lds_s + token * sstride + turn * 16);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            operand(now.c[j]), operand(tok.c[j]), acc[i], 4, 4, 0,
-            (int)(now.s[j] >> (8 * q)), 0, (int)(tok.s[j] >> (8 * q)));
+    Turn tok;
+    if constexpr (kPacked) {
+      load_turn<true>(xc + (int64_t)token * nb * 16, xs + (int64_t)token * nb,
+                      turn * 16, nb, q, tok);
+    } else {
+      load_turn<false>((const uint8_t*)smem + token * crow, nullptr, turn * 16,
+                       nb, q, tok);
+      tok.s = *(const u32x4*)(lds_s + token * sstride + turn * 16);
     }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          operand(now.c[j]), operand(tok.c[j]), acc, 4, 4, 0,
+          (int)(now.s[j] >> (8 * q)), 0, (int)(tok.s[j] >> (8 * q)));
   }
 
   __syncthreads();  // the tokens' place is taken by the partial sums
-  v4f* part = (v4f*)smem;  // [wave][MT][64]
-#pragma unroll
-  for (int i = 0; i < MT; i++) part[(wave * MT + i) * 64 + lane] = acc[i];
+  v4f* part = (v4f*)smem;  // [wave][64]
+  part[threadIdx.x] = acc;
   __syncthreads();
-  for (int e = threadIdx.x; e < MT * 64; e += 512) {
-    const int token = (e >> 6) * 16 + (e & 15);
-    const int64_t col = n0 + 4 * ((e & 63) >> 4);
-    const int valid = (int)min((int64_t)4, n - col);
-    if (token >= m || valid <= 0) continue;
-    v4f sum = part[e];
-    for (int w = 1; w < kWaves; w++) sum += part[w * MT * 64 + e];
-    float f[4];
-    for (int r = 0; r < 4; r++)
-      f[r] = sum[r] + (bias && r < valid ? bias_at<T>(bias, col + r) : 0.f);
-    store4<T>(y, (int64_t)token * n + col, f, valid);
-  }
+  if (wave) return;
+  const int64_t col = n0 + 4 * q;
+  const int valid = (int)min((int64_t)4, n - col);
+  if (l15 >= m || valid <= 0) return;
+  v4f sum = part[lane];
+#pragma unroll
+  for (int w = 1; w < kWaves; w++) sum += part[w * 64 + lane];
+  float f[4];
+  for (int r = 0; r < 4; r++)
+    f[r] = sum[r] + (bias && r < valid ? bias_at<T>(bias, col + r) : 0.f);
+  store4<T>(y, (int64_t)l15 * n + col, f, valid);
 }
 
 // ---------------------------------------------------------------------------
 // launching
 // ---------------------------------------------------------------------------
-constexpr int kFewTokens = 64;
-constexpr int64_t kFusedLds = 150 << 10;
+// Few tokens: up to 16. Their kernel quantises them itself where that is
+// less work than a launch more (us, itself and with a launch: weights of 4096
+// x 4096, m = 4: 5.0, 6.2; m = 8: 6.5, 6.4; 8192 x 8192, m = 4: 12.7, 14.2; m
+// = 8: 17.1, 15.1; 8192 x 1024, m = 16: 4.9, 6.5). From codes it is the better
+// one for weights up to 2^25 elements, above which the tokens that each
+// block reads weigh more (m = 16, against small tiles: 4096 x 4096 7.1, 9.3;
+// 8192 x 8192 17.0, 13.5).
+constexpr int64_t kFewTokens = 16;
+constexpr int64_t kFusedElements = 1 << 15;
+constexpr int64_t kFewWeights = 1 << 25;
 
 int64_t few_lds(int64_t m, int64_t nb) {
-  return nb > 1 << 14 ? 1 << 30
-                      : m * (few_codes((int)nb) + few_scales((int)nb));
+  return m * (few_codes((int)nb) + few_scales((int)nb));
 }
 
 bool fuses(int64_t m, int64_t nb) {
-  return m <= kFewTokens && few_lds(m, nb) <= kFusedLds;
+  return m <= kFewTokens && m * nb * kMxBlock <= kFusedElements;
+}
+
+bool few(int64_t m, int64_t n, int64_t nb, bool packed) {
+  return m <= kFewTokens &&
+         ((!packed && fuses(m, nb)) || n * nb * kMxBlock <= kFewWeights);
 }
 
 template <LmType T, int WM, int WN, int FM, int FN>
@@ -595,6 +803,20 @@ void run_tile(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
     throw std::runtime_error("product too large for one launch");
   tile_kernel<T, WM, WN, FM, FN>
       <<<dim3((unsigned)(tm * tn)), WM * WN * 64, 2 * (BM + BN) * 128,
+         stream>>>(xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
+  HIP_CHECK(hipGetLastError());
+}
+
+template <LmType T, int WM, int WN, int WK, int kStages>
+void run_small(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
+               const uint2* ws, const void* bias, void* y, int64_t m,
+               int64_t n, int nb, hipStream_t stream) {
+  constexpr int BM = WM * 32, BN = WN * 32;
+  int64_t tm = (m + BM - 1) / BM, tn = (n + BN - 1) / BN;
+  if (tm * tn >= (int64_t)1 << 28)
+    throw std::runtime_error("product too large for one launch");
+  small_kernel<T, WM, WN, WK, kStages>
+      <<<dim3((unsigned)(tm * tn)), 256, kStages * ((BM + BN) * 128 + 1024),
          stream>>>(xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
   HIP_CHECK(hipGetLastError());
 }
@@ -645,14 +867,29 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   HIP_CHECK(hipGetLastError());
   if (x) xc = codes;
   auto* xs2 = (const uint2*)xst;
-  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
-  const int64_t mid = ((m + 127) / 128) * ((n + 127) / 128);
-  if (big >= 256)
-    run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
-  else if (mid >= 256)
-    run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
+  // The largest tiles of which there are enough to fill the chip. In us, of
+  // m x n x k with tiles of 256 x 256, 128 x 128, 64 x 64, 32 x 64, 32 x 32:
+  // 2000 x 5001 x 2056 30.6, 33.0, 41.7, 49.0, 74.0
+  // 2000 x 4096 x 4096 39.1, 33.4, 47.0, 56.8, 86.9
+  //  800 x 4096 x 4096 34.8, 23.0, 26.0, 28.7, 40.1
+  //  333 x 5001 x 2056 25.7, 15.3, 13.9, 16.5, 20.2
+  //  333 x 4096 x 4096 32.3, 20.4, 15.7, 17.1, 22.3
+  //  100 x 4096 x 4096 30.8, 19.5, 12.4, 11.1, 11.1
+  //  333 x 700 x 700   20.9, 11.6,  9.1,  8.2,  7.6
+  auto tiles = [&](int64_t bm, int64_t bn) {
+    return ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
+  };
+  const int b = (int)nb;
+  if (tiles(256, 256) >= 144)
+    run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
+  else if (tiles(128, 128) >= 192)
+    run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
+  else if (tiles(64, 64) >= 256)
+    run_small<T, 2, 2, 1, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
+  else if (tiles(32, 64) >= 256)
+    run_small<T, 1, 2, 2, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else
-    run_tile<T, 2, 2, 1, 1>(xc, xs2, wc, wst, bias, y, m, n, (int)nb, stream);
+    run_small<T, 1, 1, 4, 6>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
 }
 
 template <LmType T>
@@ -661,49 +898,33 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
                 const void* bias, void* y, int64_t m, int64_t n, int64_t k,
                 void* scratch, hipStream_t stream) {
   const int64_t nb = mx_blocks(k);
-  const bool fused = x && fuses(m, nb);
-  if (m <= kFewTokens && x && !fused) {
-    uint8_t* codes = (uint8_t*)scratch;
-    uint8_t* scales = codes + m * nb * kMxBytes;
-    launch_mx_quantize(T, x, stride, codes, scales, m, k, stream);
-    xc = codes;
-    xs = scales;
+  if (!few(m, n, nb, x == nullptr))
+    return run_tiles<T>(x, stride, xc, xs, wc, ws, bias, y, m, n, k, scratch,
+                        stream);
+  const dim3 grid((unsigned)((n + 15) / 16));
+  const int64_t sums = 512 * sizeof(v4f);
+  if (x && fuses(m, nb)) {
+    few_kernel<T, false><<<grid, 512, std::max(few_lds(m, nb), sums), stream>>>(
+        x, stride, nullptr, nullptr, wc, ws, bias, y, (int)m, n, k, (int)nb);
+  } else {
+    if (x) {
+      uint8_t* codes = (uint8_t*)scratch;
+      uint8_t* scales = codes + m * nb * kMxBytes;
+      launch_mx_quantize(T, x, stride, codes, scales, m, k, stream);
+      xc = codes;
+      xs = scales;
+    }
+    few_kernel<T, true><<<grid, 512, sums, stream>>>(
+        nullptr, 0, xc, xs, wc, ws, bias, y, (int)m, n, k, (int)nb);
   }
-  if (m <= kFewTokens) {
-    auto go = [&](auto mt, auto packed) {
-      constexpr int MT = decltype(mt)::value;
-      constexpr bool P = decltype(packed)::value;
-      int64_t lds = std::max<int64_t>(P ? 0 : few_lds(m, nb),
-                                      (int64_t)8 * MT * 64 * 16);
-      few_kernel<T, MT, P>
-          <<<dim3((unsigned)((n + 15) / 16)), 512, lds,
-             stream>>>(x, stride, xc, xs, wc, ws, bias, y, (int)m, n, k,
-                       (int)nb);
-      HIP_CHECK(hipGetLastError());
-    };
-    auto by_mt = [&](auto packed) {
-      switch ((m + 15) / 16) {
-        case 1:
-          return go(std::integral_constant<int, 1>{}, packed);
-        case 2:
-          return go(std::integral_constant<int, 2>{}, packed);
-        case 3:
-          return go(std::integral_constant<int, 3>{}, packed);
-        default:
-          return go(std::integral_constant<int, 4>{}, packed);
-      }
-    };
-    fused ? by_mt(std::false_type{}) : by_mt(std::true_type{});
-    return;
-  }
-  run_tiles<T>(x, stride, xc, xs, wc, ws, bias, y, m, n, k, scratch, stream);
+  HIP_CHECK(hipGetLastError());
 }
 
 }  // namespace
 
 int64_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, bool packed) {
   const int64_t nb = mx_blocks(k);
-  if (m <= kFewTokens)
+  if (few(m, n, nb, packed))
     return packed || fuses(m, nb) ? 0 : m * nb * (kMxBytes + 1);
   TileSpace space = tile_space(m, n, nb, packed);
   return space.codes + space.xs + space.ws;

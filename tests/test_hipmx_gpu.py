@@ -136,6 +136,12 @@ SHAPES = [
     (49, 128, 16384), (64, 1000, 777), (64, 16, 8192), (65, 64, 32),
     (65, 200, 1056), (127, 129, 255), (128, 128, 256), (129, 300, 300),
     (300, 257, 480), (1000, 96, 2048), (513, 4097, 288), (2049, 2050, 520),
+    # few tokens, quantised in a launch of their own, and long rows
+    (16, 64, 8192), (3, 40, 20001), (16, 8200, 4200),
+    # tiles of 32 x 64, with and without a rest of k
+    (96, 8200, 300), (65, 8192, 512), (33, 8191, 2080),
+    # a step of k more or less than the loads under way
+    (40, 64, 1536), (40, 64, 1537), (40, 64, 1280), (200, 8200, 768),
 ]
 
 
