@@ -6,10 +6,12 @@ this file (in-tree, so it travels to GPU boxes with the repo snapshot).
 Usage: python -m code_interpreter_amd.ops.build [--force]
 """
 
+import importlib.util
 import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
 from pathlib import Path
 
 OPS_DIR = Path(__file__).resolve().parent
@@ -43,6 +45,8 @@ LM_MODULE_SOURCES = [
     HIP_DIR / "mxfp4_gemm.hip",
     HIP_DIR / "scoring.hip",
 ]
+# host code against torch's headers
+TORCH_SOURCES = {HIP_DIR / "hiplm.cpp"}
 MODULES = [
     (OUTPUT, SOURCES),
     (GEMM_OUTPUT, GEMM_MODULE_SOURCES),
@@ -64,29 +68,62 @@ def needs_build() -> bool:
     return any(_needs(out, sources) for out, sources in MODULES)
 
 
-def _compile(output: Path, sources, verbose: bool) -> None:
-    hipcc = os.environ.get("HIPCC", "hipcc")
-    py_include = sysconfig.get_paths()["include"]
-    cmd = [
-        hipcc,
-        f"--offload-arch={ARCH}",
-        "-O3",
-        # packed fp32 arithmetic, which the compiler makes of ordinary float
-        # code, has given wrong results in some of its forms
-        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-        "-std=c++17",
-        "-fPIC",
-        "-shared",
-        "-x", "hip",
-        *[str(s) for s in sources],
-        f"-I{py_include}",
-        f"-I{HIP_DIR}",
-        "-o",
-        str(output),
-    ]
+def _torch_dir() -> Path:
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("_hiplm is built against torch, which is not here")
+    return Path(spec.submodule_search_locations[0])
+
+
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print("+", " ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+
+
+def _compile_torch(source: Path, output: Path, verbose: bool) -> None:
+    include = _torch_dir() / "include"
+    _run([
+        os.environ.get("CXX", "g++"),
+        "-O2", "-std=c++17", "-fPIC", "-c", str(source), "-o", str(output),
+        "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DHIPBLAS_V2",
+        f"-I{include}", f"-I{include}/torch/csrc/api/include",
+        f"-I{os.environ.get('ROCM_PATH', '/opt/rocm')}/include",
+        f"-I{sysconfig.get_paths()['include']}", f"-I{HIP_DIR}",
+    ], verbose)
+
+
+def _compile(output: Path, sources, verbose: bool) -> None:
+    hipcc = os.environ.get("HIPCC", "hipcc")
+    py_include = sysconfig.get_paths()["include"]
+    with tempfile.TemporaryDirectory() as scratch:
+        cmd = [
+            hipcc,
+            f"--offload-arch={ARCH}",
+            "-O3",
+            # packed fp32 arithmetic, which the compiler makes of ordinary
+            # float code, has given wrong results in some of its forms
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+            "-std=c++17",
+            "-fPIC",
+            "-shared",
+            "-x", "hip",
+            *[str(s) for s in sources if s not in TORCH_SOURCES],
+            f"-I{py_include}",
+            f"-I{HIP_DIR}",
+            "-o",
+            str(output),
+        ]
+        with_torch = [s for s in sources if s in TORCH_SOURCES]
+        for source in with_torch:
+            obj = Path(scratch) / (source.stem + ".o")
+            _compile_torch(source, obj, verbose)
+            cmd += ["-x", "none", str(obj)]
+        if with_torch:
+            # loaded after torch, which has them in the process already
+            cmd += [f"-L{_torch_dir() / 'lib'}", "-ltorch_python",
+                    "-ltorch_cpu", "-lc10_hip", "-lc10"]
+        _run(cmd, verbose)
 
 
 def build(force: bool = False, verbose: bool = True) -> Path:

@@ -3,86 +3,347 @@
 // process that uses torch must load the kernels after torch, so that they
 // register with the runtime whose streams and memory it hands them.
 //
-// Surface: stateless raw-pointer entry points only -- the caller (torch)
-// owns memory and streams, and has checked shapes and types.
+// Surface: tensors that the caller (hipmx, hiplm) has checked. Results and
+// scratch come from torch's allocator, on the stream that uses them: of a
+// captured graph, its own. The operators with gradients are nodes of torch's
+// graph. All of that stands here and not in python because the host's part
+// is the longer one where there is little work (us of host time, python and
+// here: quantising 16 x 4096 8.3, 6; a row's log probabilities 18, 10; a
+// loss with its gradient 94, 55, of which torch's own engine takes 40). It
+// is host code: the only file that uses torch's headers.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#include <string>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+#include <torch/csrc/utils/pybind.h>
 
 #include "lm.h"
 
 namespace {
 
-#define NOGIL_BEGIN           \
-  std::string _nogil_err;     \
-  Py_BEGIN_ALLOW_THREADS;     \
-  try {
-#define NOGIL_END                                               \
-  }                                                             \
-  catch (const std::exception& _e) { _nogil_err = _e.what(); }  \
-  Py_END_ALLOW_THREADS;                                         \
-  if (!_nogil_err.empty()) throw std::runtime_error(_nogil_err);
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
-#define WRAP_BEGIN try {
-#define WRAP_END                                   \
-  }                                                \
-  catch (const std::exception& e) {                \
-    PyErr_SetString(PyExc_RuntimeError, e.what()); \
-    return nullptr;                                \
+at::ScalarType scalar_type(int64_t code) {
+  return code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf;
+}
+
+// x as [rows, v] with neighbouring elements in a row: a view where its
+// strides allow one, else a copy
+struct Rows {
+  Tensor x;
+  int64_t rows, v, stride;
+
+  explicit Rows(const Tensor& t) : x(t) {
+    v = t.size(-1);
+    rows = t.numel() / v;
+    if (t.dim() != 2) x = t.reshape({rows, v});
+    if (v > 1 && x.stride(1) != 1) x = x.contiguous();
+    stride = rows > 1 ? x.stride(0) : v;
+  }
+};
+
+// makes x's device the current one, and gives its current stream
+struct Launch {
+  c10::DeviceGuard guard;
+  hipStream_t stream;
+
+  explicit Launch(const Tensor& x)
+      : guard(x.device()),
+        stream(c10::hip::getCurrentHIPStream(x.device().index()).stream()) {}
+};
+
+at::IntArrayRef lead(const Tensor& t) {
+  return t.sizes().slice(0, t.dim() - 1);
+}
+
+std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t last) {
+  std::vector<int64_t> size(lead.begin(), lead.end());
+  size.push_back(last);
+  return size;
+}
+
+Tensor empty(const Tensor& like, at::IntArrayRef size, at::ScalarType type) {
+  return at::empty(size, like.options().dtype(type).requires_grad(false));
+}
+
+template <class T = float>
+T* data(const Tensor& t) {
+  return t.defined() ? (T*)t.data_ptr() : nullptr;
+}
+
+// ---------------------------------------------------------------------------
+// microscaled 4-bit
+// ---------------------------------------------------------------------------
+std::pair<Tensor, Tensor> quantize(const Tensor& x, int64_t code) {
+  Rows r(x);
+  const int64_t nb = mx_blocks(r.v);
+  Tensor codes = empty(x, with_last(lead(x), nb * kMxBytes), at::kByte);
+  Tensor scales = empty(x, with_last(lead(x), nb), at::kByte);
+  if (r.rows) {
+    Launch on(x);
+    launch_mx_quantize((LmType)code, r.x.data_ptr(), r.stride,
+                       data<uint8_t>(codes), data<uint8_t>(scales), r.rows,
+                       r.v, on.stream);
+  }
+  return {codes, scales};
+}
+
+Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t k,
+                  int64_t code) {
+  Tensor out = empty(codes, with_last(lead(scales), k), scalar_type(code));
+  if (out.numel()) {
+    Launch on(codes);
+    launch_mx_dequantize((LmType)code, data<uint8_t>(codes),
+                         data<uint8_t>(scales), out.data_ptr(),
+                         out.numel() / k, k, on.stream);
+  }
+  return out;
+}
+
+// x: a tensor, or the codes of one with its scales in xs
+Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
+              const Tensor& ws, const Tensor& bias, int64_t k, int64_t code) {
+  const bool packed = xs.defined();
+  const int64_t n = ws.size(0);
+  Tensor y = empty(wc, with_last(lead(x), n), scalar_type(code));
+  if (!y.numel()) return y;
+  const int64_t m = y.numel() / n;
+  Launch on(x);
+  const int64_t need = mx_linear_workspace(m, n, k, packed);
+  Tensor work = need ? empty(wc, {need}, at::kByte) : Tensor();
+  const Tensor b = bias.defined() ? bias.contiguous() : bias;
+  if (packed) {
+    launch_mx_linear((LmType)code, nullptr, 0, data<uint8_t>(x),
+                     data<uint8_t>(xs), data<uint8_t>(wc), data<uint8_t>(ws),
+                     data<void>(b), y.data_ptr(), m, n, k, data<void>(work),
+                     on.stream);
+  } else {
+    Rows r(x);
+    launch_mx_linear((LmType)code, r.x.data_ptr(), r.stride, nullptr, nullptr,
+                     data<uint8_t>(wc), data<uint8_t>(ws), data<void>(b),
+                     y.data_ptr(), m, n, k, data<void>(work), on.stream);
+  }
+  return y;
+}
+
+// ---------------------------------------------------------------------------
+// rows of logits
+// ---------------------------------------------------------------------------
+// A gradient of a gradient is not computed. Where the backward itself is
+// recorded, its result answers with an error when one is asked for.
+Tensor once(const Tensor& dx, const variable_list& grads) {
+  if (!at::GradMode::is_enabled()) return dx;
+  bool recorded = false;
+  for (const Tensor& g : grads) recorded |= g.defined() && g.requires_grad();
+  if (!recorded) return dx;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "this operator has no second derivative", 1);
+  return (*error)({dx.detach().requires_grad_()})[0];
+}
+
+struct Scores {
+  Tensor logprobs, entropy, stats;
+};
+
+Scores score(const Tensor& logits, const Tensor& tokens, const Tensor& top_lp,
+             const Tensor& top_ids, int64_t code, double inv_t, int64_t ignore,
+             bool grad) {
+  const LmType t = (LmType)code;
+  Rows r(logits);
+  const int top = (int)top_ids.size(-1);
+  Scores s = {empty(logits, lead(logits), at::kFloat),
+              empty(logits, lead(logits), at::kFloat), Tensor()};
+  if (grad) s.stats = empty(logits, {r.rows, 4}, at::kFloat);
+  if (r.rows) {
+    Launch on(logits);
+    Tensor work =
+        empty(logits, {score_workspace(t, r.rows, r.v, top)}, at::kByte);
+    launch_token_logprobs(t, r.x.data_ptr(), r.stride, r.rows, r.v,
+                          data<int64_t>(tokens), ignore, (float)inv_t, top,
+                          data(s.logprobs), data(s.entropy), data(top_lp),
+                          data<int64_t>(top_ids), data<RowStats>(s.stats),
+                          work.data_ptr(), on.stream);
+  }
+  return s;
+}
+
+class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits,
+                               const Tensor& tokens, const Tensor& top_lp,
+                               const Tensor& top_ids, int64_t code,
+                               double inv_t, int64_t ignore) {
+    Scores s = score(logits, tokens, top_lp, top_ids, code, inv_t, ignore,
+                     true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, tokens, s.stats});
+    ctx->saved_data["code"] = code;
+    ctx->saved_data["inv_t"] = inv_t;
+    return {s.logprobs, s.entropy};
   }
 
-// The arguments of a call in their order; the first that is not what is asked
-// for leaves an exception.
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(7);
+    if (!grads[0].defined() && !grads[1].defined()) return result;
+    Tensor dx;
+    {
+      at::NoGradGuard plain;
+      auto saved = ctx->get_saved_variables();
+      const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
+      Rows r(logits);
+      dx = empty(logits, logits.sizes(), logits.scalar_type());
+      if (r.rows) {
+        const Tensor g_lp = grads[0].defined() ? grads[0].contiguous() : Tensor();
+        const Tensor g_h = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        Launch on(logits);
+        launch_token_logprobs_bwd(
+            (LmType)ctx->saved_data["code"].toInt(), r.x.data_ptr(), r.stride,
+            r.rows, r.v, data<int64_t>(tokens),
+            (float)ctx->saved_data["inv_t"].toDouble(),
+            data<RowStats>(stats), data(g_lp), data(g_h),
+            dx.data_ptr(), on.stream);
+      }
+    }
+    result[0] = once(dx, grads);
+    return result;
+  }
+};
+
+// how: 0 none, 1 sum, 2 mean. kept: the rows' numbers, the teacher's shares,
+// what the loss was divided by and the rows' losses, one behind the other
+struct Loss {
+  Tensor loss, kept;
+};
+
+Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
+             int64_t code, int64_t teacher_code, double inv_t, int64_t how) {
+  const LmType t = (LmType)code;
+  Rows r(logits);
+  const int64_t k = ids.size(-1);
+  Loss l = {empty(logits, how ? at::IntArrayRef() : lead(logits), at::kFloat),
+            empty(logits, {r.rows * (4 + k) + (how ? 1 + r.rows : 0)},
+                  at::kFloat)};
+  if (!r.rows) {
+    l.loss.zero_();
+    return l;
+  }
+  float* stats = data(l.kept);
+  float* q = stats + 4 * r.rows;
+  float* count = how ? q + r.rows * k : nullptr;
+  Launch on(logits);
+  Tensor work = empty(logits, {score_workspace(t, r.rows, r.v, 0)}, at::kByte);
+  launch_distill(t, r.x.data_ptr(), r.stride, r.rows, r.v,
+                 (LmType)teacher_code, teacher.data_ptr(), data<int64_t>(ids),
+                 (int)k, (float)inv_t, how ? count + 1 : data(l.loss), q,
+                 (RowStats*)stats, how ? data(l.loss) : nullptr, count,
+                 how == 2, work.data_ptr(), on.stream);
+  return l;
+}
+
+class Distill : public torch::autograd::Function<Distill> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits,
+                               const Tensor& teacher, const Tensor& ids,
+                               int64_t code, int64_t teacher_code,
+                               double inv_t, int64_t how) {
+    Loss l = distill(logits, teacher, ids, code, teacher_code, inv_t, how);
+    ctx->save_for_backward({logits, ids, l.kept});
+    ctx->saved_data["code"] = code;
+    ctx->saved_data["inv_t"] = inv_t;
+    ctx->saved_data["whole"] = how != 0;
+    return {l.loss};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(7);
+    Tensor dx;
+    {
+      at::NoGradGuard plain;
+      auto saved = ctx->get_saved_variables();
+      const Tensor &logits = saved[0], &ids = saved[1], &kept = saved[2];
+      Rows r(logits);
+      dx = empty(logits, logits.sizes(), logits.scalar_type());
+      if (r.rows) {
+        const Tensor grad = grads[0].contiguous();
+        const int64_t k = ids.size(-1);
+        const bool whole = ctx->saved_data["whole"].toBool();
+        const float* stats = data(kept);
+        const float* q = stats + 4 * r.rows;
+        Launch on(logits);
+        launch_distill_bwd((LmType)ctx->saved_data["code"].toInt(),
+                           r.x.data_ptr(), r.stride, r.rows, r.v,
+                           data<int64_t>(ids), q, (int)k,
+                           (float)ctx->saved_data["inv_t"].toDouble(),
+                           (const RowStats*)stats, data(grad), whole ? 0 : 1,
+                           whole ? q + r.rows * k : nullptr, dx.data_ptr(),
+                           on.stream);
+      }
+    }
+    result[0] = once(dx, grads);
+    return result;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// the module
+// ---------------------------------------------------------------------------
+// The arguments of a call, in their order.
 class Args {
  public:
-  Args(PyObject* const* args, Py_ssize_t n, Py_ssize_t want)
-      : args_(args), good_(n == want) {
-    if (!good_)
-      PyErr_Format(PyExc_TypeError, "%zd arguments wanted, got %zd", want, n);
+  Args(PyObject* const* args, Py_ssize_t n, Py_ssize_t want) : args_(args) {
+    TORCH_CHECK_TYPE(n == want, want, " arguments wanted, got ", n);
   }
-  int64_t integer() {
-    if (!good_) return 0;
+  const Tensor& tensor() {
+    TORCH_CHECK_TYPE(THPVariable_Check(*args_), "a tensor is wanted");
+    return THPVariable_Unpack(*args_++);
+  }
+  Tensor tensor_or_none() {
+    if (*args_ != Py_None) return tensor();
+    args_++;
+    return Tensor();
+  }
+  int64_t integer(int64_t low = INT64_MIN, int64_t high = INT64_MAX) {
     const long long v = PyLong_AsLongLong(*args_++);
-    good_ = !(v == -1 && PyErr_Occurred());
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK(v >= low && v <= high, "an argument is out of its range");
     return v;
   }
-  template <class P = void>
-  P* pointer() {
-    if (!good_) return nullptr;
-    const unsigned long long v = PyLong_AsUnsignedLongLong(*args_++);
-    good_ = !(v == ~0ull && PyErr_Occurred());
-    return (P*)v;
-  }
-  float real() {
-    if (!good_) return 0;
+  int64_t type() { return integer(0, 2); }
+  double real() {
     const double v = PyFloat_AsDouble(*args_++);
-    good_ = !(v == -1 && PyErr_Occurred());
-    return (float)v;
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    return v;
   }
-  LmType type() {
-    const int64_t v = integer();
-    if (good_ && (v < 0 || v > 2)) {
-      PyErr_SetString(PyExc_RuntimeError, "bad dtype code");
-      good_ = false;
-    }
-    return (LmType)v;
-  }
-  int within(int64_t low, int64_t high, const char* what) {
-    const int64_t v = integer();
-    if (good_ && (v < low || v > high)) {
-      PyErr_SetString(PyExc_RuntimeError, what);
-      good_ = false;
-    }
-    return (int)v;
-  }
-  bool good() const { return good_; }
 
  private:
   PyObject* const* args_;
-  bool good_;
 };
+
+PyObject* tuple(std::initializer_list<Tensor> tensors) {
+  THPObjectPtr out(PyTuple_New((Py_ssize_t)tensors.size()));
+  if (!out) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : tensors) {
+    PyObject* o = THPVariable_Wrap(t);
+    if (!o) throw python_error();
+    PyTuple_SET_ITEM(out.get(), i++, o);
+  }
+  return out.release();
+}
+
+bool needs_grad(const Tensor& t) {
+  return at::GradMode::is_enabled() && t.requires_grad();
+}
 
 PyObject* py_is_available(PyObject*, PyObject*) {
   int count = 0;
@@ -92,219 +353,130 @@ PyObject* py_is_available(PyObject*, PyObject*) {
 }
 
 PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 8);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer();
-  auto* codes = a.pointer<uint8_t>();
-  auto* scales = a.pointer<uint8_t>();
-  const int64_t rows = a.integer(), k = a.integer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_mx_quantize(t, x, stride, codes, scales, rows, k, stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
+  HANDLE_TH_ERRORS
+  Args a(args, n, 2);
+  const Tensor& x = a.tensor();
+  const int64_t code = a.type();
+  std::pair<Tensor, Tensor> q;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard plain;
+    q = quantize(x, code);
+  }
+  return tuple({q.first, q.second});
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 7);
-  const LmType t = a.type();
-  auto* codes = a.pointer<uint8_t>();
-  auto* scales = a.pointer<uint8_t>();
-  void* out = a.pointer();
-  const int64_t rows = a.integer(), k = a.integer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_mx_dequantize(t, codes, scales, out, rows, k, stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
-}
-
-PyObject* py_mx_linear_workspace(PyObject*, PyObject* const* args,
-                                 Py_ssize_t n) {
+  HANDLE_TH_ERRORS
   Args a(args, n, 4);
-  const int64_t m = a.integer(), cols = a.integer(), k = a.integer();
-  const bool packed = a.integer() != 0;
-  if (!a.good()) return nullptr;
-  return PyLong_FromLongLong(mx_linear_workspace(m, cols, k, packed));
+  const Tensor &codes = a.tensor(), &scales = a.tensor();
+  const int64_t k = a.integer(1), code = a.type();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = dequantize(codes, scales, k, code);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 14);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer();
-  auto* xc = a.pointer<uint8_t>();
-  auto* xs = a.pointer<uint8_t>();
-  auto* wc = a.pointer<uint8_t>();
-  auto* ws = a.pointer<uint8_t>();
-  const void* bias = a.pointer();
-  void* y = a.pointer();
-  const int64_t m = a.integer(), cols = a.integer(), k = a.integer();
-  void* work = a.pointer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_mx_linear(t, x, stride, xc, xs, wc, ws, bias, y, m, cols, k, work,
-                   stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
-}
-
-PyObject* py_score_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 4);
-  const LmType t = a.type();
-  const int64_t rows = a.integer(), v = a.integer();
-  const int top = a.within(0, kMaxTop, "bad top");
-  if (!a.good()) return nullptr;
-  return PyLong_FromLongLong(score_workspace(t, rows, v, top));
+  HANDLE_TH_ERRORS
+  Args a(args, n, 7);
+  const Tensor& x = a.tensor();
+  const Tensor xs = a.tensor_or_none();
+  const Tensor &wc = a.tensor(), &ws = a.tensor();
+  const Tensor bias = a.tensor_or_none();
+  const int64_t k = a.integer(1), code = a.type();
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard plain;
+    y = linear(x, xs, wc, ws, bias, k, code);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 16);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
-  auto* tokens = a.pointer<int64_t>();
+  HANDLE_TH_ERRORS
+  Args a(args, n, 6);
+  const Tensor &logits = a.tensor(), &tokens = a.tensor();
+  const int64_t code = a.type(), top = a.integer(0, kMaxTop);
+  const double inv_t = a.real();
   const int64_t ignore = a.integer();
-  const float inv_t = a.real();
-  const int top = a.within(0, kMaxTop, "bad top");
-  auto* logprobs = a.pointer<float>();
-  auto* entropy = a.pointer<float>();
-  auto* top_lp = a.pointer<float>();
-  auto* top_ids = a.pointer<int64_t>();
-  auto* stats = a.pointer<RowStats>();
-  void* work = a.pointer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_token_logprobs(t, x, stride, rows, v, tokens, ignore, inv_t, top,
-                        logprobs, entropy, top_lp, top_ids, stats, work,
-                        stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
-}
-
-PyObject* py_token_logprobs_bwd(PyObject*, PyObject* const* args,
-                                Py_ssize_t n) {
-  Args a(args, n, 12);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
-  auto* tokens = a.pointer<int64_t>();
-  const float inv_t = a.real();
-  auto* stats = a.pointer<RowStats>();
-  auto* g_lp = a.pointer<float>();
-  auto* g_h = a.pointer<float>();
-  void* dx = a.pointer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_token_logprobs_bwd(t, x, stride, rows, v, tokens, inv_t, stats, g_lp,
-                            g_h, dx, stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
+  Tensor logprobs, entropy, top_lp, top_ids;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const auto size = with_last(lead(logits), top);
+    top_lp = empty(logits, size, at::kFloat);
+    top_ids = empty(logits, size, at::kLong);
+    if (needs_grad(logits)) {
+      auto out = TokenLogprobs::apply(logits, tokens, top_lp, top_ids, code,
+                                      inv_t, ignore);
+      logprobs = out[0];
+      entropy = out[1];
+    } else {
+      at::NoGradGuard plain;
+      Scores s = score(logits, tokens, top_lp, top_ids, code, inv_t, ignore,
+                       false);
+      logprobs = s.logprobs;
+      entropy = s.entropy;
+    }
+  }
+  return tuple({logprobs, entropy, top_lp, top_ids});
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 18);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
-  const LmType tt = a.type();
-  const void* teacher = a.pointer();
-  auto* ids = a.pointer<int64_t>();
-  const int k = a.within(1, kMaxRecord, "bad record length");
-  const float inv_t = a.real();
-  auto* row_loss = a.pointer<float>();
-  auto* q = a.pointer<float>();
-  auto* stats = a.pointer<RowStats>();
-  auto* total = a.pointer<float>();
-  auto* count = a.pointer<float>();
-  const bool mean = a.integer() != 0;
-  void* work = a.pointer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_distill(t, x, stride, rows, v, tt, teacher, ids, k, inv_t, row_loss,
-                 q, stats, total, count, mean, work, stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
-}
-
-PyObject* py_distill_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 15);
-  const LmType t = a.type();
-  const void* x = a.pointer();
-  const int64_t stride = a.integer(), rows = a.integer(), v = a.integer();
-  auto* ids = a.pointer<int64_t>();
-  auto* q = a.pointer<float>();
-  const int k = a.within(1, kMaxRecord, "bad record length");
-  const float inv_t = a.real();
-  auto* stats = a.pointer<RowStats>();
-  auto* grad = a.pointer<float>();
-  const int64_t grad_stride = a.integer();
-  auto* count = a.pointer<float>();
-  void* dx = a.pointer();
-  auto stream = (hipStream_t)a.pointer();
-  if (!a.good()) return nullptr;
-  WRAP_BEGIN
-  NOGIL_BEGIN
-  launch_distill_bwd(t, x, stride, rows, v, ids, q, k, inv_t, stats, grad,
-                     grad_stride, count, dx, stream);
-  NOGIL_END
-  Py_RETURN_NONE;
-  WRAP_END
+  HANDLE_TH_ERRORS
+  Args a(args, n, 7);
+  const Tensor &logits = a.tensor(), &teacher = a.tensor(), &ids = a.tensor();
+  const int64_t code = a.type(), teacher_code = a.type();
+  const double inv_t = a.real();
+  const int64_t how = a.integer(0, 2);
+  TORCH_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= kMaxRecord,
+              "bad record length");
+  Tensor loss;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (needs_grad(logits)) {
+      loss = Distill::apply(logits, teacher, ids, code, teacher_code, inv_t,
+                            how)[0];
+    } else {
+      at::NoGradGuard plain;
+      loss = distill(logits, teacher, ids, code, teacher_code, inv_t, how).loss;
+    }
+  }
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
 }
 
 #define FAST(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL
 
+// a dtype is 0 float32, 1 bfloat16, 2 float16
 PyMethodDef methods[] = {
     {"is_available", py_is_available, METH_NOARGS, "GPU present?"},
     {"mx_quantize", FAST(py_mx_quantize),
-     "mx_quantize(dtype, x, stride, codes, scales, rows, k, stream)"},
+     "mx_quantize(x, dtype) -> (codes, scales)"},
     {"mx_dequantize", FAST(py_mx_dequantize),
-     "mx_dequantize(dtype, codes, scales, out, rows, k, stream)"},
-    {"mx_linear_workspace", FAST(py_mx_linear_workspace),
-     "mx_linear_workspace(m, n, k, packed) -> bytes"},
+     "mx_dequantize(codes, scales, k, dtype) -> values"},
     {"mx_linear", FAST(py_mx_linear),
-     "mx_linear(dtype, x, stride, xcodes, xscales, wcodes, wscales, bias, y, "
-     "m, n, k, workspace, stream)"},
-    {"score_workspace", FAST(py_score_workspace),
-     "score_workspace(dtype, rows, v, top) -> bytes"},
+     "mx_linear(x or its codes, its scales or None, weight codes, weight "
+     "scales, bias or None, k, dtype) -> y"},
     {"token_logprobs", FAST(py_token_logprobs),
-     "token_logprobs(dtype, x, stride, rows, v, tokens, ignore, inv_t, top, "
-     "logprobs, entropy, top_lp, top_ids, stats, workspace, stream)"},
-    {"token_logprobs_bwd", FAST(py_token_logprobs_bwd),
-     "token_logprobs_bwd(dtype, x, stride, rows, v, tokens, inv_t, stats, "
-     "g_logprobs, g_entropy, dx, stream)"},
+     "token_logprobs(logits, tokens, dtype, top, inv_t, ignore) -> (logprobs, "
+     "entropy, top_logprobs, top_tokens)"},
     {"distill", FAST(py_distill),
-     "distill(dtype, x, stride, rows, v, teacher_dtype, teacher, ids, k, "
-     "inv_t, row_loss, q, stats, total, count, mean, workspace, stream)"},
-    {"distill_bwd", FAST(py_distill_bwd),
-     "distill_bwd(dtype, x, stride, rows, v, ids, q, k, inv_t, stats, grad, "
-     "grad_stride, count, dx, stream)"},
+     "distill(logits, teacher, ids, dtype, teacher dtype, inv_t, reduction) "
+     "-> loss; reduction: 0 none, 1 sum, 2 mean"},
     {nullptr, nullptr, 0, nullptr},
 };
 
 struct PyModuleDef module_def = {
     PyModuleDef_HEAD_INIT, "_hiplm",
-    "gfx950 language-model kernels (raw pointers, caller's stream)",
-    -1, methods,
+    "gfx950 language-model kernels for torch tensors", -1, methods,
 };
 
 }  // namespace

@@ -33,7 +33,7 @@ STATS = {"token_logprobs": 0, "topk_distill_loss": 0}
 TokenLogprobs = namedtuple(
     "TokenLogprobs", ["logprobs", "entropy", "top_logprobs", "top_tokens"])
 
-_functions = {}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def _check_logits(logits) -> int:
@@ -96,16 +96,9 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
     if not logits.is_cuda:
         return _cpu_token_logprobs(torch, logits, tokens, top, t,
                                    int(ignore_index))
-    f32 = torch.float32
-    top_lp = logits.new_empty((*lead, top), dtype=f32)
-    top_ids = tokens.new_empty((*lead, top))
-    args = (logits, tokens, top_lp, top_ids, code, 1.0 / t, int(ignore_index))
-    if logits.requires_grad and torch.is_grad_enabled():
-        logprobs, entropy = _function("logprobs", torch).apply(*args)
-    else:
-        logprobs, entropy, _ = _logprobs(torch, *args, False)
     STATS["token_logprobs"] += 1
-    return TokenLogprobs(logprobs, entropy, top_lp, top_ids)
+    return TokenLogprobs(*hiptorch.ensure_hiplm().token_logprobs(
+        logits, tokens, code, top, 1.0 / t, int(ignore_index)))
 
 
 def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
@@ -149,171 +142,15 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
         teacher_logits = teacher_logits.detach()
     ids = _check_ids(torch, "teacher_tokens", teacher_tokens, t_shape,
                      logits.device)
-    if reduction not in ("mean", "sum", "none"):
+    how = _REDUCTIONS.get(reduction)
+    if how is None:
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got "
                          f"{reduction!r}")
     if not logits.is_cuda:
         return _cpu_distill(torch, logits, teacher_logits, ids, t, reduction)
-    args = (logits, teacher_logits.contiguous(), ids, code, t_code, 1.0 / t,
-            reduction)
-    if logits.requires_grad and torch.is_grad_enabled():
-        loss = _function("distill", torch).apply(*args)
-    else:
-        loss, _ = _distill(torch, *args)
     STATS["topk_distill_loss"] += 1
-    return loss
-
-
-# ---------------------------------------------------------------------------
-# GPU tensors
-# ---------------------------------------------------------------------------
-# Scratch comes from torch's allocator, on the stream that uses it: of a
-# captured graph, its own.
-_STATS_BYTES = 16  # what a row leaves for its backward
-
-
-def _logprobs(torch, logits, tokens, top_lp, top_ids, code, inv_t, ignore,
-              grad):
-    """(log probabilities, entropies, what the backward needs or None)."""
-    ext = hiptorch.ensure_hiplm()
-    x, stride = hiptorch.rows_view(logits)
-    rows, v = x.shape
-    top = top_ids.shape[-1]
-    lead = logits.shape[:-1]
-    logprobs = top_lp.new_empty(lead)
-    entropy = top_lp.new_empty(lead)
-    stats = top_lp.new_empty((rows, _STATS_BYTES // 4)) if grad else None
-    if rows:
-        work = x.new_empty((ext.score_workspace(code, rows, v, top),),
-                           dtype=torch.uint8)
-        with hiptorch.on_device(x) as stream:
-            ext.token_logprobs(
-                code, x.data_ptr(), stride, rows, v, tokens.data_ptr(),
-                ignore, inv_t, top, logprobs.data_ptr(), entropy.data_ptr(),
-                top_lp.data_ptr(), top_ids.data_ptr(),
-                stats.data_ptr() if grad else 0, work.data_ptr(), stream)
-    return logprobs, entropy, stats
-
-
-def _distill(torch, logits, teacher, ids, code, t_code, inv_t, reduction):
-    """(the loss, what the backward needs: the rows' numbers, the teacher's
-    shares, what the loss was divided by and the rows' losses, one behind the
-    other; None without rows)."""
-    ext = hiptorch.ensure_hiplm()
-    x, stride = hiptorch.rows_view(logits)
-    rows, v = x.shape
-    k = teacher.shape[-1]
-    f32 = torch.float32
-    whole = reduction != "none"
-    loss = x.new_empty(() if whole else logits.shape[:-1], dtype=f32)
-    if not rows:
-        return loss.zero_(), None
-    kept = loss.new_empty((rows * (_STATS_BYTES // 4 + k)
-                           + (1 + rows if whole else 0),))
-    stats = kept.data_ptr()
-    q = stats + rows * _STATS_BYTES
-    count = q + rows * k * 4
-    work = x.new_empty((ext.score_workspace(code, rows, v, 0),),
-                       dtype=torch.uint8)
-    with hiptorch.on_device(x) as stream:
-        ext.distill(
-            code, x.data_ptr(), stride, rows, v, t_code, teacher.data_ptr(),
-            ids.data_ptr(), k, inv_t,
-            count + 4 if whole else loss.data_ptr(), q, stats,
-            loss.data_ptr() if whole else 0, count if whole else 0,
-            reduction == "mean", work.data_ptr(), stream)
-    return loss, kept
-
-
-def _function(name, torch):
-    """The autograd function of that name; made at its first use, since
-    importing this module must not import torch."""
-    if not _functions:
-        _make_functions(torch)
-    return _functions[name]
-
-
-def _make_functions(torch):
-    from torch.autograd.function import once_differentiable
-
-    # what makes a second derivative an error costs time on every call, and
-    # is needed only where a graph of the backward is asked for
-    def once(backward):
-        slow = once_differentiable(backward)
-
-        def run(ctx, *grads):
-            if torch.is_grad_enabled():
-                return slow(ctx, *grads)
-            return backward(ctx, *grads)
-
-        return staticmethod(run)
-
-    class TokenLogprobsFunction(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, logits, tokens, top_lp, top_ids, code, inv_t,
-                    ignore):
-            logprobs, entropy, stats = _logprobs(
-                torch, logits, tokens, top_lp, top_ids, code, inv_t, ignore,
-                True)
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(logits, tokens, stats)
-            ctx.code, ctx.inv_t = code, inv_t
-            return logprobs, entropy
-
-        @once
-        def backward(ctx, g_lp, g_h):
-            none = (None,) * 6
-            if g_lp is None and g_h is None:
-                return (None, *none)
-            logits, tokens, stats = ctx.saved_tensors
-            x, stride = hiptorch.rows_view(logits)
-            rows, v = x.shape
-            dx = x.new_empty(logits.shape)
-            if rows:
-                g_lp = None if g_lp is None else g_lp.contiguous()
-                g_h = None if g_h is None else g_h.contiguous()
-                with hiptorch.on_device(x) as stream:
-                    _hiplm().token_logprobs_bwd(
-                        ctx.code, x.data_ptr(), stride, rows, v,
-                        tokens.data_ptr(), ctx.inv_t, stats.data_ptr(),
-                        0 if g_lp is None else g_lp.data_ptr(),
-                        0 if g_h is None else g_h.data_ptr(),
-                        dx.data_ptr(), stream)
-            return (dx, *none)
-
-    class DistillFunction(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, logits, teacher, ids, code, t_code, inv_t,
-                    reduction):
-            loss, kept = _distill(torch, logits, teacher, ids, code, t_code,
-                                  inv_t, reduction)
-            ctx.save_for_backward(logits, ids, kept)
-            ctx.code, ctx.inv_t, ctx.whole = code, inv_t, reduction != "none"
-            return loss
-
-        @once
-        def backward(ctx, grad):
-            logits, ids, kept = ctx.saved_tensors
-            dx = logits.new_empty(logits.shape)
-            if kept is not None:
-                x, stride = hiptorch.rows_view(logits)
-                rows, v = x.shape
-                k = ids.shape[-1]
-                grad = grad.contiguous()
-                stats = kept.data_ptr()
-                q = stats + rows * _STATS_BYTES
-                with hiptorch.on_device(x) as stream:
-                    _hiplm().distill_bwd(
-                        ctx.code, x.data_ptr(), stride, rows, v,
-                        ids.data_ptr(), q, k, ctx.inv_t, stats,
-                        grad.data_ptr(), 0 if ctx.whole else 1,
-                        q + rows * k * 4 if ctx.whole else 0, dx.data_ptr(),
-                        stream)
-            return (dx,) + (None,) * 6
-
-    _hiplm = hiptorch.ensure_hiplm
-    _functions["logprobs"] = TokenLogprobsFunction
-    _functions["distill"] = DistillFunction
+    return hiptorch.ensure_hiplm().distill(
+        logits, teacher_logits.contiguous(), ids, code, t_code, 1.0 / t, how)
 
 
 # ---------------------------------------------------------------------------

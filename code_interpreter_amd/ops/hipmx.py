@@ -113,20 +113,9 @@ def quantize(x) -> MXFP4Tensor:
     shape = x.shape
     if not shape or not shape[-1]:
         raise ValueError(f"x needs a last axis, got {list(shape)}")
-    lead, k = shape[:-1], shape[-1]
-    nb = _blocks(k)
     if not x.is_cuda:
-        return MXFP4Tensor(*_cpu_quantize(torch, x.detach()), k)
-    ext = hiptorch.ensure_hiplm()
-    x2, stride = hiptorch.rows_view(x)
-    rows = x2.shape[0]
-    u8 = torch.uint8
-    codes = x.new_empty((*lead, nb * 16), dtype=u8)
-    scales = x.new_empty((*lead, nb), dtype=u8)
-    if rows:
-        with hiptorch.on_device(x) as stream:
-            ext.mx_quantize(code, x2.data_ptr(), stride, codes.data_ptr(),
-                            scales.data_ptr(), rows, k, stream)
+        return MXFP4Tensor(*_cpu_quantize(torch, x.detach()), shape[-1])
+    codes, scales = hiptorch.ensure_hiplm().mx_quantize(x, code)
     STATS["quantize"] += 1
     return MXFP4Tensor.__new__(MXFP4Tensor)._set(codes, scales, shape)
 
@@ -137,16 +126,9 @@ def _dequantize(q: MXFP4Tensor, dtype=None):
     code = hiptorch.check_dtype("dtype", dtype)
     if not q.codes.is_cuda:
         return _cpu_dequantize(torch, q).to(dtype)
-    ext = hiptorch.ensure_hiplm()
-    k = q.shape[-1]
-    out = q.codes.new_empty(q.shape, dtype=dtype)
-    rows = out.numel() // k
-    if rows:
-        with hiptorch.on_device(out) as stream:
-            ext.mx_dequantize(code, q.codes.data_ptr(), q.scales.data_ptr(),
-                              out.data_ptr(), rows, k, stream)
     STATS["dequantize"] += 1
-    return out
+    return hiptorch.ensure_hiplm().mx_dequantize(q.codes, q.scales,
+                                                 q.shape[-1], code)
 
 
 def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
@@ -199,43 +181,16 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
         if torch.is_grad_enabled():
             raise RuntimeError("hipmx.linear has no backward: call it under "
                                "torch.no_grad(), or detach its inputs")
-    lead = shape[:-1]
     if not wcodes.is_cuda:
         q = input if packed else quantize(input)
         y = _cpu_dequantize(torch, q) @ _cpu_dequantize(torch, weight).T
         if bias is not None:
             y = y + bias.detach().float()
         return y.to(dtype)
-    ext = hiptorch.ensure_hiplm()
-    y = wcodes.new_empty((*lead, n), dtype=dtype)
-    m = 1
-    for d in lead:
-        m *= d
-    if m == 0 or n == 0:
-        return y
-    if packed:
-        x_ptr = stride = 0
-        xc, xs = data.data_ptr(), input.scales.data_ptr()
-    else:
-        x2, stride = hiptorch.rows_view(input)
-        x_ptr, xc, xs = x2.data_ptr(), 0, 0
-    b_ptr = 0
-    if bias is not None:
-        bias = bias.contiguous()
-        b_ptr = bias.data_ptr()
-    need = ext.mx_linear_workspace(m, n, k, packed)
-    w_ptr = 0
-    if need:
-        # from torch's allocator, on the stream that uses it: of a captured
-        # graph, its own
-        work = wcodes.new_empty((need,))
-        w_ptr = work.data_ptr()
-    with hiptorch.on_device(y) as stream:
-        ext.mx_linear(code, x_ptr, stride, xc, xs, wcodes.data_ptr(),
-                      weight.scales.data_ptr(), b_ptr, y.data_ptr(), m, n, k,
-                      w_ptr, stream)
     STATS["linear"] += 1
-    return y
+    return hiptorch.ensure_hiplm().mx_linear(
+        data, input.scales if packed else None, wcodes, weight.scales, bias,
+        k, code)
 
 
 # ---------------------------------------------------------------------------

@@ -74,33 +74,25 @@ def ensure_hiplm():
 # token's worth of work the host's part is the longer one
 # ---------------------------------------------------------------------------
 _lm_codes = {}  # the kernels' code of each type that they take
-_raw = {}       # torch's own handles of the current device and stream
+_tensor = []    # torch.Tensor, and the layout that they take
 
 
 def lm_torch():
     """torch, with the tables above filled."""
     import torch
 
-    if not _raw:
+    if not _tensor:
         _lm_codes.update({torch.float32: 0, torch.bfloat16: 1,
                           torch.float16: 2})
-        _raw["tensor"] = torch.Tensor
-        _raw["strided"] = torch.strided
-        _raw["set"] = torch.cuda.set_device
-        # the public calls make an object each time: these are their cores
-        _raw["device"] = getattr(torch._C, "_cuda_getDevice",
-                                 torch.cuda.current_device)
-        _raw["stream"] = getattr(
-            torch._C, "_cuda_getCurrentRawStream",
-            lambda i: torch.cuda.current_stream(i).cuda_stream)
+        _tensor.extend((torch.Tensor, torch.strided))
     return torch
 
 
 def check_tensor(name, x):
     """A TypeError that names x where it is no strided tensor."""
-    if not isinstance(x, _raw["tensor"]):
+    if not isinstance(x, _tensor[0]):
         raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
-    if x.layout is not _raw["strided"]:
+    if x.layout is not _tensor[1]:
         raise TypeError(f"{name} must be a strided tensor, got {x.layout}")
 
 
@@ -110,40 +102,6 @@ def check_dtype(name, dtype) -> int:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got "
                         f"{dtype}")
     return code
-
-
-def rows_view(x):
-    """x as [rows, k] with neighbouring elements in a row, and the distance
-    of its rows: a view where its strides allow one, else a copy."""
-    if x.dim() != 2:
-        k = x.shape[-1]
-        x = x.reshape(x.numel() // k, k)
-    stride, inner = x.stride()
-    rows, k = x.shape
-    if inner != 1 and k > 1:
-        x = x.contiguous()
-        stride = k
-    return x, (stride if rows > 1 else k)
-
-
-class on_device:
-    """Makes x's device the current one while kernels are launched on it, and
-    gives its current stream."""
-
-    __slots__ = ("_index", "_before")
-
-    def __init__(self, x):
-        self._index = x.get_device()
-
-    def __enter__(self):
-        before = self._before = _raw["device"]()
-        if before != self._index:
-            _raw["set"](self._index)
-        return _raw["stream"](self._index)
-
-    def __exit__(self, *_):
-        if self._before != self._index:
-            _raw["set"](self._before)
 
 
 # route only when the kernel launch is worth more than its overhead;

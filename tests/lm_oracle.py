@@ -153,3 +153,28 @@ def distill(x, teacher, ids, t, reduction):
         return loss, grad, size
     by = max(count, 1) if reduction == "mean" else 1
     return loss.sum() / by, grad / by, size / by
+
+
+# ---------------------------------------------------------------------------
+# writes behind a tensor's end
+# ---------------------------------------------------------------------------
+# The caching allocator hands out blocks of whole 512 bytes, the best fitting
+# free one first. Free blocks of a result's size are filled with a pattern
+# beforehand; what stands between the result's end and its block's has to be
+# there still.
+def fill_free_blocks(torch, *sizes):
+    for size in sizes:
+        whole = -(-size // 512) * 512
+        blocks = [torch.full((whole,), 0xA5, dtype=torch.uint8, device="cuda")
+                  for _ in range(12)]
+        del blocks
+
+
+def behind(torch, t):
+    """The bytes between a tensor's end and its block's."""
+    size = t.numel() * t.element_size()
+    whole = -(-size // 512) * 512
+    storage = torch._C._construct_storage_from_data_pointer(
+        t.data_ptr(), t.device, whole)
+    every = torch.empty(0, dtype=torch.uint8, device=t.device).set_(storage)
+    return every[size:].cpu()

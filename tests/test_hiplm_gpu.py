@@ -428,45 +428,29 @@ def test_forward_and_backward_in_a_graph(lm, rows):
 
 
 @pytest.mark.parametrize("rows,v,top", [(1, 9, 3), (3, 2049, 128),
-                                        (5, 50001, 20), (1030, 333, 0)])
-def test_kernels_write_their_results_alone(lm, rows, v, top):
-    """The entry points that the wrappers call, into buffers with edges."""
+                                        (5, 50001, 20), (1030, 333, 1)])
+def test_results_end_where_they_end(lm, rows, v, top):
     torch, hiplm = lm
-    import hiptorch
+    import lm_oracle as oracle
 
-    ext = hiptorch.ensure_hiplm()
-    stream = torch.cuda.current_stream().cuda_stream
-    edge, kept = 4096, []
-
-    def buffer(size):
-        b = torch.full((2 * edge + size,), 0xA5, dtype=torch.uint8,
-                       device="cuda")
-        kept.append((b, size))
-        return b.data_ptr() + edge
-
-    x = torch.randn(rows, v, device="cuda").bfloat16()
+    x = torch.randn(rows, v, device="cuda").bfloat16().requires_grad_(True)
     tokens = torch.randint(v, (rows,), device="cuda")
-    stats, g = buffer(16 * rows), torch.ones(rows, device="cuda")
-    ext.token_logprobs(1, x.data_ptr(), v, rows, v, tokens.data_ptr(), -100,
-                       1.0, top, buffer(4 * rows), buffer(4 * rows),
-                       buffer(4 * rows * top), buffer(8 * rows * top), stats,
-                       buffer(ext.score_workspace(1, rows, v, top)), stream)
-    dx = buffer(2 * rows * v)
-    ext.token_logprobs_bwd(1, x.data_ptr(), v, rows, v, tokens.data_ptr(), 1.0,
-                           stats, g.data_ptr(), 0, dx, stream)
-    k = 7
-    teacher = torch.randn(rows, k, device="cuda")
-    ids = torch.randint(v, (rows, k), device="cuda")
-    q, total = buffer(4 * rows * k), buffer(8)
-    ext.distill(1, x.data_ptr(), v, rows, v, 0, teacher.data_ptr(),
-                ids.data_ptr(), k, 1.0, buffer(4 * rows), q, stats, total,
-                total + 4, True, buffer(ext.score_workspace(1, rows, v, 0)), stream)
-    ext.distill_bwd(1, x.data_ptr(), v, rows, v, ids.data_ptr(), q, k, 1.0,
-                    stats, g.data_ptr(), 0, total + 4, buffer(2 * rows * v),
-                    stream)
-    torch.cuda.synchronize()
-    for b, size in kept:
-        assert (b[:edge] == 0xA5).all() and (b[edge + size:] == 0xA5).all()
+    g, one = torch.ones(rows, device="cuda"), torch.ones((), device="cuda")
+
+    def ends(call):  # one call's results, looked at before the next
+        oracle.fill_free_blocks(torch, 4 * rows, 4 * rows * top,
+                                8 * rows * top, 2 * rows * v, 4)
+        out = call()
+        torch.cuda.synchronize()
+        for t in out:
+            assert (oracle.behind(torch, t) == 0xA5).all()
+        return out
+
+    r = ends(lambda: hiplm.token_logprobs(x, tokens, top=top))
+    ends(lambda: torch.autograd.grad([r.logprobs, r.entropy], [x], [g, g]))
+    (loss,) = ends(lambda: [hiplm.topk_distill_loss(x, r.top_logprobs,
+                                                    r.top_tokens)])
+    ends(lambda: torch.autograd.grad(loss, [x], one))
 
 
 def test_on_another_stream(lm):

@@ -227,28 +227,28 @@ def test_linear_inputs_of_other_strides(mx):
 
 @pytest.mark.parametrize("m,n,k", [(1, 5, 40), (3, 17, 64), (40, 37, 100),
                                    (70, 37, 64), (129, 131, 288),
-                                   (4097, 4100, 32)])
-def test_linear_writes_its_results_alone(mx, m, n, k):
+                                   (2049, 2055, 32), (4097, 4101, 32)])
+def test_results_end_where_they_end(mx, m, n, k):
     torch, hipmx = mx
-    import hiptorch
+    import lm_oracle as oracle
 
-    # the entry point that the wrapper calls, into the middle of a buffer
-    ext = hiptorch.ensure_hiplm()
     x, w, _ = operands(torch, hipmx, m, n, k, "bfloat16")
-    edge = 4096
-    out = torch.full((edge + m * n + edge,), 7.0, dtype=torch.bfloat16,
-                     device="cuda")
-    need = ext.mx_linear_workspace(m, n, k, False)
-    work = torch.full((edge + need + edge,), 9, dtype=torch.uint8,
-                      device="cuda")
-    ext.mx_linear(1, x.data_ptr(), k, 0, 0, w.codes.data_ptr(),
-                  w.scales.data_ptr(), 0, out.data_ptr() + 2 * edge, m, n, k,
-                  work.data_ptr() + edge, torch.cuda.current_stream().cuda_stream)
-    torch.cuda.synchronize()
-    y = out[edge:edge + m * n].view(m, n)
-    assert torch.equal(y, hipmx.linear(x, w))
-    assert (out[:edge] == 7).all() and (out[edge + m * n:] == 7).all()
-    assert (work[:edge] == 9).all() and (work[edge + need:] == 9).all()
+    nb = -(-k // 32)
+    bias = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+
+    def ends(call):  # one call's results, looked at before the next
+        oracle.fill_free_blocks(torch, 2 * m * n, 2 * m * k, m * nb * 16,
+                                m * nb)
+        out = call()
+        torch.cuda.synchronize()
+        for t in out:
+            assert (oracle.behind(torch, t) == 0xA5).all()
+
+    q = hipmx.quantize(x)
+    ends(lambda: [hipmx.linear(x, w, bias)])
+    ends(lambda: [hipmx.linear(q, w)])
+    ends(lambda: (lambda p: [p.codes, p.scales])(hipmx.quantize(x)))
+    ends(lambda: [q.dequantize()])
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
