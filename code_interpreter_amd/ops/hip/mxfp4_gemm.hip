@@ -84,7 +84,7 @@ __device__ __forceinline__ float bias_at(const void* bias, int64_t i) {
 // a row's own order a wave would touch a cache line for every row.
 constexpr int kPrepareThreads = 256;
 constexpr int kPrepareRows = 32;  // of a block that quantises one step
-constexpr int kLayRows = kPrepareThreads, kLaySteps = 8;  // of one that does not
+constexpr int kLayRows = kPrepareThreads, kLaySteps = 4;  // of one that does not
 
 __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
                                                uint2* to, int64_t rows,
@@ -94,12 +94,18 @@ __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
   const int t0 = blk % parts * kLaySteps;
   if (row >= rows) return;
   const uint8_t* p = from + row * nb;
+  struct __attribute__((packed)) raw8 {
+    uint32_t x, y;
+    __device__ operator uint2() const { return {x, y}; }
+  };
   uint2 v[kLaySteps];
 #pragma unroll
   for (int i = 0; i < kLaySteps; i++)
     if (t0 + i < steps)
-      v[i] = {load_scales(p, (t0 + i) * 8, nb),
-              load_scales(p, (t0 + i) * 8 + 4, nb)};
+      v[i] = (t0 + i) * 8 + 8 <= nb
+                 ? *(const raw8*)(p + (t0 + i) * 8)
+                 : uint2{load_scales(p, (t0 + i) * 8, nb),
+                         load_scales(p, (t0 + i) * 8 + 4, nb)};
 #pragma unroll
   for (int i = 0; i < kLaySteps; i++)
     if (t0 + i < steps) to[(t0 + i) * rows + row] = v[i];
@@ -442,26 +448,27 @@ __global__ __launch_bounds__(WM* WN * 64, 1) void tile_kernel(
 // ---------------------------------------------------------------------------
 // The time is the memory's answer, not the products': so a block keeps the
 // loads of kStages - 1 steps under way, in a ring of buffers, and small tiles
-// make many blocks. 4 waves make a tile of 32 WM tokens x 32 WN outputs; of
-// the 4 instructions of a step WK waves take a share each, and their sums are
-// added in a fixed order at the end. Rows stand in shared memory as for the
+// make many blocks. WM x WN x WK waves make a tile of 32 WM tokens x 32 WN
+// outputs; of the 4 instructions of a step WK waves take a share each, and
+// their sums are added in a fixed order at the end. Rows stand in shared memory as for the
 // large tiles; the scales of a step come the same way, 4 bytes a lane.
 template <LmType T, int WM, int WN, int WK, int kStages>
-__global__ __launch_bounds__(256) void small_kernel(
+__global__ __launch_bounds__(WM* WN* WK * 64) void small_kernel(
     const uint8_t* __restrict__ xc, const uint2* __restrict__ xs,
     const uint8_t* __restrict__ wc, const uint2* __restrict__ ws,
     const void* __restrict__ bias, void* __restrict__ y, int64_t m, int64_t n,
     int nb, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__  // buffer descriptors are no type on the host
-  static_assert(WM * WN * WK == 4, "");
+  constexpr int kWaves = WM * WN * WK;
   constexpr int BM = WM * 32, BN = WN * 32;
   constexpr int kRow = 128;
   constexpr int kScales = (BM + BN) * kRow;  // behind the rows
-  constexpr int kBuf = kScales + 1024;
-  constexpr int kLoads = (BM + BN) / 32;  // of a wave, 8 rows each
-  constexpr int kPerStep = kLoads + 1;    // with one of scales
+  constexpr int kBuf = kScales + kWaves * 256;
+  constexpr int kLoads = (BM + BN) / 8 / kWaves;  // of a wave, 8 rows each
+  constexpr int kPerStep = kLoads + 1;            // with one of scales
   constexpr int kWait = (kStages - 2) * kPerStep;
-  static_assert(kWait < 64, "");
+  static_assert(kWaves % 2 == 0 && BM % (8 * kWaves) == 0 &&
+                    BN % (8 * kWaves) == 0 && kWait < 64, "");
   constexpr int kOut = BN + 4;  // floats between tokens in the epilogue
   static_assert(WK * BM * kOut * 4 <= kStages * kBuf, "");
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -499,15 +506,16 @@ __global__ __launch_bounds__(256) void small_kernel(
   uint32_t off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; i++) {
-    const int64_t r = (i * 4 + wave) * 8 + (lane >> 3);
-    const int64_t at = i * 32 < BN ? min(r, n - 1 - n0)
-                                   : min(r - BN, m - 1 - m0);
+    const int64_t r = (i * kWaves + wave) * 8 + (lane >> 3);
+    const int64_t at = i * kWaves * 8 < BN ? min(r, n - 1 - n0)
+                                           : min(r - BN, m - 1 - m0);
     off[i] = (uint32_t)(at * row_bytes) + unit * 16;
   }
   // scales: words 2 r, 2 r + 1 of row r. A wave behind the last word loads
   // the first ones once more, to a place that is not read. Rows behind the
   // operand's last one get some other row's, or 0: they are not stored.
   constexpr int kScaleWaves = (BM + BN) * 2 / 64;
+  static_assert(kScaleWaves <= kWaves, "");
   const int word0 = (wave % kScaleWaves) * 64;
   const bool of_x = word0 >= BN * 2;
   const auto sr = of_x ? buffer(xs, m * steps * 8) : buffer(ws, n * steps * 8);
@@ -520,8 +528,8 @@ __global__ __launch_bounds__(256) void small_kernel(
     const int less = t == full ? back : 0;
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
-      lds_void* at = (lds_void*)(to + (i * 4 + wave) * 1024);
-      if (i * 32 < BN)
+      lds_void* at = (lds_void*)(to + (i * kWaves + wave) * 1024);
+      if (i * kWaves * 8 < BN)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             wr, at, 16, (int)off[i] - less, t * kRow, 0, 0);
       else
@@ -601,8 +609,8 @@ __global__ __launch_bounds__(256) void small_kernel(
                                 acc[4 * g + 3]};
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < BM * BN / 1024; i++) {
-    const int e = (i * 256 + threadIdx.x) * 4;
+  for (int i = 0; i < BM * BN / (kWaves * 256); i++) {
+    const int e = (i * kWaves * 64 + threadIdx.x) * 4;
     const int64_t row = m0 + e / BN, col = n0 + e % BN;
     const int valid = (int)min((int64_t)4, n - col);
     if (row >= m || valid <= 0) continue;
@@ -816,8 +824,9 @@ void run_small(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
   if (tm * tn >= (int64_t)1 << 28)
     throw std::runtime_error("product too large for one launch");
   small_kernel<T, WM, WN, WK, kStages>
-      <<<dim3((unsigned)(tm * tn)), 256, kStages * ((BM + BN) * 128 + 1024),
-         stream>>>(xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
+      <<<dim3((unsigned)(tm * tn)), WM * WN * WK * 64,
+         kStages * ((BM + BN) * 128 + WM * WN * WK * 256), stream>>>(
+          xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
   HIP_CHECK(hipGetLastError());
 }
 
@@ -868,14 +877,16 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   if (x) xc = codes;
   auto* xs2 = (const uint2*)xst;
   // The largest tiles of which there are enough to fill the chip. In us, of
-  // m x n x k with tiles of 256 x 256, 128 x 128, 64 x 64, 32 x 64, 32 x 32:
-  // 2000 x 5001 x 2056 30.6, 33.0, 41.7, 49.0, 74.0
-  // 2000 x 4096 x 4096 39.1, 33.4, 47.0, 56.8, 86.9
-  //  800 x 4096 x 4096 34.8, 23.0, 26.0, 28.7, 40.1
-  //  333 x 5001 x 2056 25.7, 15.3, 13.9, 16.5, 20.2
-  //  333 x 4096 x 4096 32.3, 20.4, 15.7, 17.1, 22.3
-  //  100 x 4096 x 4096 30.8, 19.5, 12.4, 11.1, 11.1
-  //  333 x 700 x 700   20.9, 11.6,  9.1,  8.2,  7.6
+  // m x n x k with tiles of 256 x 256, 128 x 128 (2 buffers), 64 x 128, 64 x
+  // 64 (3), 32 x 64 (4), 32 x 32 (6):
+  // 2000 x 5001 x 2056 30.6, 33.0,    -,    -, 49.0, 74.0
+  // 2000 x 4096 x 4096 39.1, 33.4,    -,    -, 56.8, 86.9
+  //  800 x 4096 x 4096 34.8, 22.5, 21.7, 25.5, 28.7, 40.1
+  //  500 x 4096 x 4096    -, 21.2, 16.4, 16.7, 21.5,    -
+  //  333 x 5001 x 2056 25.7, 15.2, 12.0, 13.4, 16.4, 20.2
+  //  200 x 4096 x 4096    -, 19.5, 14.2, 13.0, 12.5,    -
+  //  100 x 4096 x 4096 30.8, 19.3, 13.5, 12.2, 10.8, 11.1
+  //  333 x 700 x 700   20.9, 11.6,    -,  9.1,  8.2,  7.6
   auto tiles = [&](int64_t bm, int64_t bn) {
     return ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
   };
@@ -884,8 +895,10 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
     run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(128, 128) >= 192)
     run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
+  else if (tiles(64, 128) >= 160)
+    run_small<T, 2, 4, 1, 3>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(64, 64) >= 256)
-    run_small<T, 2, 2, 1, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
+    run_small<T, 2, 2, 1, 3>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(32, 64) >= 256)
     run_small<T, 1, 2, 2, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else

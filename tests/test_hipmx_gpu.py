@@ -140,6 +140,8 @@ SHAPES = [
     (16, 64, 8192), (3, 40, 20001), (16, 8200, 4200),
     # tiles of 32 x 64, with and without a rest of k
     (96, 8200, 300), (65, 8192, 512), (33, 8191, 2080),
+    # tiles of 64 x 128, 64 x 64 and 128 x 128 with a rest of k
+    (333, 5001, 296), (130, 5600, 544), (1600, 2000, 1000),
     # a step of k more or less than the loads under way
     (40, 64, 1536), (40, 64, 1537), (40, 64, 1280), (200, 8200, 768),
 ]
