@@ -272,21 +272,25 @@ struct Top {
     __syncthreads();
   }
 
-  // elements larger than `least` and not less than `bound` to the keys
-  __device__ void append(const u32x4* w, int64_t base, float thread_max,
+  // Elements larger than `least` and not less than `bound` to the keys. Words
+  // in which no lane has one, most of them, are passed over as a whole.
+  __device__ void append(const u32x4* w, const float* word_max, int64_t base,
                          float bound) {
-    if (!(thread_max > least && thread_max >= bound)) return;
     uint32_t which = 0;  // of the thread's elements
 #pragma unroll
-    for (int i = 0; i < U; i++)
+    for (int i = 0; i < U; i++) {
+      if (!__any((word_max[i] > least) & (word_max[i] >= bound))) continue;
 #pragma unroll
       for (int j = 0; j < E::kVec; j++) {
         const float x = E::get(w[i], j);
         which |= (uint32_t)((x > least) & (x >= bound)) << (i * E::kVec + j);
       }
+    }
+    if (!which) return;
     int at = atomicAdd(&sh.count, __popc(which));
 #pragma unroll
-    for (int i = 0; i < U; i++)
+    for (int i = 0; i < U; i++) {
+      if (!(which >> (i * E::kVec) & ((1u << E::kVec) - 1))) continue;
 #pragma unroll
       for (int j = 0; j < E::kVec; j++) {
         if (!(which >> (i * E::kVec + j) & 1)) continue;
@@ -296,6 +300,7 @@ struct Top {
               (uint32_t)(base + (i * kThreads + threadIdx.x) * E::kVec + j));
         at++;
       }
+    }
   }
 
   __device__ void merge(int n) {
@@ -320,8 +325,8 @@ struct Top {
     return key_value((uint64_t)max(found, 0x007FFFFFu) << 32);
   }
 
-  __device__ void take_bounded(const u32x4* w, int64_t base,
-                               float thread_max) {
+  __device__ void take_bounded(const u32x4* w, const float* word_max,
+                               int64_t base, float thread_max) {
     const int tid = threadIdx.x;
     const float mine = bound_of_wave(thread_max);
     if ((tid & 63) == 0) sh.bound[tid >> 6] = mine;
@@ -329,7 +334,7 @@ struct Top {
     float bound = sh.bound[0];
 #pragma unroll
     for (int i = 1; i < kWaves; i++) bound = fminf(bound, sh.bound[i]);
-    append(w, base, thread_max, bound);
+    append(w, word_max, base, bound);
     __syncthreads();
     int n = sh.count;
     __syncthreads();
@@ -374,7 +379,8 @@ struct Top {
     return sh.count;
   }
 
-  __device__ void take(const u32x4* w, int64_t base, float thread_max) {
+  __device__ void take(const u32x4* w, const float* word_max, int64_t base,
+                       float thread_max) {
     const int now = chunk % 3;
     chunk++;
     if (__any(thread_max > least) && (threadIdx.x & 63) == 0) sh.flag[now] = 1;
@@ -384,9 +390,9 @@ struct Top {
     if (!sh.flag[now]) return;
     if (have < k) {
       if (count > have) merge(count);
-      return take_bounded(w, base, thread_max);
+      return take_bounded(w, word_max, base, thread_max);
     }
-    append(w, base, thread_max, -INFINITY);
+    append(w, word_max, base, -INFINITY);
     __syncthreads();
     const int n = sh.count;
     if (n < 3 * k + 32) {
@@ -398,7 +404,7 @@ struct Top {
     if (threadIdx.x == 0) sh.count = count;
     __syncthreads();
     merge(count);  // what was there before this chunk
-    take_bounded(w, base, thread_max);
+    take_bounded(w, word_max, base, thread_max);
   }
 
   __device__ void finish() {
@@ -406,6 +412,150 @@ struct Top {
     if (count > have) merge(count);
   }
 };
+
+// ---------------------------------------------------------------------------
+// what is made of a row's sums
+// ---------------------------------------------------------------------------
+struct LogprobsEnd {
+  const int64_t* tokens;
+  int64_t ignore;
+  float inv_t;
+  int top;
+  float *logprobs, *entropy, *top_lp;
+  int64_t* top_ids;
+  RowStats* stats;
+};
+
+struct DistillEnd {
+  LmType type;  // of the teacher's record
+  const void* teacher;
+  const int64_t* ids;
+  int k;
+  float inv_t;
+  float *row_loss, *q;
+  RowStats* stats;
+};
+
+// a row's log probability, entropy and what its backward needs, by one
+// thread
+template <LmType T>
+__device__ void write_row(int64_t row, const typename Elem<T>::type* x,
+                          int64_t stride, int64_t v, const Triple& t,
+                          const LogprobsEnd& e) {
+  const int64_t token = e.tokens[row];
+  const float log2_sum = log2f(t.s);
+  const bool ignored = token == e.ignore;
+  const bool outside = !ignored && (token < 0 || token >= v);
+  const bool empty = t.m == -INFINITY && t.s == 0.f;
+  float lp, h;
+  if (ignored) {
+    lp = h = 0.f;
+  } else if (outside) {
+    lp = h = NAN;
+  } else if (empty) {
+    lp = -INFINITY;
+    h = 0.f;
+  } else {
+    const float xt = Elem<T>::load(x + row * stride + token);
+    lp = (xt - t.m) * e.inv_t - log2_sum * kLn2;
+    h = (log2_sum - t.u / t.s) * kLn2;
+    if (!(t.s == t.s)) lp = NAN;
+  }
+  e.logprobs[row] = lp;
+  e.entropy[row] = h;
+  if (e.stats)
+    e.stats[row] = {outside ? NAN : t.m, log2_sum, h,
+                  ignored || (empty && !outside) ? 0.f : 1.f};
+}
+
+// an alternative of a row; key 0 stands for none
+__device__ void write_top(int64_t row, int place, uint64_t key,
+                          const Triple& t, const LogprobsEnd& e) {
+  if (e.tokens[row] == e.ignore) key = 0;
+  const int64_t at = row * e.top + place;
+  e.top_lp[at] =
+      key ? (key_value(key) - t.m) * e.inv_t - log2f(t.s) * kLn2 : -INFINITY;
+  e.top_ids[at] = key ? (int64_t)key_index(key) : -1;
+}
+
+__device__ float load_any(LmType t, const void* p, int64_t i) {
+  switch (t) {
+    case LmType::F32:
+      return ((const float*)p)[i];
+    case LmType::BF16:
+      return Elem<LmType::BF16>::load((const uint16_t*)p + i);
+    default:
+      return Elem<LmType::F16>::load((const uint16_t*)p + i);
+  }
+}
+
+// a row by a wave: the teacher's softmax over its record, and
+// T^2 sum q (ln q - ln p). Returns (in every lane) the loss, and whether the
+// row has a record.
+struct RowLoss {
+  float loss;
+  bool there;
+};
+
+template <LmType T, class GetSums>
+__device__ RowLoss distill_row(
+    int64_t row, const typename Elem<T>::type* x, int64_t stride, int64_t v,
+    const DistillEnd& e, float c, GetSums sums) {
+  constexpr int kMine = kMaxRecord / 64;
+  const int lane = threadIdx.x & 63;
+  float z[kMine];
+  int64_t id[kMine];
+  float top = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    int at = lane + 64 * i;
+    id[i] = at < e.k ? e.ids[row * e.k + at] : -1;
+    z[i] = id[i] != -1 ? load_any(e.type, e.teacher, row * e.k + at) : -INFINITY;
+    if (z[i] == -INFINITY) id[i] = -1;
+    bad |= z[i] != z[i] || z[i] == INFINITY ||
+           (id[i] != -1 && (id[i] < 0 || id[i] >= v));
+    top = fmaxf(top, z[i]);
+  }
+  bad = __any(bad);
+  float xs[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    xs[i] = id[i] != -1 && !bad ? Elem<T>::load(x + row * stride + id[i]) : 0.f;
+  const Triple t = sums();
+  const bool empty = t.m == -INFINITY && t.s == 0.f;
+  const float log2_sum = log2f(t.s);
+  top = wave_max(top);
+  const bool absent = top == -INFINITY && !bad;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    sum += id[i] != -1 ? exp2_raw((z[i] - top) * c) : 0.f;
+  sum = wave_sum(sum);
+  const float log2_q = log2f(sum);
+  float loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    int at = lane + 64 * i;
+    float share = 0.f;
+    if (id[i] != -1 && !bad) {
+      float lq = (z[i] - top) * c - log2_q;
+      share = exp2_raw(lq);
+      float lp = empty ? -INFINITY : (xs[i] - t.m) * c - log2_sum;
+      if (share > 0.f) loss = fmaf(share, lq - lp, loss);
+    }
+    if (at < e.k) e.q[row * e.k + at] = share;
+  }
+  loss = wave_sum(loss) * (kLn2 / (e.inv_t * e.inv_t));
+  loss = absent ? 0.f : bad ? NAN : loss;
+  if (lane == 0) {
+    e.row_loss[row] = loss;
+    // in the entropy's place: whether the row counts in the mean
+    e.stats[row] = {bad ? NAN : t.m, log2_sum, absent ? 0.f : 1.f,
+                  absent || (empty && !bad) ? 0.f : 1.f};
+  }
+  return {loss, !absent};
+}
 
 // ---------------------------------------------------------------------------
 // one pass over a row, or over one of `splits` parts of it
@@ -419,12 +569,15 @@ struct Part {
   float pad;
 };
 
-template <LmType T, int U, bool kEntropy, bool kTop>
+// `direct`: a row is one block's, which also makes the results of its sums;
+// else they are left in parts and part_keys, for a kernel that joins them.
+template <LmType T, int U, bool kTop, class End>
 __global__ __launch_bounds__(kThreads, 4) void score_kernel(
     const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
-    int splits, int64_t part_len, float c, int k, Part* __restrict__ parts,
-    uint64_t* __restrict__ part_keys) {
+    int splits, int64_t part_len, float c, bool direct, End end_of_row,
+    Part* __restrict__ parts, uint64_t* __restrict__ part_keys) {
   using E = Elem<T>;
+  constexpr bool kDistill = std::is_same<End, DistillEnd>::value;
   constexpr int kChunk = kThreads * E::kVec * U;
   __shared__ typename std::conditional<kTop, TopShared, int>::type sh;
   __shared__ Triple wave_t[kWaves];
@@ -434,6 +587,8 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
   const int64_t end = min(v, begin + part_len);
   const typename E::type* src = x + row * stride;
   const int tid = threadIdx.x;
+  int k = 0;
+  if constexpr (kTop) k = end_of_row.top;
 
   typename std::conditional<kTop, Top<T, U>, NoTop>::type best(sh, k);
 
@@ -453,12 +608,15 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
         next[i] = load_vec<T>(
             src, base + kChunk + (int64_t)(i * kThreads + tid) * E::kVec, end);
     }
-    float chunk_max = -INFINITY;
+    float word_max[U], chunk_max = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < U; i++)
+    for (int i = 0; i < U; i++) {
+      word_max[i] = E::get(w[i], 0);
 #pragma unroll
-      for (int j = 0; j < E::kVec; j++)
-        chunk_max = fmaxf(chunk_max, E::get(w[i], j));
+      for (int j = 1; j < E::kVec; j++)
+        word_max[i] = fmaxf(word_max[i], E::get(w[i], j));
+      chunk_max = fmaxf(chunk_max, word_max[i]);
+    }
     if (chunk_max > t.m) t = under(t, chunk_max, c);
     const float m = or_zero(t.m);
     float s = 0.f, u = 0.f;
@@ -469,24 +627,37 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
         float y = (E::get(w[i], j) - m) * c;
         float e = exp2_raw(y);
         s += e;
-        if constexpr (kEntropy) u = fmaf(e, fmaxf(y, kLow), u);
+        if constexpr (!kDistill) u = fmaf(e, fmaxf(y, kLow), u);
       }
     t.s += s;
     t.u += u;
-    if constexpr (kTop) best.take(w, base, chunk_max);
+    if constexpr (kTop) best.take(w, word_max, base, chunk_max);
   }
 
   t = join_wave(t, c);
   if ((tid & 63) == 0) wave_t[tid >> 6] = t;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kWaves; i++) t = join(t, wave_t[i], c);
-    parts[blockIdx.x].t = t;
-  }
-  if constexpr (kTop) {
+  if constexpr (kTop)
     best.finish();
-    for (int i = tid; i < k; i += kThreads)
-      part_keys[(int64_t)blockIdx.x * k + i] = i < best.have ? sh.keys[i] : 0;
+  else
+    __syncthreads();
+  t = wave_t[0];
+  for (int i = 1; i < kWaves; i++) t = join(t, wave_t[i], c);
+  if (!direct) {
+    if (tid == 0) parts[blockIdx.x].t = t;
+    if constexpr (kTop) {
+      if (tid < k)
+        part_keys[(int64_t)blockIdx.x * k + tid] =
+            tid < best.have ? sh.keys[tid] : 0;
+    }
+  } else if constexpr (kDistill) {
+    if (tid < 64)
+      distill_row<T>(row, x, stride, v, end_of_row, c, [&] { return t; });
+  } else {
+    if (tid == 0) write_row<T>(row, x, stride, v, t, end_of_row);
+    if constexpr (kTop) {
+      if (tid < k)
+        write_top(row, tid, tid < best.have ? sh.keys[tid] : 0, t, end_of_row);
+    }
   }
 }
 
@@ -501,52 +672,16 @@ __device__ Triple join_parts(const Part* parts, int splits, float c) {
 // ---------------------------------------------------------------------------
 // token log probabilities
 // ---------------------------------------------------------------------------
-// a row's log probability, entropy and what its backward needs, by one
-// thread
-template <LmType T>
-__device__ void write_row(int64_t row, const typename Elem<T>::type* x,
-                          int64_t stride, int64_t v, const Triple& t,
-                          float log2_sum, int64_t token, int64_t ignore,
-                          float inv_t, float* logprobs, float* entropy,
-                          RowStats* stats) {
-  const bool ignored = token == ignore;
-  const bool outside = !ignored && (token < 0 || token >= v);
-  const bool empty = t.m == -INFINITY && t.s == 0.f;
-  float lp, h;
-  if (ignored) {
-    lp = h = 0.f;
-  } else if (outside) {
-    lp = h = NAN;
-  } else if (empty) {
-    lp = -INFINITY;
-    h = 0.f;
-  } else {
-    const float xt = Elem<T>::load(x + row * stride + token);
-    lp = (xt - t.m) * inv_t - log2_sum * kLn2;
-    h = (log2_sum - t.u / t.s) * kLn2;
-    if (!(t.s == t.s)) lp = NAN;
-  }
-  logprobs[row] = lp;
-  entropy[row] = h;
-  if (stats)
-    stats[row] = {outside ? NAN : t.m, log2_sum, h,
-                  ignored || (empty && !outside) ? 0.f : 1.f};
-}
-
 // a wave a row, without alternatives
 template <LmType T>
 __global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
     const typename Elem<T>::type* __restrict__ x, int64_t stride,
-    int64_t rows, int64_t v, const int64_t* __restrict__ tokens,
-    int64_t ignore, float inv_t, float c, const Part* __restrict__ parts,
-    int splits, float* __restrict__ logprobs, float* __restrict__ entropy,
-    RowStats* __restrict__ stats) {
+    int64_t rows, int64_t v, float c, const Part* __restrict__ parts,
+    int splits, LogprobsEnd e) {
   int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= rows) return;
   const Triple t = join_parts(parts + row * splits, splits, c);
-  if ((threadIdx.x & 63) == 0)
-    write_row<T>(row, x, stride, v, t, log2f(t.s), tokens[row], ignore, inv_t,
-                 logprobs, entropy, stats);
+  if ((threadIdx.x & 63) == 0) write_row<T>(row, x, stride, v, t, e);
 }
 
 // the r-th largest of the lanes' keys, 0 counting as none
@@ -574,17 +709,14 @@ __device__ uint64_t rth_of_wave(uint64_t key, int lanes, int r) {
 template <LmType T>
 __global__ __launch_bounds__(kThreads) void top_rows_kernel(
     const typename Elem<T>::type* __restrict__ x, int64_t stride, int64_t v,
-    const int64_t* __restrict__ tokens, int64_t ignore, float inv_t, float c,
-    const Part* __restrict__ parts, const uint64_t* __restrict__ part_keys,
-    int splits, int k, float* __restrict__ logprobs,
-    float* __restrict__ entropy, float* __restrict__ top_lp,
-    int64_t* __restrict__ top_ids, RowStats* __restrict__ stats) {
+    float c, const Part* __restrict__ parts,
+    const uint64_t* __restrict__ part_keys, int splits, LogprobsEnd e) {
   constexpr int kMine = kMaxKeys / kThreads;
   __shared__ uint64_t keys[kMaxKeys];
   __shared__ uint64_t best[kMaxTop], bounds[kWaves];
   __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, k = e.top;
   const uint64_t* src = part_keys + row * splits * k;
   const int all = splits * k;
   uint64_t mine[kMine];
@@ -597,7 +729,6 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
       rth_of_wave(lane < splits ? src[lane * k + place - 1] : 0, splits,
                   (k + place - 1) / place);
   const Triple t = join_parts(parts + row * splits, splits, c);
-  const int64_t token = tokens[row];
   if (lane == 0) bounds[tid >> 6] = bound_of_wave;
   if (tid == 0) count = 0;
   if (tid < k) best[tid] = 0;
@@ -617,17 +748,9 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
     for (int j = 0; j < n; j++) rank += keys[j] > key;
     if (rank < k) best[rank] = key;
   }
-  const float log2_sum = log2f(t.s);
-  if (tid == 0)
-    write_row<T>(row, x, stride, v, t, log2_sum, token, ignore, inv_t,
-                 logprobs, entropy, stats);
+  if (tid == 0) write_row<T>(row, x, stride, v, t, e);
   __syncthreads();
-  if (tid < k) {
-    const uint64_t key = token == ignore ? 0 : best[tid];
-    top_lp[row * k + tid] =
-        key ? (key_value(key) - t.m) * inv_t - log2_sum * kLn2 : -INFINITY;
-    top_ids[row * k + tid] = key ? (int64_t)key_index(key) : -1;
-  }
+  if (tid < k) write_top(row, tid, best[tid], t, e);
 }
 
 // dx_j = -p_j (a + b ln p_j) at every j, and g_lp / T more at the token,
@@ -689,87 +812,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(
 // ---------------------------------------------------------------------------
 // distillation
 // ---------------------------------------------------------------------------
-__device__ float load_any(LmType t, const void* p, int64_t i) {
-  switch (t) {
-    case LmType::F32:
-      return ((const float*)p)[i];
-    case LmType::BF16:
-      return Elem<LmType::BF16>::load((const uint16_t*)p + i);
-    default:
-      return Elem<LmType::F16>::load((const uint16_t*)p + i);
-  }
-}
-
-// a row by a wave: the teacher's softmax over its record, and
-// T^2 sum q (ln q - ln p). Returns (in every lane) the loss, and whether the
-// row has a record.
-struct RowLoss {
-  float loss;
-  bool there;
-};
-
-template <LmType T>
-__device__ RowLoss distill_row(
-    int64_t row, const typename Elem<T>::type* x, int64_t stride, int64_t v,
-    LmType tt, const void* teacher, const int64_t* ids, int k, float inv_t,
-    float c, const Part* parts, int splits, float* row_loss, float* q,
-    RowStats* stats) {
-  constexpr int kMine = kMaxRecord / 64;
-  const int lane = threadIdx.x & 63;
-  float z[kMine];
-  int64_t id[kMine];
-  float top = -INFINITY;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < kMine; i++) {
-    int at = lane + 64 * i;
-    id[i] = at < k ? ids[row * k + at] : -1;
-    z[i] = id[i] != -1 ? load_any(tt, teacher, row * k + at) : -INFINITY;
-    if (z[i] == -INFINITY) id[i] = -1;
-    bad |= z[i] != z[i] || z[i] == INFINITY ||
-           (id[i] != -1 && (id[i] < 0 || id[i] >= v));
-    top = fmaxf(top, z[i]);
-  }
-  bad = __any(bad);
-  float xs[kMine];
-#pragma unroll
-  for (int i = 0; i < kMine; i++)
-    xs[i] = id[i] != -1 && !bad ? Elem<T>::load(x + row * stride + id[i]) : 0.f;
-  const Triple t = join_parts(parts + row * splits, splits, c);
-  const bool empty = t.m == -INFINITY && t.s == 0.f;
-  const float log2_sum = log2f(t.s);
-  top = wave_max(top);
-  const bool absent = top == -INFINITY && !bad;
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kMine; i++)
-    sum += id[i] != -1 ? exp2_raw((z[i] - top) * c) : 0.f;
-  sum = wave_sum(sum);
-  const float log2_q = log2f(sum);
-  float loss = 0.f;
-#pragma unroll
-  for (int i = 0; i < kMine; i++) {
-    int at = lane + 64 * i;
-    float share = 0.f;
-    if (id[i] != -1 && !bad) {
-      float lq = (z[i] - top) * c - log2_q;
-      share = exp2_raw(lq);
-      float lp = empty ? -INFINITY : (xs[i] - t.m) * c - log2_sum;
-      if (share > 0.f) loss = fmaf(share, lq - lp, loss);
-    }
-    if (at < k) q[row * k + at] = share;
-  }
-  loss = wave_sum(loss) * (kLn2 / (inv_t * inv_t));
-  loss = absent ? 0.f : bad ? NAN : loss;
-  if (lane == 0) {
-    row_loss[row] = loss;
-    // in the entropy's place: whether the row counts in the mean
-    stats[row] = {bad ? NAN : t.m, log2_sum, absent ? 0.f : 1.f,
-                  absent || (empty && !bad) ? 0.f : 1.f};
-  }
-  return {loss, !absent};
-}
-
 // The waves' sums, in their order, by the block's first thread.
 __device__ void write_total(double s, double n, int mean, float* total,
                             float* count) {
@@ -793,29 +835,28 @@ __device__ void write_total(double s, double n, int mean, float* total,
 // kWhole: one block for all rows, which also adds them up
 template <LmType T, bool kWhole>
 __global__ __launch_bounds__(kWhole ? 1024 : kThreads) void
-distill_rows_kernel(
-    const typename Elem<T>::type* __restrict__ x, int64_t stride,
-    int64_t rows, int64_t v, LmType tt, const void* __restrict__ teacher,
-    const int64_t* __restrict__ ids, int k, float inv_t, float c,
-    const Part* __restrict__ parts, int splits, float* __restrict__ row_loss,
-    float* __restrict__ q, RowStats* __restrict__ stats, int mean,
-    float* __restrict__ total, float* __restrict__ count) {
+distill_rows_kernel(const typename Elem<T>::type* __restrict__ x,
+                    int64_t stride, int64_t rows, int64_t v, float c,
+                    const Part* __restrict__ parts, int splits, DistillEnd e,
+                    int mean, float* __restrict__ total,
+                    float* __restrict__ count) {
   const int64_t first =
       (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  auto make = [&](int64_t row) {
+    return distill_row<T>(row, x, stride, v, e, c, [&] {
+      return join_parts(parts + row * splits, splits, c);
+    });
+  };
   if constexpr (kWhole) {
     double s = 0, n = 0;
     for (int64_t row = first; row < rows; row += 16) {
-      const RowLoss r =
-          distill_row<T>(row, x, stride, v, tt, teacher, ids, k, inv_t, c,
-                         parts, splits, row_loss, q, stats);
+      const RowLoss r = make(row);
       s += r.loss;
       n += r.there;
     }
     write_total(s, n, mean, total, count);
   } else {
-    if (first < rows)
-      distill_row<T>(first, x, stride, v, tt, teacher, ids, k, inv_t, c, parts,
-                     splits, row_loss, q, stats);
+    if (first < rows) make(first);
   }
 }
 
@@ -907,10 +948,15 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
 // ---------------------------------------------------------------------------
 // launching
 // ---------------------------------------------------------------------------
-// Parts of a row. A block keeps about 16 KB in flight, and a few blocks a
-// compute unit are needed to keep memory busy: rows are split until there
-// are kWant blocks, into parts of whole chunks.
+// Parts of a row. Rows are split into parts of whole chunks until there are
+// kWant blocks (kWantPlain without alternatives, which leave less to do
+// between the loads); kWhole rows and more are not, which saves the launch
+// that joins the parts. In us for 512 and 1024 blocks: 509 x 50001 f32
+// without alternatives 20.9, 23.7, with 5 of them 30.4, 31.4; 256 x 131072
+// bf16 17.7, 18.8 and 37.2, 31.0.
 constexpr int64_t kWant = 1024;
+constexpr int64_t kWantPlain = 512;
+constexpr int64_t kWhole = 384;
 constexpr int64_t kMaxSplits = 64;
 
 struct Plan {
@@ -923,11 +969,13 @@ int vec_of(LmType t) { return t == LmType::F32 ? 4 : 8; }
 Plan plan_of(LmType t, int64_t rows, int64_t v, int top) {
   Plan p;
   int64_t word = (int64_t)kThreads * vec_of(t);
-  p.unroll = rows * ((v + 4 * word - 1) / (4 * word)) >= kWant ? 4 : 1;
+  const int64_t want = top ? kWant : kWantPlain;
+  p.unroll = rows * ((v + 4 * word - 1) / (4 * word)) >= want ? 4 : 1;
   int64_t chunk = word * p.unroll;
   int64_t chunks = (v + chunk - 1) / chunk;
   int64_t splits = std::min(std::min(chunks, kMaxSplits),
-                            std::max<int64_t>(1, kWant / rows));
+                            std::max<int64_t>(1, want / rows));
+  if (rows >= kWhole) splits = 1;
   if (top) splits = std::min<int64_t>(splits, kMaxKeys / top);
   p.part_len = (chunks + splits - 1) / splits * chunk;
   p.splits = (v + p.part_len - 1) / p.part_len;
@@ -955,21 +1003,21 @@ void by_type(LmType t, F f) {
   HIP_CHECK(hipGetLastError());
 }
 
-template <bool kEntropy>
+template <class End>
 void run_score(LmType t, const void* x, int64_t stride, int64_t rows,
-               int64_t v, const Plan& p, float c, int top, Part* parts,
-               uint64_t* keys, hipStream_t stream) {
+               int64_t v, const Plan& p, float c, bool top, bool direct,
+               const End& end, Part* parts, uint64_t* keys,
+               hipStream_t stream) {
   check_grid(rows * p.splits);
   auto go = [&](auto type, auto unroll, auto with_top) {
     constexpr LmType T = decltype(type)::value;
-    score_kernel<T, decltype(unroll)::value, kEntropy,
-                 decltype(with_top)::value>
+    score_kernel<T, decltype(unroll)::value, decltype(with_top)::value, End>
         <<<dim3((unsigned)(rows * p.splits)), kThreads, 0, stream>>>(
             (const typename Elem<T>::type*)x, stride, v, (int)p.splits,
-            p.part_len, c, top, parts, keys);
+            p.part_len, c, direct, end, parts, keys);
   };
   auto by_top = [&](auto type, auto unroll) {
-    if constexpr (kEntropy) {
+    if constexpr (std::is_same<End, LogprobsEnd>::value) {
       if (top) return go(type, unroll, std::true_type{});
     }
     go(type, unroll, std::false_type{});
@@ -1000,19 +1048,22 @@ void launch_token_logprobs(LmType t, const void* x, int64_t stride,
   const float c = inv_t * kLog2e;
   Part* parts = (Part*)ws;
   uint64_t* keys = (uint64_t*)(parts + rows * p.splits);
-  run_score<true>(t, x, stride, rows, v, p, c, top, parts, keys, stream);
+  const LogprobsEnd e = {tokens,  ignore, inv_t,   top,  logprobs,
+                         entropy, top_lp, top_ids, stats};
+  const bool direct = p.splits == 1;
+  run_score(t, x, stride, rows, v, p, c, top > 0, direct, e, parts, keys,
+            stream);
+  if (direct) return;
   by_type(t, [&](auto type) {
     constexpr LmType T = decltype(type)::value;
     auto* xt = (const typename Elem<T>::type*)x;
     if (top)
       top_rows_kernel<T><<<dim3((unsigned)rows), kThreads, 0, stream>>>(
-          xt, stride, v, tokens, ignore, inv_t, c, parts, keys, (int)p.splits,
-          top, logprobs, entropy, top_lp, top_ids, stats);
+          xt, stride, v, c, parts, keys, (int)p.splits, e);
     else
       logprobs_rows_kernel<T>
           <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
-             stream>>>(xt, stride, rows, v, tokens, ignore, inv_t, c, parts,
-                       (int)p.splits, logprobs, entropy, stats);
+             stream>>>(xt, stride, rows, v, c, parts, (int)p.splits, e);
   });
 }
 
@@ -1044,22 +1095,25 @@ void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
   Plan p = plan_of(t, rows, v, 0);
   const float c = inv_t * kLog2e;
   Part* parts = (Part*)ws;
+  const DistillEnd e = {tt, teacher, ids, k, inv_t, row_loss, q, stats};
   // up to 4 rows a wave a launch less is the shorter way
   const bool whole = total && rows <= 64;
-  run_score<false>(t, x, stride, rows, v, p, c, 0, parts, nullptr, stream);
-  by_type(t, [&](auto type) {
-    constexpr LmType T = decltype(type)::value;
-    auto go = [&](auto w) {
-      constexpr bool W = decltype(w)::value;
-      distill_rows_kernel<T, W>
-          <<<dim3(W ? 1 : (unsigned)((rows + kWaves - 1) / kWaves)),
-             W ? 1024 : kThreads, 0, stream>>>(
-              (const typename Elem<T>::type*)x, stride, rows, v, tt, teacher,
-              ids, k, inv_t, c, parts, (int)p.splits, row_loss, q, stats, mean,
-              total, count);
-    };
-    whole ? go(std::true_type{}) : go(std::false_type{});
-  });
+  const bool direct = p.splits == 1 && !whole;
+  run_score(t, x, stride, rows, v, p, c, false, direct, e, parts, nullptr,
+            stream);
+  if (!direct)
+    by_type(t, [&](auto type) {
+      constexpr LmType T = decltype(type)::value;
+      auto go = [&](auto w) {
+        constexpr bool W = decltype(w)::value;
+        distill_rows_kernel<T, W>
+            <<<dim3(W ? 1 : (unsigned)((rows + kWaves - 1) / kWaves)),
+               W ? 1024 : kThreads, 0, stream>>>(
+                (const typename Elem<T>::type*)x, stride, rows, v, c, parts,
+                (int)p.splits, e, mean, total, count);
+      };
+      whole ? go(std::true_type{}) : go(std::false_type{});
+    });
   if (total && !whole) {
     distill_total_kernel<<<1, 1024, 0, stream>>>(row_loss, stats, rows, mean,
                                                  total, count);
