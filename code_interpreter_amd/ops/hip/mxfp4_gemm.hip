@@ -83,7 +83,10 @@ __device__ __forceinline__ float bias_at(const void* bias, int64_t i) {
 // row's end. Rows' scales for a step are then neighbours in memory, where in
 // a row's own order a wave would touch a cache line for every row.
 constexpr int kPrepareThreads = 256;
-constexpr int kPrepareRows = 32;  // of a block that quantises one step
+
+// A block that quantises takes kPrepareSteps steps of kPrepareRows rows: 8192
+// x 8192 bf16 in 42 us, 46 with 1 step, 45 with 4.
+constexpr int kPrepareSteps = 2, kPrepareRows = 32 / kPrepareSteps;
 constexpr int kLayRows = kPrepareThreads, kLaySteps = 4;  // of one that does not
 
 __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
@@ -128,30 +131,33 @@ __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
   if constexpr (kPacked) {
     lay_out_scales(xs, (uint2*)xst, m, nb, steps, blockIdx.x);
   } else {
-    constexpr int kGroups = kPrepareRows * 32 / kPrepareThreads;
-    const int t = blockIdx.x % steps;
-    const int64_t row0 = (int64_t)(blockIdx.x / steps) * kPrepareRows +
-                         (threadIdx.x >> 5);
-    const int col = threadIdx.x & 31;  // of the step's groups of 8 elements
-    const int blk = t * 8 + (col >> 2);
+    constexpr int kRowGroups = kPrepareSteps * 32;
+    constexpr int kGroups = kPrepareRows * kRowGroups / kPrepareThreads;
+    const int parts = (steps + kPrepareSteps - 1) / kPrepareSteps;
+    const int64_t row0 = (int64_t)(blockIdx.x / parts) * kPrepareRows +
+                         threadIdx.x / kRowGroups;
+    // of a row's groups of 8 elements, and the block it belongs to
+    const int col = blockIdx.x % parts * kRowGroups + threadIdx.x % kRowGroups;
+    const int blk = col >> 2;
+    if (blk >= steps * 8) return;  // whole waves or halves: of 32 groups
     u32x4 w[kGroups], w2[kGroups];
 #pragma unroll
     for (int i = 0; i < kGroups; i++) {
-      const int64_t row = row0 + i * (kPrepareThreads / 32);
+      const int64_t row = row0 + i * (kPrepareThreads / kRowGroups);
       if (row < m)
-        load8<T>(x + row * stride * Size<T>::value,
-                 (int64_t)t * 256 + col * kPer, k, w[i], w2[i]);
+        load8<T>(x + row * stride * Size<T>::value, (int64_t)col * kPer, k,
+                 w[i], w2[i]);
     }
 #pragma unroll
     for (int i = 0; i < kGroups; i++) {
-      const int64_t row = row0 + i * (kPrepareThreads / 32);
+      const int64_t row = row0 + i * (kPrepareThreads / kRowGroups);
       if (row >= m) break;
       uint32_t byte = block_scale<T>(w[i], w2[i]);
       if (blk < nb)
-        codes[(row * nb + t * 8) * 4 + col] =
+        codes[row * nb * 4 + col] =
             byte == 255 ? 0u : encode<T>(w[i], w2[i], scale_value(byte));
       if ((col & 3) == 0)
-        xst[(t * m + row) * 8 + (col >> 2)] =
+        xst[((blk >> 3) * m + row) * 8 + (blk & 7)] =
             blk < nb ? (uint8_t)byte : 0x7F;
     }
   }
@@ -860,7 +866,9 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   };
   const int64_t w_blocks = lay_blocks(n);
   const int64_t x_blocks =
-      x ? (m + kPrepareRows - 1) / kPrepareRows * steps : lay_blocks(m);
+      x ? (m + kPrepareRows - 1) / kPrepareRows *
+              ((steps + kPrepareSteps - 1) / kPrepareSteps)
+        : lay_blocks(m);
   // a token tile's offsets into the codes are 32 bits
   if (x_blocks + w_blocks >= (int64_t)1 << 31 || nb * kMxBytes >= 1 << 23)
     throw std::runtime_error("product too large for one launch");
@@ -880,8 +888,11 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   // m x n x k with tiles of 256 x 256, 128 x 128 (2 buffers), 64 x 128, 64 x
   // 64 (3), 32 x 64 (4), 32 x 32 (6):
   // 2000 x 5001 x 2056 30.6, 33.0,    -,    -, 49.0, 74.0
-  // 2000 x 4096 x 4096 39.1, 33.4,    -,    -, 56.8, 86.9
-  //  800 x 4096 x 4096 34.8, 22.5, 21.7, 25.5, 28.7, 40.1
+  // 2000 x 4096 x 4096 38.8, 33.5, 40.5,    -, 56.8, 86.9
+  // 1200 x 8192 x 8192 60.6, 74.8, 78.2,    -,    -,    -
+  //  800 x 8192 x 8192 56.1, 48.3, 58.5,    -,    -,    -
+  //  800 x 4096 x 4096 34.0, 22.5, 22.1, 25.5, 28.7, 40.1
+  //  333 x 8192 x 8192 52.1, 34.1, 32.4,    -,    -,    -
   //  500 x 4096 x 4096    -, 21.2, 16.4, 16.7, 21.5,    -
   //  333 x 5001 x 2056 25.7, 15.2, 12.0, 13.4, 16.4, 20.2
   //  200 x 4096 x 4096    -, 19.5, 14.2, 13.0, 12.5,    -
@@ -893,7 +904,7 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   const int b = (int)nb;
   if (tiles(256, 256) >= 144)
     run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
-  else if (tiles(128, 128) >= 192)
+  else if (tiles(128, 128) >= 240)
     run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(64, 128) >= 160)
     run_small<T, 2, 4, 1, 3>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
