@@ -902,9 +902,11 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
     return ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
   };
   const int b = (int)nb;
+  // the small tiles' scales are addressed in 31 bits
+  const bool far = std::max(m, n) * steps * 8 >= (int64_t)1 << 31;
   if (tiles(256, 256) >= 144)
     run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
-  else if (tiles(128, 128) >= 240)
+  else if (tiles(128, 128) >= 240 || far)
     run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(64, 128) >= 160)
     run_small<T, 2, 4, 1, 3>(xc, xs2, wc, wst, bias, y, m, n, b, stream);

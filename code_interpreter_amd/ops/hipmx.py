@@ -24,6 +24,7 @@ torch, to the same codes. Products have no backward.
 import hiptorch
 
 BLOCK = 32
+MAX_K = (1 << 24) - 32  # of a product
 
 STATS = {"quantize": 0, "dequantize": 0, "linear": 0}
 
@@ -137,7 +138,7 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
     input: a tensor [..., k] (float32, bfloat16, float16), which is quantised
     as by ``quantize`` on the way in and gives the result its type, or an
     MXFP4Tensor, with the result's type in ``dtype`` (bfloat16 if not given).
-    weight: [n, k]. bias: [n], of the result's type. Sums are float32; the
+    weight: [n, k], k below 2^24. bias: [n], of the result's type. Sums are float32; the
     result is rounded once. There is no backward: tensors that require a
     gradient are refused while gradients are enabled.
     """
@@ -148,6 +149,8 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
     if len(weight.shape) != 2:
         raise ValueError(f"weight must be [n, k], got {list(weight.shape)}")
     n, k = weight.shape
+    if k > MAX_K:
+        raise ValueError(f"the last axis is {k} long, {MAX_K} is the most")
     wcodes = weight.codes
     packed = isinstance(input, MXFP4Tensor)
     if packed:

@@ -501,3 +501,26 @@ def test_a_head_records_and_a_student_learns(lm):
             1, said.top_tokens, said.top_logprobs),
         said.top_logprobs, said.top_tokens)
     assert abs(same.item()) < 64 * relative(vocab)
+
+
+def test_far_offsets(lm):
+    """Logits whose later rows stand behind 2^32 bytes and elements."""
+    torch, hiplm = lm
+    rows, v = 70_000, 65_537  # 4.6e9 elements
+    x = torch.zeros(rows, v, dtype=torch.bfloat16, device="cuda")
+    x[-30:] = torch.randn(30, v, device="cuda").bfloat16()
+    tokens = torch.randint(v, (rows,), device="cuda")
+    teacher = torch.randn(rows, 5, device="cuda")
+    ids = torch.randint(v, (rows, 5), device="cuda")
+    outs = []
+    for cut in (slice(None), slice(rows - 400, None)):
+        z = x[cut].detach().requires_grad_(True)
+        r = hiplm.token_logprobs(z, tokens[cut], top=3)
+        loss = hiplm.topk_distill_loss(z, teacher[cut], ids[cut],
+                                       reduction="none")
+        (dx,) = torch.autograd.grad(r.logprobs, [z], torch.ones_like(loss))
+        (dz,) = torch.autograd.grad(loss, [z], torch.ones_like(loss))
+        outs.append([t[-400:].detach().clone() for t in (*r, loss, dx, dz)])
+        del dx, dz, z, r, loss
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)

@@ -141,6 +141,9 @@ def test_refusals():
         hipmx.linear(x[:, :32], w)
     with pytest.raises(ValueError, match=r"\[n, k\]"):
         hipmx.linear(x, hipmx.quantize(torch.randn(2, 8, 64)))
+    with pytest.raises(ValueError, match="is the most"):
+        long = hipmx.quantize(torch.zeros(1, 1 << 24))
+        hipmx.linear(torch.zeros(1, 1 << 24), long)
     with pytest.raises(ValueError, match="bias must be"):
         hipmx.linear(x, w, torch.zeros(7))
     with pytest.raises(ValueError, match="bias must be"):

@@ -323,3 +323,48 @@ def test_mixed_devices_are_refused(mx):
         hipmx.MXFP4Tensor(w.codes, w.scales.cpu(), 96)
     moved = w.to("cpu")
     assert torch.equal(moved.dequantize(), w.dequantize().cpu())
+
+
+def test_far_offsets(mx):
+    """Tensors whose later rows stand behind 2^32 bytes and elements."""
+    torch, hipmx = mx
+    rows, k = 140_000, 32_768  # 4.6e9 elements, 2.3e9 bytes of codes
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda")
+    last = torch.randn(64, k, device="cuda").bfloat16()
+    x[:64] = last.flip(0)
+    x[-64:] = last
+    q, want = hipmx.quantize(x), hipmx.quantize(last)
+    assert torch.equal(q.codes[-64:], want.codes)
+    assert torch.equal(q.scales[-64:], want.scales)
+    del x
+    v = q.dequantize()
+    assert torch.equal(v[-64:], want.dequantize())
+    del v
+    # as a weight, twice as long: the last rows' codes are behind 4 GB
+    w = hipmx.MXFP4Tensor(torch.cat([q.codes, q.codes]),
+                          torch.cat([q.scales, q.scales]), k)
+    del q
+    for m in (2, 20, 300):
+        t = torch.randn(m, k, device="cuda").bfloat16()
+        y = hipmx.linear(t, w)
+        near = hipmx.linear(t, want)
+        torch.testing.assert_close(y[:, -64:], near, rtol=0.02, atol=0.5)
+        torch.testing.assert_close(y[:, :64], near.flip(1), rtol=0.02,
+                                   atol=0.5)
+    # as tokens: the rows of the result too
+    y = hipmx.linear(w, want)
+    near = hipmx.linear(want, want)
+    torch.testing.assert_close(y[-64:], near, rtol=0.02, atol=0.5)
+
+
+def test_long_rows(mx):
+    torch, hipmx = mx
+    k = hipmx.MAX_K
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(2, k, generator=g, device="cuda").sign()
+    w = hipmx.quantize(torch.randn(3, k, generator=g, device="cuda").sign())
+    want = x.double() @ w.dequantize(torch.float32).double().T
+    # sums of ones: whole numbers below 2^24, exact in any order
+    assert torch.equal(hipmx.linear(x, w).double(), want)
+    assert torch.equal(hipmx.linear(x.repeat(20, 1), w).double(),
+                       want.repeat(20, 1))
