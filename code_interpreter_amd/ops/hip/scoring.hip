@@ -260,10 +260,14 @@ struct Top {
   using E = Elem<T>;
   TopShared& sh;
   const int k;
+  const typename E::type* const src;  // the row, and where its part ends
+  const int64_t end;
   int have = 0, count = 0, chunk = 0;  // equal in all threads
   float least = -INFINITY;
 
-  __device__ Top(TopShared& sh, int k) : sh(sh), k(k) {
+  __device__ Top(TopShared& sh, int k, const typename E::type* src,
+                 int64_t end)
+      : sh(sh), k(k), src(src), end(end) {
     if (threadIdx.x == 0) {
       sh.count = 0;
       sh.least = least;
@@ -341,25 +345,29 @@ struct Top {
     if (n > kCap) {
       if (tid == 0) sh.count = have;
       __syncthreads();
-      n = one_by_one(w, base);
+      n = one_by_one(base);
     }
     merge(n);
   }
 
-  __device__ int one_by_one(const u32x4* w, int64_t base) {
+  // Seldom used, and so from memory: held against the chunk in registers its
+  // keys would cost all chunks theirs.
+  __device__ int one_by_one(int64_t base) {
     const int tid = threadIdx.x;
     uint64_t last = ~0ull;
     for (int r = 0; r < k; r++) {
       uint64_t mine = 0;
-#pragma unroll
-      for (int i = 0; i < U; i++)
+#pragma unroll 1
+      for (int i = 0; i < U; i++) {
+        const int64_t at = base + (int64_t)(i * kThreads + tid) * E::kVec;
+        const u32x4 w = load_vec<T>(src, at, end);
 #pragma unroll
         for (int j = 0; j < E::kVec; j++) {
-          const float x = E::get(w[i], j);
-          const uint64_t key = make_key(
-              x, (uint32_t)(base + (i * kThreads + tid) * E::kVec + j));
+          const float x = E::get(w, j);
+          const uint64_t key = make_key(x, (uint32_t)(at + j));
           if (x > least && key < last && key > mine) mine = key;
         }
+      }
 #pragma unroll
       for (int d = 32; d; d >>= 1) {
         const uint64_t o = __shfl_xor((unsigned long long)mine, d);
@@ -561,7 +569,7 @@ __device__ RowLoss distill_row(
 // one pass over a row, or over one of `splits` parts of it
 // ---------------------------------------------------------------------------
 struct NoTop {
-  __device__ NoTop(int&, int) {}
+  __device__ NoTop(int&, int, const void*, int64_t) {}
 };
 
 struct Part {
@@ -590,7 +598,8 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
   int k = 0;
   if constexpr (kTop) k = end_of_row.top;
 
-  typename std::conditional<kTop, Top<T, U>, NoTop>::type best(sh, k);
+  typename std::conditional<kTop, Top<T, U>, NoTop>::type best(sh, k, src,
+                                                                  end);
 
   Triple t = {-INFINITY, 0.f, 0.f};
   u32x4 next[U];
