@@ -16,6 +16,12 @@
 // has m = -inf and S = 0 and is reported as empty. A NaN or +inf makes S
 // NaN, and with it all of the row's numbers.
 //
+// Memory bounds all of it, with the vector units close behind for 16-bit
+// logits: 9 instructions an element forward, an exponential among them. 4096
+// x 131072 bf16: 217 us forward, 4.9 TB/s; backward 340 us, 6.3 TB/s (part
+// of what is read again comes from the chip's cache). Distillation backward,
+// 4096 x 65536: 190 us, 5.6 TB/s. A large copy: 4.8 TB/s.
+//
 // All sums are 32-bit, over a fixed split of the row and in a fixed order:
 // the same input gives the same bits.
 
