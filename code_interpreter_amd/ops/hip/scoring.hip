@@ -338,7 +338,9 @@ struct Top {
   __device__ void take_bounded(const u32x4* w, const float* word_max,
                                int64_t base, float thread_max) {
     const int tid = threadIdx.x;
-    const float mine = bound_of_wave(thread_max);
+    // NaN's order would be the largest of all
+    const float mine =
+        bound_of_wave(thread_max == thread_max ? thread_max : -INFINITY);
     if ((tid & 63) == 0) sh.bound[tid >> 6] = mine;
     __syncthreads();
     float bound = sh.bound[0];
@@ -402,10 +404,7 @@ struct Top {
     // the flag of the chunk after the next: it is set behind another barrier
     if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
     if (!sh.flag[now]) return;
-    if (have < k) {
-      if (count > have) merge(count);
-      return take_bounded(w, word_max, base, thread_max);
-    }
+    if (have < k) return take_bounded(w, word_max, base, thread_max);
     append(w, word_max, base, -INFINITY);
     __syncthreads();
     const int n = sh.count;

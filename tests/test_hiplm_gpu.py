@@ -175,6 +175,28 @@ def test_top_of_hard_rows(lm):
                                one.top_tokens.repeat(150, 1))
 
 
+@pytest.mark.parametrize("rows", [1, 500])
+def test_top_of_rows_with_nan(lm, rows):
+    """Numbers are chosen from what is one, also where some of a block's
+    threads see nothing but NaN; all log probabilities of the row are NaN."""
+    torch, hiplm = lm
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(rows, 30011, generator=g)
+    x[:, :600] = math.nan     # what a block's first threads take
+    x[:, 9000:20000] = math.nan
+    x[0, 25000] = math.inf
+    tokens = torch.full((rows,), 700)
+    for dtype in DTYPES:
+        few = x.to(getattr(torch, dtype))
+        for top in (1, 7, 40, 128):
+            r = hiplm.token_logprobs(few.cuda(), tokens.cuda(), top=top)
+            want = few.float().nan_to_num(-math.inf, math.inf).sort(
+                dim=-1, descending=True, stable=True)[1][:, :top]
+            assert torch.equal(r.top_tokens.cpu(), want)
+            for part in (r.logprobs, r.entropy, r.top_logprobs):
+                assert part.isnan().all()
+
+
 def check_grad(torch, got, want, size, v, dtype):
     """One rounding to the logits' type, and the error of p: of its exponent,
     and of the row's sum. The hardware's exponential has no subnormal
