@@ -37,16 +37,21 @@ at::ScalarType scalar_type(int64_t code) {
   return code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf;
 }
 
+// t's values as they stand in memory: of a view that negates, a copy
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+Tensor plain(const Tensor& t) { return resolved(t).contiguous(); }
+
 // x as [rows, v] with neighbouring elements in a row: a view where its
 // strides allow one, else a copy
 struct Rows {
   Tensor x;
   int64_t rows, v, stride;
 
-  explicit Rows(const Tensor& t) : x(t) {
+  explicit Rows(const Tensor& t) : x(resolved(t)) {
     v = t.size(-1);
     rows = t.numel() / v;
-    if (t.dim() != 2) x = t.reshape({rows, v});
+    if (t.dim() != 2) x = x.reshape({rows, v});
     if (v > 1 && x.stride(1) != 1) x = x.contiguous();
     stride = rows > 1 ? x.stride(0) : v;
   }
@@ -121,7 +126,7 @@ Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
   Launch on(x);
   const int64_t need = mx_linear_workspace(m, n, k, packed);
   Tensor work = need ? empty(wc, {need}, at::kByte) : Tensor();
-  const Tensor b = bias.defined() ? bias.contiguous() : bias;
+  const Tensor b = bias.defined() ? plain(bias) : bias;
   if (packed) {
     launch_mx_linear((LmType)code, nullptr, 0, data<uint8_t>(x),
                      data<uint8_t>(xs), data<uint8_t>(wc), data<uint8_t>(ws),
@@ -197,14 +202,14 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
     if (!grads[0].defined() && !grads[1].defined()) return result;
     Tensor dx;
     {
-      at::NoGradGuard plain;
+      at::NoGradGuard no_grad;
       auto saved = ctx->get_saved_variables();
       const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
-        const Tensor g_lp = grads[0].defined() ? grads[0].contiguous() : Tensor();
-        const Tensor g_h = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor g_lp = grads[0].defined() ? plain(grads[0]) : Tensor();
+        const Tensor g_h = grads[1].defined() ? plain(grads[1]) : Tensor();
         Launch on(logits);
         launch_token_logprobs_bwd(
             (LmType)ctx->saved_data["code"].toInt(), r.x.data_ptr(), r.stride,
@@ -229,6 +234,7 @@ Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
              int64_t code, int64_t teacher_code, double inv_t, int64_t how) {
   const LmType t = (LmType)code;
   Rows r(logits);
+  const Tensor record = plain(teacher);
   const int64_t k = ids.size(-1);
   Loss l = {empty(logits, how ? at::IntArrayRef() : lead(logits), at::kFloat),
             empty(logits, {r.rows * (4 + k) + (how ? 1 + r.rows : 0)},
@@ -243,7 +249,7 @@ Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
   Launch on(logits);
   Tensor work = empty(logits, {score_workspace(t, r.rows, r.v, 0)}, at::kByte);
   launch_distill(t, r.x.data_ptr(), r.stride, r.rows, r.v,
-                 (LmType)teacher_code, teacher.data_ptr(), data<int64_t>(ids),
+                 (LmType)teacher_code, record.data_ptr(), data<int64_t>(ids),
                  (int)k, (float)inv_t, how ? count + 1 : data(l.loss), q,
                  (RowStats*)stats, how ? data(l.loss) : nullptr, count,
                  how == 2, work.data_ptr(), on.stream);
@@ -268,13 +274,13 @@ class Distill : public torch::autograd::Function<Distill> {
     variable_list result(7);
     Tensor dx;
     {
-      at::NoGradGuard plain;
+      at::NoGradGuard no_grad;
       auto saved = ctx->get_saved_variables();
       const Tensor &logits = saved[0], &ids = saved[1], &kept = saved[2];
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
-        const Tensor grad = grads[0].contiguous();
+        const Tensor grad = plain(grads[0]);
         const int64_t k = ids.size(-1);
         const bool whole = ctx->saved_data["whole"].toBool();
         const float* stats = data(kept);
@@ -360,7 +366,7 @@ PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   std::pair<Tensor, Tensor> q;
   {
     pybind11::gil_scoped_release no_gil;
-    at::NoGradGuard plain;
+    at::NoGradGuard no_grad;
     q = quantize(x, code);
   }
   return tuple({q.first, q.second});
@@ -392,7 +398,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor y;
   {
     pybind11::gil_scoped_release no_gil;
-    at::NoGradGuard plain;
+    at::NoGradGuard no_grad;
     y = linear(x, xs, wc, ws, bias, k, code);
   }
   return THPVariable_Wrap(y);
@@ -418,7 +424,7 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
       logprobs = out[0];
       entropy = out[1];
     } else {
-      at::NoGradGuard plain;
+      at::NoGradGuard no_grad;
       Scores s = score(logits, tokens, top_lp, top_ids, code, inv_t, ignore,
                        false);
       logprobs = s.logprobs;
@@ -445,7 +451,7 @@ PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
       loss = Distill::apply(logits, teacher, ids, code, teacher_code, inv_t,
                             how)[0];
     } else {
-      at::NoGradGuard plain;
+      at::NoGradGuard no_grad;
       loss = distill(logits, teacher, ids, code, teacher_code, inv_t, how).loss;
     }
   }

@@ -10,6 +10,13 @@ enum class LmType : int { F32 = 0, BF16 = 1, F16 = 2 };
 constexpr int kMxBlock = 32;   // elements that share a scale
 constexpr int kMxBytes = 16;   // bytes of codes of a block
 
+// a grid of one axis: its threads are counted in 32 bits
+inline dim3 lm_grid(int64_t blocks, int threads) {
+  if (blocks > (int64_t)0xFFFFFFFF / threads)
+    throw std::runtime_error("too many rows for one launch");
+  return dim3((unsigned)blocks);
+}
+
 inline int64_t mx_blocks(int64_t k) { return (k + kMxBlock - 1) / kMxBlock; }
 
 // x: [rows][k], row stride in elements. codes: [rows][blocks][16],

@@ -527,16 +527,16 @@ __global__ __launch_bounds__(WM* WN* WK * 64) void small_kernel(
     off[i] = (uint32_t)(at * row_bytes) + unit * 16;
   }
   // scales: words 2 r, 2 r + 1 of row r. A wave behind the last word loads
-  // the first ones once more, to a place that is not read. Rows behind the
-  // operand's last one get some other row's, or 0: they are not stored.
+  // the first ones once more, to a place that is not read.
   constexpr int kScaleWaves = (BM + BN) * 2 / 64;
   static_assert(kScaleWaves <= kWaves, "");
   const int word0 = (wave % kScaleWaves) * 64;
   const bool of_x = word0 >= BN * 2;
   const auto sr = of_x ? buffer(xs, m * steps * 8) : buffer(ws, n * steps * 8);
   const int sstep = (int)(of_x ? m : n) * 8;
-  const int soff = (int)(of_x ? m0 : n0) * 8 +
-                   (word0 + lane - (of_x ? BN * 2 : 0)) * 4;
+  const int64_t r0 = of_x ? m0 : n0, last = (of_x ? m : n) - 1;
+  const int64_t srow = min(r0 + (word0 + lane - (of_x ? BN * 2 : 0)) / 2, last);
+  const int soff = (int)srow * 8 + (lane & 1) * 4;
 
   auto stage = [&](int t, int into) {
     char* to = smem + into * kBuf;
@@ -823,10 +823,8 @@ void run_tile(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
               int64_t n, int nb, hipStream_t stream) {
   constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
   int64_t tm = (m + BM - 1) / BM, tn = (n + BN - 1) / BN;
-  if (tm * tn >= (int64_t)1 << 28)
-    throw std::runtime_error("product too large for one launch");
   tile_kernel<T, WM, WN, FM, FN>
-      <<<dim3((unsigned)(tm * tn)), WM * WN * 64, 2 * (BM + BN) * 128,
+      <<<lm_grid(tm * tn, WM * WN * 64), WM * WN * 64, 2 * (BM + BN) * 128,
          stream>>>(xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
   HIP_CHECK(hipGetLastError());
 }
@@ -837,10 +835,8 @@ void run_small(const uint8_t* xc, const uint2* xs, const uint8_t* wc,
                int64_t n, int nb, hipStream_t stream) {
   constexpr int BM = WM * 32, BN = WN * 32;
   int64_t tm = (m + BM - 1) / BM, tn = (n + BN - 1) / BN;
-  if (tm * tn >= (int64_t)1 << 28)
-    throw std::runtime_error("product too large for one launch");
   small_kernel<T, WM, WN, WK, kStages>
-      <<<dim3((unsigned)(tm * tn)), WM * WN * WK * 64,
+      <<<lm_grid(tm * tn, WM * WN * WK * 64), WM * WN * WK * 64,
          kStages * ((BM + BN) * 128 + WM * WN * WK * 256), stream>>>(
           xc, xs, wc, ws, bias, y, m, n, nb, (int)tm, (int)tn);
   HIP_CHECK(hipGetLastError());
@@ -880,9 +876,9 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
               ((steps + kPrepareSteps - 1) / kPrepareSteps)
         : lay_blocks(m);
   // a token tile's offsets into the codes are 32 bits
-  if (x_blocks + w_blocks >= (int64_t)1 << 31 || nb * kMxBytes >= 1 << 23)
-    throw std::runtime_error("product too large for one launch");
-  const dim3 grid((unsigned)(x_blocks + w_blocks));
+  if (nb * kMxBytes >= 1 << 23)
+    throw std::runtime_error("rows too long for one launch");
+  const dim3 grid = lm_grid(x_blocks + w_blocks, kPrepareThreads);
   if (x)
     prepare_kernel<T, false><<<grid, kPrepareThreads, 0, stream>>>(
         (const char*)x, stride, nullptr, (uint32_t*)codes, xst, m, k,
@@ -937,7 +933,7 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
   if (!few(m, n, nb, x == nullptr))
     return run_tiles<T>(x, stride, xc, xs, wc, ws, bias, y, m, n, k, scratch,
                         stream);
-  const dim3 grid((unsigned)((n + 15) / 16));
+  const dim3 grid = lm_grid((n + 15) / 16, 512);
   const int64_t sums = 512 * sizeof(v4f);
   if (x && fuses(m, nb)) {
     few_kernel<T, false><<<grid, 512, std::max(few_lds(m, nb), sums), stream>>>(

@@ -123,12 +123,9 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(
 
 constexpr int kUnroll = 4;
 
-unsigned grid_of(int64_t groups) {
+dim3 grid_of(int64_t groups) {
   int64_t per = (int64_t)kThreads * kUnroll;
-  int64_t blocks = (groups + per - 1) / per;
-  if (blocks >= (int64_t)1 << 31)
-    throw std::runtime_error("too many elements for one launch");
-  return (unsigned)blocks;
+  return lm_grid((groups + per - 1) / per, kThreads);
 }
 
 }  // namespace
@@ -138,7 +135,7 @@ void launch_mx_quantize(LmType t, const void* x, int64_t stride,
                         int64_t k, hipStream_t stream) {
   const int64_t per_row = mx_blocks(k) * 4, groups = rows * per_row;
   const bool flat = k % kMxBlock == 0 && (stride == k || rows == 1);
-  const dim3 grid(grid_of(groups));
+  const dim3 grid = grid_of(groups);
   auto* x8 = (const char*)x;
   auto* c32 = (uint32_t*)codes;
   switch (t) {
@@ -163,7 +160,7 @@ void launch_mx_dequantize(LmType t, const uint8_t* codes,
                           int64_t k, hipStream_t stream) {
   const int64_t per_row = mx_blocks(k) * 4, groups = rows * per_row;
   const bool flat = k % kMxBlock == 0;
-  const dim3 grid(grid_of(groups));
+  const dim3 grid = grid_of(groups);
   auto* c32 = (const uint32_t*)codes;
   switch (t) {
     case LmType::F32:

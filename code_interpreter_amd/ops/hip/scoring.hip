@@ -972,6 +972,8 @@ constexpr int64_t kWant = 1024;
 constexpr int64_t kWantPlain = 512;
 constexpr int64_t kWhole = 384;
 constexpr int64_t kMaxSplits = 64;
+// of distillation: up to 4 rows a wave, where a launch less is the shorter way
+constexpr int64_t kOneBlock = 64;
 
 struct Plan {
   int unroll;        // words of 16 bytes a thread holds at a time
@@ -996,11 +998,6 @@ Plan plan_of(LmType t, int64_t rows, int64_t v, int top) {
   return p;
 }
 
-void check_grid(int64_t blocks) {
-  if (blocks >= (int64_t)1 << 31)
-    throw std::runtime_error("too many rows for one launch");
-}
-
 template <class F>
 void by_type(LmType t, F f) {
   switch (t) {
@@ -1022,11 +1019,11 @@ void run_score(LmType t, const void* x, int64_t stride, int64_t rows,
                int64_t v, const Plan& p, float c, bool top, bool direct,
                const End& end, Part* parts, uint64_t* keys,
                hipStream_t stream) {
-  check_grid(rows * p.splits);
+  const dim3 grid = lm_grid(rows * p.splits, kThreads);
   auto go = [&](auto type, auto unroll, auto with_top) {
     constexpr LmType T = decltype(type)::value;
     score_kernel<T, decltype(unroll)::value, decltype(with_top)::value, End>
-        <<<dim3((unsigned)(rows * p.splits)), kThreads, 0, stream>>>(
+        <<<grid, kThreads, 0, stream>>>(
             (const typename Elem<T>::type*)x, stride, v, (int)p.splits,
             p.part_len, c, direct, end, parts, keys);
   };
@@ -1049,6 +1046,7 @@ void run_score(LmType t, const void* x, int64_t stride, int64_t rows,
 
 int64_t score_workspace(LmType t, int64_t rows, int64_t v, int top) {
   Plan p = plan_of(t, rows, v, top);
+  if (p.splits == 1 && rows > kOneBlock) return 0;  // one block makes a row
   return rows * p.splits * (int64_t)(sizeof(Part) + 8 * (int64_t)top);
 }
 
@@ -1072,11 +1070,11 @@ void launch_token_logprobs(LmType t, const void* x, int64_t stride,
     constexpr LmType T = decltype(type)::value;
     auto* xt = (const typename Elem<T>::type*)x;
     if (top)
-      top_rows_kernel<T><<<dim3((unsigned)rows), kThreads, 0, stream>>>(
+      top_rows_kernel<T><<<lm_grid(rows, kThreads), kThreads, 0, stream>>>(
           xt, stride, v, c, parts, keys, (int)p.splits, e);
     else
       logprobs_rows_kernel<T>
-          <<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), kThreads, 0,
+          <<<lm_grid((rows + kWaves - 1) / kWaves, kThreads), kThreads, 0,
              stream>>>(xt, stride, rows, v, c, parts, (int)p.splits, e);
   });
 }
@@ -1092,9 +1090,8 @@ void launch_token_logprobs_bwd(LmType t, const void* x, int64_t stride,
     constexpr int U = 4;
     constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * U;
     int64_t chunks = (v + chunk - 1) / chunk;
-    check_grid(rows * chunks);
     logprobs_bwd_kernel<T, U>
-        <<<dim3((unsigned)(rows * chunks)), kThreads, 0, stream>>>(
+        <<<lm_grid(rows * chunks, kThreads), kThreads, 0, stream>>>(
             (const typename Elem<T>::type*)x, stride, v, (int)chunks, tokens,
             inv_t, inv_t * kLog2e, stats, g_lp, g_h,
             (typename Elem<T>::type*)dx);
@@ -1110,8 +1107,7 @@ void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
   const float c = inv_t * kLog2e;
   Part* parts = (Part*)ws;
   const DistillEnd e = {tt, teacher, ids, k, inv_t, row_loss, q, stats};
-  // up to 4 rows a wave a launch less is the shorter way
-  const bool whole = total && rows <= 64;
+  const bool whole = total && rows <= kOneBlock;
   const bool direct = p.splits == 1 && !whole;
   run_score(t, x, stride, rows, v, p, c, false, direct, e, parts, nullptr,
             stream);
@@ -1121,7 +1117,7 @@ void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
       auto go = [&](auto w) {
         constexpr bool W = decltype(w)::value;
         distill_rows_kernel<T, W>
-            <<<dim3(W ? 1 : (unsigned)((rows + kWaves - 1) / kWaves)),
+            <<<lm_grid(W ? 1 : (rows + kWaves - 1) / kWaves, kThreads),
                W ? 1024 : kThreads, 0, stream>>>(
                 (const typename Elem<T>::type*)x, stride, rows, v, c, parts,
                 (int)p.splits, e, mean, total, count);
@@ -1146,9 +1142,8 @@ void launch_distill_bwd(LmType t, const void* x, int64_t stride,
     constexpr int U = 4;
     constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * U;
     int64_t chunks = (v + chunk - 1) / chunk;
-    check_grid(rows * chunks);
     distill_bwd_kernel<T, U>
-        <<<dim3((unsigned)(rows * chunks)), kThreads, 0, stream>>>(
+        <<<lm_grid(rows * chunks, kThreads), kThreads, 0, stream>>>(
             (const typename Elem<T>::type*)x, stride, v, (int)chunks, ids, q,
             k, inv_t, inv_t * kLog2e, stats, grad, grad_stride, count,
             (typename Elem<T>::type*)dx);

@@ -150,7 +150,7 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
         return _cpu_distill(torch, logits, teacher_logits, ids, t, reduction)
     STATS["topk_distill_loss"] += 1
     return hiptorch.ensure_hiplm().distill(
-        logits, teacher_logits.contiguous(), ids, code, t_code, 1.0 / t, how)
+        logits, teacher_logits, ids, code, t_code, 1.0 / t, how)
 
 
 # ---------------------------------------------------------------------------

@@ -21,6 +21,8 @@ and raise where the extension is missing; CPU tensors are computed in plain
 torch, to the same codes. Products have no backward.
 """
 
+from operator import attrgetter
+
 import hiptorch
 
 BLOCK = 32
@@ -43,7 +45,12 @@ class MXFP4Tensor:
     be 0.
     """
 
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("_codes", "_scales", "_shape")
+
+    # not to be replaced one by one: the kernels rely on their fitting
+    codes = property(attrgetter("_codes"))
+    scales = property(attrgetter("_scales"))
+    shape = property(attrgetter("_shape"))
 
     def __init__(self, codes, scales, k: int):
         torch = hiptorch.lm_torch()
@@ -70,7 +77,7 @@ class MXFP4Tensor:
         self._set(codes, scales.contiguous(), torch.Size((*lead, k)))
 
     def _set(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, shape
+        self._codes, self._scales, self._shape = codes, scales, shape
         return self
 
     @property

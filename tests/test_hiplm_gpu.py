@@ -546,3 +546,41 @@ def test_far_offsets(lm):
         del dx, dz, z, r, loss
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_views_that_negate(lm):
+    """torch keeps a conjugate's imaginary part as a view with a mark; the
+    kernels get its values."""
+    torch, hiplm = lm
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.randn(3, 1000, 2, generator=g, device="cuda")
+    x = torch.view_as_complex(z).conj().imag
+    assert x.is_neg()
+    record = torch.view_as_complex(z).conj().imag[:, 5:9]
+    tokens = torch.tensor([1, 2, 3], device="cuda")
+    ids = torch.arange(12, device="cuda").reshape(3, 4)
+    results = []
+    for a, b in ((x, record), (x.resolve_neg(), record.resolve_neg())):
+        a = a.detach().requires_grad_(True)
+        r = hiplm.token_logprobs(a, tokens, top=3)
+        loss = hiplm.topk_distill_loss(a, b, ids)
+        weight = torch.view_as_complex(z[:, :1]).conj().imag[:, 0]
+        grad, = torch.autograd.grad([r.logprobs, loss], [a],
+                                    [weight, torch.ones((), device="cuda")])
+        results.append([*r, loss, grad])
+    for one, other in zip(*results):
+        assert torch.equal(one, other)
+
+
+def test_as_many_rows_as_a_launch_has(lm):
+    torch, hiplm = lm
+    rows = (1 << 24) - 1
+    x = torch.ones(rows + 1, 1, dtype=torch.bfloat16, device="cuda")
+    tokens = torch.zeros(rows + 1, dtype=torch.long, device="cuda")
+    few = x[:rows].requires_grad_(True)
+    r = hiplm.token_logprobs(few, tokens[:rows])
+    grad, = torch.autograd.grad(r.logprobs.sum(), [few])
+    for part in (r.logprobs, r.entropy, grad):
+        assert not part.any()
+    with pytest.raises(RuntimeError, match="too many rows"):
+        hiplm.token_logprobs(x, tokens)

@@ -2,6 +2,7 @@
 the format against its definition, the refusals, and the dispatch from
 torch's own linear."""
 
+import copy
 import sys
 from pathlib import Path
 
@@ -187,3 +188,12 @@ def test_parts_are_checked_and_shared():
     big[:, 5:37] = q.codes
     t = hipmx.MXFP4Tensor(big[:, 5:37], q.scales, 40)
     assert torch.equal(t.dequantize(), q.dequantize())
+
+
+def test_parts_are_not_replaced():
+    q = hipmx.quantize(torch.ones(2, 40))
+    for name in ("codes", "scales", "shape"):
+        with pytest.raises(AttributeError):
+            setattr(q, name, getattr(q, name))
+    again = copy.deepcopy(q)
+    assert torch.equal(again.codes, q.codes) and again.shape == q.shape

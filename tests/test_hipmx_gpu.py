@@ -368,3 +368,22 @@ def test_long_rows(mx):
     assert torch.equal(hipmx.linear(x, w).double(), want)
     assert torch.equal(hipmx.linear(x.repeat(20, 1), w).double(),
                        want.repeat(20, 1))
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_views_that_negate(mx, m):
+    """torch keeps a conjugate's imaginary part as a view with a mark; the
+    kernels get its values."""
+    torch, hipmx = mx
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.randn(m, 100, 2, generator=g, device="cuda")
+    x = torch.view_as_complex(z).conj().imag
+    assert x.is_neg()
+    q, want = hipmx.quantize(x), hipmx.quantize(x.resolve_neg())
+    assert torch.equal(q.codes, want.codes)
+    assert torch.equal(q.scales, want.scales)
+    w = hipmx.quantize(torch.randn(m, 100, generator=g, device="cuda"))
+    bias = x[:, 0]
+    assert bias.is_neg()
+    assert torch.equal(hipmx.linear(x, w, bias),
+                       hipmx.linear(x.resolve_neg(), w, bias.resolve_neg()))
