@@ -347,8 +347,13 @@ PyObject* tuple(std::initializer_list<Tensor> tensors) {
   return out.release();
 }
 
+bool has_tangent(const Tensor& t) {
+  return t.defined() && t._fw_grad(0).defined();
+}
+
+// also with a forward-mode tangent, which torch then refuses
 bool needs_grad(const Tensor& t) {
-  return at::GradMode::is_enabled() && t.requires_grad();
+  return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t);
 }
 
 PyObject* py_is_available(PyObject*, PyObject*) {
@@ -395,6 +400,8 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor &wc = a.tensor(), &ws = a.tensor();
   const Tensor bias = a.tensor_or_none();
   const int64_t k = a.integer(1), code = a.type();
+  TORCH_CHECK(!has_tangent(x) && !has_tangent(bias),
+              "hipmx.linear has no forward-mode derivative");
   Tensor y;
   {
     pybind11::gil_scoped_release no_gil;

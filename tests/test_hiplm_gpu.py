@@ -584,3 +584,20 @@ def test_as_many_rows_as_a_launch_has(lm):
         assert not part.any()
     with pytest.raises(RuntimeError, match="too many rows"):
         hiplm.token_logprobs(x, tokens)
+
+
+def test_forward_mode_is_refused(lm):
+    torch, hiplm = lm
+    import hipmx
+    from torch.autograd import forward_ad
+
+    x = torch.randn(2, 64, device="cuda")
+    ids = torch.zeros(2, 1, dtype=torch.long, device="cuda")
+    w = hipmx.quantize(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: hiplm.token_logprobs(dual, ids[:, 0]),
+                     lambda: hiplm.topk_distill_loss(dual, x[:, :1], ids),
+                     lambda: hipmx.linear(dual, w)):
+            with pytest.raises(RuntimeError, match="jvp|forward-mode"):
+                call()
