@@ -188,33 +188,62 @@ __device__ __forceinline__ Triple join_wave(Triple a, float c) {
   return {a.m, wave_sum(a.s), wave_sum(a.u)};
 }
 
-// order-preserving bits of a value above, the complement of its index
-// below: a larger key is a better alternative, of equal values the earlier.
-// 0 stands for none. Both zeros are one value.
+// bits that order as the values do. Both zeros are one value.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
+}
+
+// a value's order above, the complement of its index below: a larger key is a
+// better alternative, of equal values the earlier. 0 stands for none.
 __device__ __forceinline__ uint64_t make_key(float x, uint32_t index) {
-  uint32_t b = __float_as_uint(x + 0.f);
-  b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (uint64_t)b << 32 | (uint32_t)~index;
+  return (uint64_t)order_of(x) << 32 | (uint32_t)~index;
 }
 __device__ __forceinline__ float key_value(uint64_t key) {
-  uint32_t b = (uint32_t)(key >> 32);
-  return __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
+  return value_of((uint32_t)(key >> 32));
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) {
   return ~(uint32_t)key;
 }
 
+// The r-th largest of the kMany numbers that each lane of a wave holds, 0 if
+// there are not so many, from the top kBits of them (a lower bound of it, for
+// numbers that have more): each bit is set where r of them stay at or above.
+template <int kBits, int kMany>
+__device__ __forceinline__ uint32_t rth_of_wave(const uint32_t (&x)[kMany],
+                                                int r) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int bit = 31; bit > 31 - kBits; bit--) {
+    const uint32_t with = found | 1u << bit;
+    int there = 0;
+#pragma unroll
+    for (int i = 0; i < kMany; i++) there += __popcll(__ballot(x[i] >= with));
+    if (there >= r) found = with;
+  }
+  return found;
+}
+
+// of a value's order in a key: all that a 16-bit type has, or all
+template <LmType T>
+constexpr int kOrderBits = T == LmType::F32 ? 32 : 20;
+
 // ---------------------------------------------------------------------------
 // alternatives
 // ---------------------------------------------------------------------------
-constexpr int kCap = 2048;  // candidates that are held at a time
+// candidates that are held at a time: the best so far and those of a word a
+// thread, at least
+constexpr int kCap = kMaxTop + kThreads * 8;
+constexpr int kFew = 256;  // that are ranked as they are
 
 struct TopShared {
   // the best so far, then candidates; a pair more than there can be
   alignas(16) uint64_t keys[kCap + 2];
   uint64_t best[kMaxTop];
-  uint64_t wave_key[kWaves];
-  float bound[kWaves];
+  uint64_t most[kThreads];  // the threads' largest
   float least;    // a candidate is larger than this
   int count;      // entries of keys
   int flag[3];    // whether a chunk has candidates, by its number mod 3
@@ -255,12 +284,14 @@ __device__ int rank_keys(TopShared& sh, int n, int k) {
 // when there are 3 k + 32 or more, or at the end: ranking raises the bar for
 // what follows, and costs the square of their number.
 //
-// For the first chunk, and where candidates do not fit: in each of the 4
-// waves ceil(k / 4) threads hold an element that is not below the
-// ceil(k / 4)-th largest of the threads' own maxima. So the least of the four
-// is a lower bound of the chunk's k-th largest element. Not many elements
-// pass it but where many are equal. Where the candidates still do not fit,
-// the k best are taken one by one.
+// For the first chunk, and where candidates are many: k threads hold an
+// element that is not below the k-th largest of the threads' own maxima, which
+// so is a lower bound of the chunk's k-th largest element. Not many elements
+// pass it but where many are equal, or few threads have one at all. Candidates
+// that still are many are spread over all threads, whose largest give a bound
+// once more, by index among equal ones. Those that do not fit come word by
+// word: 64 rows of 131072 equal bf16 logits with 20 alternatives take 32 us, 18
+// where they differ.
 template <LmType T, int U>
 struct Top {
   using E = Elem<T>;
@@ -284,33 +315,27 @@ struct Top {
 
   // Elements larger than `least` and not less than `bound` to the keys. Words
   // in which no lane has one, most of them, are passed over as a whole.
-  __device__ void append(const u32x4* w, const float* word_max, int64_t base,
+  __device__ void append(const u32x4& w, float word_max, int64_t at,
                          float bound) {
-    uint32_t which = 0;  // of the thread's elements
+    if (!__any((word_max > least) & (word_max >= bound))) return;
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      if (!__any((word_max[i] > least) & (word_max[i] >= bound))) continue;
-#pragma unroll
-      for (int j = 0; j < E::kVec; j++) {
-        const float x = E::get(w[i], j);
-        which |= (uint32_t)((x > least) & (x >= bound)) << (i * E::kVec + j);
-      }
+    for (int j = 0; j < E::kVec; j++) {
+      const float x = E::get(w, j);
+      if (!((x > least) & (x >= bound))) continue;
+      const int place = atomicAdd(&sh.count, 1);
+      if (place < kCap) sh.keys[place] = make_key(x, (uint32_t)(at + j));
     }
-    if (!which) return;
-    int at = atomicAdd(&sh.count, __popc(which));
+  }
+
+  __device__ int64_t place_of(int64_t base, int i) const {
+    return base + (int64_t)(i * kThreads + threadIdx.x) * E::kVec;
+  }
+
+  __device__ void append_all(const u32x4* w, const float* word_max,
+                             int64_t base, float bound) {
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      if (!(which >> (i * E::kVec) & ((1u << E::kVec) - 1))) continue;
-#pragma unroll
-      for (int j = 0; j < E::kVec; j++) {
-        if (!(which >> (i * E::kVec + j) & 1)) continue;
-        if (at < kCap)
-          sh.keys[at] = make_key(
-              E::get(w[i], j),
-              (uint32_t)(base + (i * kThreads + threadIdx.x) * E::kVec + j));
-        at++;
-      }
-    }
+    for (int i = 0; i < U; i++)
+      append(w[i], word_max[i], place_of(base, i), bound);
   }
 
   __device__ void merge(int n) {
@@ -318,105 +343,114 @@ struct Top {
     least = sh.least;
   }
 
-  // The ceil(k / 4)-th largest of a wave's lanes' maxima, by the bits of its
-  // order from the top: each is set where enough lanes stay at or above it.
-  // kBits of them give 16-bit types exactly, and a lower bound for the rest.
-  __device__ float bound_of_wave(float lane_max) const {
-    constexpr int kBits = 20;
-    const uint32_t order = (uint32_t)(make_key(lane_max, 0) >> 32);
-    const int r = (k + kWaves - 1) / kWaves;
-    uint32_t found = 0;
+  // The k-th largest of the threads' numbers, from the top bits of them.
+  __device__ uint32_t kth_of_block(uint32_t mine) {
+    uint32_t* const order = (uint32_t*)sh.most;
+    order[threadIdx.x] = mine;
+    __syncthreads();
+    uint32_t all[kWaves];
 #pragma unroll
-    for (int bit = 31; bit > 31 - kBits; bit--) {
-      const uint32_t with = found | 1u << bit;
-      if (__popcll(__ballot(order >= with)) >= r) found = with;
+    for (int i = 0; i < kWaves; i++)
+      all[i] = order[i * 64 + (threadIdx.x & 63)];
+    return rth_of_wave<20>(all, k);
+  }
+
+  // n > kFew keys to those that are not below the k-th largest of the threads'
+  // largest keys
+  __device__ int thin(int n) {
+    constexpr int kMine = (kCap + kThreads - 1) / kThreads;
+    const int tid = threadIdx.x;
+    uint64_t mine[kMine], most = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+      mine[i] = tid + i * kThreads < n ? sh.keys[tid + i * kThreads] : 0;
+      most = max(most, mine[i]);
     }
-    // no number's order is below that of -inf
-    return key_value((uint64_t)max(found, 0x007FFFFFu) << 32);
+    sh.most[tid] = most;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    uint32_t all[kWaves], low[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) {
+      const uint64_t key = sh.most[i * 64 + (tid & 63)];
+      all[i] = (uint32_t)(key >> 32);
+      low[i] = (uint32_t)key;
+    }
+    const uint32_t found = rth_of_wave<32>(all, k);
+    int more = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) {
+      more += __popcll(__ballot(all[i] > found));
+      if (all[i] != found) low[i] = 0;
+    }
+    const uint64_t bound =
+        (uint64_t)found << 32 | rth_of_wave<32>(low, k - more);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; i++)
+      if (mine[i] >= max(bound, (uint64_t)1))
+        sh.keys[atomicAdd(&sh.count, 1)] = mine[i];
+    __syncthreads();
+    return sh.count;
   }
 
   __device__ void take_bounded(const u32x4* w, const float* word_max,
                                int64_t base, float thread_max) {
-    const int tid = threadIdx.x;
-    // NaN's order would be the largest of all
-    const float mine =
-        bound_of_wave(thread_max == thread_max ? thread_max : -INFINITY);
-    if ((tid & 63) == 0) sh.bound[tid >> 6] = mine;
-    __syncthreads();
-    float bound = sh.bound[0];
-#pragma unroll
-    for (int i = 1; i < kWaves; i++) bound = fminf(bound, sh.bound[i]);
-    append(w, word_max, base, bound);
+    // NaN's order would be the largest of all; no number's is below -inf's
+    const uint32_t none = order_of(-INFINITY);
+    const float bound = value_of(max(
+        kth_of_block(thread_max == thread_max ? order_of(thread_max) : none),
+        none));
+    append_all(w, word_max, base, bound);
     __syncthreads();
     int n = sh.count;
+    if (n <= kCap) return settle(n);
+    // Word by word, seldom, and so from memory: held in registers until here
+    // the chunk would cost all chunks theirs.
     __syncthreads();
-    if (n > kCap) {
-      if (tid == 0) sh.count = have;
+    if (threadIdx.x == 0) sh.count = have;
+#pragma unroll 1
+    for (int i = 0; i < U; i++) {
+      const int64_t at = place_of(base, i);
+      const u32x4 word = load_vec<T>(src, at, end);
       __syncthreads();
-      n = one_by_one(base);
+      append(word, INFINITY, at, bound);
+      __syncthreads();
+      settle(sh.count);
     }
-    merge(n);
   }
 
-  // Seldom used, and so from memory: held against the chunk in registers its
-  // keys would cost all chunks theirs.
-  __device__ int one_by_one(int64_t base) {
-    const int tid = threadIdx.x;
-    uint64_t last = ~0ull;
-    for (int r = 0; r < k; r++) {
-      uint64_t mine = 0;
-#pragma unroll 1
-      for (int i = 0; i < U; i++) {
-        const int64_t at = base + (int64_t)(i * kThreads + tid) * E::kVec;
-        const u32x4 w = load_vec<T>(src, at, end);
-#pragma unroll
-        for (int j = 0; j < E::kVec; j++) {
-          const float x = E::get(w, j);
-          const uint64_t key = make_key(x, (uint32_t)(at + j));
-          if (x > least && key < last && key > mine) mine = key;
-        }
-      }
-#pragma unroll
-      for (int d = 32; d; d >>= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)mine, d);
-        mine = o > mine ? o : mine;
-      }
-      if ((tid & 63) == 0) sh.wave_key[tid >> 6] = mine;
-      __syncthreads();
-      uint64_t best = 0;
-      for (int j = 0; j < kWaves; j++)
-        best = sh.wave_key[j] > best ? sh.wave_key[j] : best;
-      __syncthreads();
-      if (!best) break;
-      if (tid == 0) sh.keys[sh.count++] = best;
-      last = best;
-    }
-    __syncthreads();
-    return sh.count;
+  // n keys to the best
+  __device__ void settle(int n) {
+    if (n > kFew) n = thin(n);
+    merge(n);
   }
 
   __device__ void take(const u32x4* w, const float* word_max, int64_t base,
                        float thread_max) {
     const int now = chunk % 3;
-    chunk++;
-    if (__any(thread_max > least) && (threadIdx.x & 63) == 0) sh.flag[now] = 1;
-    __syncthreads();
-    // the flag of the chunk after the next: it is set behind another barrier
-    if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
-    if (!sh.flag[now]) return;
-    if (have < k) return take_bounded(w, word_max, base, thread_max);
-    append(w, word_max, base, -INFINITY);
-    __syncthreads();
-    const int n = sh.count;
-    if (n < 3 * k + 32) {
-      count = n;
-      return;
+    if (chunk++) {
+      if (__any(thread_max > least) && (threadIdx.x & 63) == 0)
+        sh.flag[now] = 1;
+      __syncthreads();
+      // the flag of the chunk after the next: it is set behind another barrier
+      if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
+      if (!sh.flag[now]) return;
+      if (have == k) {
+        append_all(w, word_max, base, -INFINITY);
+        __syncthreads();
+        const int n = sh.count;
+        if (n < 3 * k + 32) {
+          count = n;
+          return;
+        }
+        __syncthreads();
+        if (n <= 2 * kFew) return merge(n);
+        if (threadIdx.x == 0) sh.count = count;
+        __syncthreads();
+        merge(count);  // what was there before this chunk
+      }
     }
-    __syncthreads();
-    if (n <= kCap) return merge(n);
-    if (threadIdx.x == 0) sh.count = count;
-    __syncthreads();
-    merge(count);  // what was there before this chunk
     take_bounded(w, word_max, base, thread_max);
   }
 
@@ -449,16 +483,28 @@ struct DistillEnd {
   RowStats* stats;
 };
 
+// A row's token, and its logit: read before the row's sums are joined, so
+// that the two loads, one upon the other, are over by then.
+struct Token {
+  float x;
+  bool ignored, outside;
+};
+
+template <LmType T>
+__device__ Token token_of(int64_t id, const typename Elem<T>::type* src,
+                          int64_t v, const LogprobsEnd& e) {
+  const bool ignored = id == e.ignore;
+  const bool outside = !ignored && (id < 0 || id >= v);
+  return {ignored || outside ? 0.f : Elem<T>::load(src + id), ignored,
+          outside};
+}
+
 // a row's log probability, entropy and what its backward needs, by one
 // thread
-template <LmType T>
-__device__ void write_row(int64_t row, const typename Elem<T>::type* x,
-                          int64_t stride, int64_t v, const Triple& t,
+__device__ void write_row(int64_t row, const Triple& t, const Token& token,
                           const LogprobsEnd& e) {
-  const int64_t token = e.tokens[row];
   const float log2_sum = log2f(t.s);
-  const bool ignored = token == e.ignore;
-  const bool outside = !ignored && (token < 0 || token >= v);
+  const bool ignored = token.ignored, outside = token.outside;
   const bool empty = t.m == -INFINITY && t.s == 0.f;
   float lp, h;
   if (ignored) {
@@ -469,8 +515,7 @@ __device__ void write_row(int64_t row, const typename Elem<T>::type* x,
     lp = -INFINITY;
     h = 0.f;
   } else {
-    const float xt = Elem<T>::load(x + row * stride + token);
-    lp = (xt - t.m) * e.inv_t - log2_sum * kLn2;
+    lp = (token.x - t.m) * e.inv_t - log2_sum * kLn2;
     h = (log2_sum - t.u / t.s) * kLn2;
     if (!(t.s == t.s)) lp = NAN;
   }
@@ -483,8 +528,9 @@ __device__ void write_row(int64_t row, const typename Elem<T>::type* x,
 
 // an alternative of a row; key 0 stands for none
 __device__ void write_top(int64_t row, int place, uint64_t key,
-                          const Triple& t, const LogprobsEnd& e) {
-  if (e.tokens[row] == e.ignore) key = 0;
+                          const Triple& t, const Token& token,
+                          const LogprobsEnd& e) {
+  if (token.ignored) key = 0;
   const int64_t at = row * e.top + place;
   e.top_lp[at] =
       key ? (key_value(key) - t.m) * e.inv_t - log2f(t.s) * kLn2 : -INFINITY;
@@ -667,10 +713,13 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
     if (tid < 64)
       distill_row<T>(row, x, stride, v, end_of_row, c, [&] { return t; });
   } else {
-    if (tid == 0) write_row<T>(row, x, stride, v, t, end_of_row);
+    const Token token =
+        token_of<T>(end_of_row.tokens[row], src, v, end_of_row);
+    if (tid == 0) write_row(row, t, token, end_of_row);
     if constexpr (kTop) {
       if (tid < k)
-        write_top(row, tid, tid < best.have ? sh.keys[tid] : 0, t, end_of_row);
+        write_top(row, tid, tid < best.have ? sh.keys[tid] : 0, t, token,
+                  end_of_row);
     }
   }
 }
@@ -694,25 +743,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows_kernel(
     int splits, LogprobsEnd e) {
   int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= rows) return;
+  const Token token = token_of<T>(e.tokens[row], x + row * stride, v, e);
   const Triple t = join_parts(parts + row * splits, splits, c);
-  if ((threadIdx.x & 63) == 0) write_row<T>(row, x, stride, v, t, e);
+  if ((threadIdx.x & 63) == 0) write_row(row, t, token, e);
 }
 
-// the r-th largest of the lanes' keys, 0 counting as none
-__device__ uint64_t rth_of_wave(uint64_t key, int lanes, int r) {
-  int not_less = 0;
-  for (int j = 0; j < lanes; j++) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)key, j);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(key >> 32), j);
-    not_less += ((uint64_t)hi << 32 | lo) >= key;
+// The r-th largest of the lanes' keys, or a lower bound of it, 0 counting as
+// none. Keys of equal values are told apart by their indexes only from kTies
+// too many on: a few equal ones are common in 16 bits, and cost less than this.
+constexpr int kTies = 8;
+
+template <LmType T>
+__device__ uint64_t rth_key(uint64_t key, int r) {
+  const uint32_t order = (uint32_t)(key >> 32);
+  const uint32_t found = rth_of_wave<kOrderBits<T>>({order}, r);
+  uint32_t below = 0;
+  if (__popcll(__ballot(order >= found)) >= r + kTies && found) {
+    const int more = __popcll(__ballot(order > found));
+    below = rth_of_wave<32>({order == found ? (uint32_t)key : 0u}, r - more);
   }
-  unsigned long long best = not_less >= r ? key : 0;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const unsigned long long o = __shfl_xor(best, d);
-    best = o > best ? o : best;
-  }
-  return best;
+  return (uint64_t)found << 32 | below;
 }
 
 // A block a row, with alternatives: joins the parts' sorted lists. Where r
@@ -733,15 +783,16 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
   const int tid = threadIdx.x, lane = tid & 63, k = e.top;
   const uint64_t* src = part_keys + row * splits * k;
   const int all = splits * k;
+  const int64_t id = e.tokens[row];
+  // splits is 64 at most: a list a lane
+  const int place = min(k, (k + splits - 1) / splits << (tid >> 6));
+  const uint64_t listed = lane < splits ? src[lane * k + place - 1] : 0;
   uint64_t mine[kMine];
 #pragma unroll
   for (int i = 0; i < kMine; i++)
     mine[i] = tid + i * kThreads < all ? src[tid + i * kThreads] : 0;
-  // splits is 64 at most: a list a lane
-  const int place = min(k, (k + splits - 1) / splits << (tid >> 6));
-  const uint64_t bound_of_wave =
-      rth_of_wave(lane < splits ? src[lane * k + place - 1] : 0, splits,
-                  (k + place - 1) / place);
+  const uint64_t bound_of_wave = rth_key<T>(listed, (k + place - 1) / place);
+  const Token token = token_of<T>(id, x + row * stride, v, e);
   const Triple t = join_parts(parts + row * splits, splits, c);
   if (lane == 0) bounds[tid >> 6] = bound_of_wave;
   if (tid == 0) count = 0;
@@ -762,9 +813,9 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
     for (int j = 0; j < n; j++) rank += keys[j] > key;
     if (rank < k) best[rank] = key;
   }
-  if (tid == 0) write_row<T>(row, x, stride, v, t, e);
+  if (tid == 0) write_row(row, t, token, e);
   __syncthreads();
-  if (tid < k) write_top(row, tid, best[tid], t, e);
+  if (tid < k) write_top(row, tid, best[tid], t, token, e);
 }
 
 // dx_j = -p_j (a + b ln p_j) at every j, and g_lp / T more at the token,

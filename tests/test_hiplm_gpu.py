@@ -176,6 +176,42 @@ def test_top_of_hard_rows(lm):
 
 
 @pytest.mark.parametrize("rows", [1, 500])
+@pytest.mark.parametrize("v", [300, 1000, 2100, 40007])
+def test_top_of_narrow_rows(lm, rows, v):
+    """What is left of a row stands where few of a block's threads see it, or
+    is so close that the candidates are many: rows shorter than a chunk, a
+    window in a masked row, falling and rising values, values that differ in
+    the last bits of a float32, rows of one value."""
+    torch, hiplm = lm
+    g = torch.Generator().manual_seed(v)
+    x = torch.full((7, v), -math.inf)
+    x[0] = torch.randn(v, generator=g)
+    x[1, v // 3: v // 3 + 1300] = torch.randn(
+        len(range(v)[v // 3: v // 3 + 1300]), generator=g)
+    x[2, ::97] = 1.0
+    x[3] = torch.arange(v) / 64.0
+    x[4] = -torch.arange(v) / 64.0
+    x[5] = 1 + torch.rand(v, generator=g) * 2.0 ** -13
+    x[6] = 0
+    tokens = torch.zeros(rows, dtype=torch.long, device="cuda")
+    for dtype in DTYPES:
+        few = x.to(getattr(torch, dtype))
+        many = few.repeat(-(-rows // 7), 1)[:max(rows, 7)]
+        values, ids = few.float().sort(dim=-1, descending=True, stable=True)
+        ids[values == -math.inf] = -1
+        for top in (1, 13, 64, 128):
+            if rows == 1:
+                got = torch.cat([hiplm.token_logprobs(
+                    row[None].cuda(), tokens, top=top).top_tokens
+                    for row in many])
+            else:
+                got = hiplm.token_logprobs(many.cuda(), tokens,
+                                           top=top).top_tokens
+            want = ids[:, :top].repeat(-(-rows // 7), 1)[:max(rows, 7)]
+            assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [1, 500])
 def test_top_of_rows_with_nan(lm, rows):
     """Numbers are chosen from what is one, also where some of a block's
     threads see nothing but NaN; all log probabilities of the row are NaN."""
