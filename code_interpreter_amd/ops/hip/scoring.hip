@@ -238,6 +238,7 @@ constexpr int kOrderBits = T == LmType::F32 ? 32 : 20;
 // thread, at least
 constexpr int kCap = kMaxTop + kThreads * 8;
 constexpr int kFew = 256;  // that are ranked as they are
+constexpr int kPending = 4;  // chunks between two looks at their number
 
 struct TopShared {
   // the best so far, then candidates; a pair more than there can be
@@ -249,22 +250,28 @@ struct TopShared {
   int flag[3];    // whether a chunk has candidates, by its number mod 3
 };
 
-// keys[0 .. n) -> the k best, sorted, at keys[0 ..), by counting for each
-// key how many are larger: keys are all different. Returns their number.
-__device__ int rank_keys(TopShared& sh, int n, int k) {
+// The k best of keys[0 .. n), which are all different, to best, sorted: each
+// key's place is the number of larger ones. keys[n] is written, and keys are
+// 16-byte aligned.
+__device__ void rank_keys(uint64_t* keys, int n, int k, uint64_t* best) {
   using Pair = uint64_t __attribute__((ext_vector_type(2)));
-  if (threadIdx.x == 0) sh.keys[n] = 0;  // the last pair's other half
+  if (threadIdx.x == 0) keys[n] = 0;  // the last pair's other half
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t key = sh.keys[i];
+    const uint64_t key = keys[i];
     int rank = 0;
 #pragma unroll 4
     for (int j = 0; j < n; j += 2) {
-      const Pair o = *(const Pair*)&sh.keys[j];
+      const Pair o = *(const Pair*)&keys[j];
       rank += (o[0] > key) + (o[1] > key);
     }
-    if (rank < k) sh.best[rank] = key;
+    if (rank < k) best[rank] = key;
   }
+}
+
+// keys[0 .. n) -> the k best, sorted, at keys[0 ..). Returns their number.
+__device__ int keep_best(TopShared& sh, int n, int k) {
+  rank_keys(sh.keys, n, k, sh.best);
   __syncthreads();
   const int have = min(n, k);
   for (int i = threadIdx.x; i < have; i += kThreads) sh.keys[i] = sh.best[i];
@@ -280,9 +287,10 @@ __device__ int rank_keys(TopShared& sh, int n, int k) {
 // registers: words w[0 .. U) of each thread, thread t's word i at element
 // base + (i * 256 + t) * kVec. Chunks come in the order of their indexes, so
 // that an element must be larger than the last of the k best so far to
-// displace it; few of a later chunk are. Candidates are gathered and ranked
-// when there are 3 k + 32 or more, or at the end: ranking raises the bar for
-// what follows, and costs the square of their number.
+// displace it; few of a later chunk are. Candidates are gathered, for kPending
+// chunks without a barrier, and ranked when there are 2 k + 32 or more, or at
+// the end: ranking raises the bar for what follows, and costs the square of
+// their number (2048 x 131072 bf16 with 64: 152 us, 161 from 3 k + 32 on).
 //
 // For the first chunk, and where candidates are many: k threads hold an
 // element that is not below the k-th largest of the threads' own maxima, which
@@ -300,11 +308,12 @@ struct Top {
   const typename E::type* const src;  // the row, and where its part ends
   const int64_t end;
   int have = 0, count = 0, chunk = 0;  // equal in all threads
+  int64_t since;  // what stands before it is settled, or in count
   float least = -INFINITY;
 
   __device__ Top(TopShared& sh, int k, const typename E::type* src,
-                 int64_t end)
-      : sh(sh), k(k), src(src), end(end) {
+                 int64_t begin, int64_t end)
+      : sh(sh), k(k), src(src), end(end), since(begin) {
     if (threadIdx.x == 0) {
       sh.count = 0;
       sh.least = least;
@@ -339,7 +348,7 @@ struct Top {
   }
 
   __device__ void merge(int n) {
-    have = count = rank_keys(sh, n, k);
+    have = count = keep_best(sh, n, k);
     least = sh.least;
   }
 
@@ -394,69 +403,68 @@ struct Top {
     return sh.count;
   }
 
-  __device__ void take_bounded(const u32x4* w, const float* word_max,
-                               int64_t base, float thread_max) {
-    // NaN's order would be the largest of all; no number's is below -inf's
-    const uint32_t none = order_of(-INFINITY);
-    const float bound = value_of(max(
-        kth_of_block(thread_max == thread_max ? order_of(thread_max) : none),
-        none));
-    append_all(w, word_max, base, bound);
-    __syncthreads();
-    int n = sh.count;
-    if (n <= kCap) return settle(n);
-    // Word by word, seldom, and so from memory: held in registers until here
-    // the chunk would cost all chunks theirs.
-    __syncthreads();
-    if (threadIdx.x == 0) sh.count = have;
-#pragma unroll 1
-    for (int i = 0; i < U; i++) {
-      const int64_t at = place_of(base, i);
-      const u32x4 word = load_vec<T>(src, at, end);
-      __syncthreads();
-      append(word, INFINITY, at, bound);
-      __syncthreads();
-      settle(sh.count);
-    }
-  }
-
   // n keys to the best
   __device__ void settle(int n) {
     if (n > kFew) n = thin(n);
     merge(n);
   }
 
-  __device__ void take(const u32x4* w, const float* word_max, int64_t base,
-                       float thread_max) {
-    const int now = chunk % 3;
-    if (chunk++) {
-      if (__any(thread_max > least) && (threadIdx.x & 63) == 0)
-        sh.flag[now] = 1;
+  // What the chunks before `upto` have left. Where candidates did not fit,
+  // what is not settled comes once more, from memory: held in registers until
+  // here the chunks would cost all rows theirs.
+  __device__ void review(int64_t upto, float bound, bool always) {
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    if (n > kCap) {
+      if (threadIdx.x == 0) sh.count = count;
       __syncthreads();
-      // the flag of the chunk after the next: it is set behind another barrier
-      if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
-      if (!sh.flag[now]) return;
-      if (have == k) {
-        append_all(w, word_max, base, -INFINITY);
+      if (count > have) merge(count);
+#pragma unroll 1
+      for (; since < upto; since += kThreads * E::kVec) {
+        const int64_t at = since + threadIdx.x * E::kVec;
+        const u32x4 word = load_vec<T>(src, at, end);
+        append(word, INFINITY, at, bound);
         __syncthreads();
-        const int n = sh.count;
-        if (n < 3 * k + 32) {
-          count = n;
-          return;
-        }
-        __syncthreads();
-        if (n <= 2 * kFew) return merge(n);
-        if (threadIdx.x == 0) sh.count = count;
-        __syncthreads();
-        merge(count);  // what was there before this chunk
+        settle(sh.count);
       }
+    } else if (n >= 2 * k + 32 || (always && n > have)) {
+      settle(n);
+    } else {
+      count = n;
     }
-    take_bounded(w, word_max, base, thread_max);
+    since = upto;
   }
 
-  __device__ void finish() {
-    __syncthreads();
-    if (count > have) merge(count);
+  __device__ void take(const u32x4* w, const float* word_max, int64_t base,
+                       float thread_max, bool last) {
+    const int64_t upto = base + kThreads * E::kVec * U;
+    const int now = chunk % 3;
+    float bound = -INFINITY;
+    chunk++;
+    if (have < k) {
+      if (now || chunk > 3) {
+        if (__any(thread_max > least) && (threadIdx.x & 63) == 0)
+          sh.flag[now] = 1;
+        __syncthreads();
+        // of the chunk after the next: it is set behind another barrier
+        if (threadIdx.x == 0) sh.flag[(now + 2) % 3] = 0;
+        if (!sh.flag[now]) {
+          since = upto;
+          return;
+        }
+      }
+      // NaN's order would be the largest of all; no number's is below -inf's
+      const uint32_t none = order_of(-INFINITY);
+      bound = value_of(max(
+          kth_of_block(thread_max == thread_max ? order_of(thread_max) : none),
+          none));
+      append_all(w, word_max, base, bound);
+      last = true;
+    } else {
+      append_all(w, word_max, base, bound);
+    }
+    if (last || chunk < 4 || chunk % kPending == 0) review(upto, bound, last);
   }
 };
 
@@ -620,7 +628,7 @@ __device__ RowLoss distill_row(
 // one pass over a row, or over one of `splits` parts of it
 // ---------------------------------------------------------------------------
 struct NoTop {
-  __device__ NoTop(int&, int, const void*, int64_t) {}
+  __device__ NoTop(int&, int, const void*, int64_t, int64_t) {}
 };
 
 struct Part {
@@ -649,8 +657,8 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
   int k = 0;
   if constexpr (kTop) k = end_of_row.top;
 
-  typename std::conditional<kTop, Top<T, U>, NoTop>::type best(sh, k, src,
-                                                                  end);
+  typename std::conditional<kTop, Top<T, U>, NoTop>::type best(
+      sh, k, src, begin, end);
 
   Triple t = {-INFINITY, 0.f, 0.f};
   u32x4 next[U];
@@ -691,15 +699,13 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
       }
     t.s += s;
     t.u += u;
-    if constexpr (kTop) best.take(w, word_max, base, chunk_max);
+    if constexpr (kTop)
+      best.take(w, word_max, base, chunk_max, base + kChunk >= end);
   }
 
   t = join_wave(t, c);
   if ((tid & 63) == 0) wave_t[tid >> 6] = t;
-  if constexpr (kTop)
-    best.finish();
-  else
-    __syncthreads();
+  __syncthreads();
   t = wave_t[0];
   for (int i = 1; i < kWaves; i++) t = join(t, wave_t[i], c);
   if (!direct) {
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
     float c, const Part* __restrict__ parts,
     const uint64_t* __restrict__ part_keys, int splits, LogprobsEnd e) {
   constexpr int kMine = kMaxKeys / kThreads;
-  __shared__ uint64_t keys[kMaxKeys];
+  __shared__ alignas(16) uint64_t keys[kMaxKeys + 2];
   __shared__ uint64_t best[kMaxTop], bounds[kWaves];
   __shared__ int count;
   const int64_t row = blockIdx.x;
@@ -806,13 +812,7 @@ __global__ __launch_bounds__(kThreads) void top_rows_kernel(
     if (mine[i] >= bound) keys[atomicAdd(&count, 1)] = mine[i];
   __syncthreads();
   const int n = count;
-  for (int i = tid; i < n; i += kThreads) {
-    const uint64_t key = keys[i];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; j++) rank += keys[j] > key;
-    if (rank < k) best[rank] = key;
-  }
+  rank_keys(keys, n, k, best);
   if (tid == 0) write_row(row, t, token, e);
   __syncthreads();
   if (tid < k) write_top(row, tid, best[tid], t, token, e);
@@ -1015,13 +1015,21 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
 // ---------------------------------------------------------------------------
 // Parts of a row. Rows are split into parts of whole chunks until there are
 // kWant blocks (kWantPlain without alternatives, which leave less to do
-// between the loads); kWhole rows and more are not, which saves the launch
-// that joins the parts. In us for 512 and 1024 blocks: 509 x 50001 f32
-// without alternatives 20.9, 23.7, with 5 of them 30.4, 31.4; 256 x 131072
-// bf16 17.7, 18.8 and 37.2, 31.0.
+// between the loads). From kWhole rows on they are not, nor are short rows: a
+// row by one block saves the launch that joins the parts, 2 us of it, 4 with
+// alternatives. In us, of rows x row, split and whole:
+//                     no alternatives    1            20            64
+//    1 x  8000 f32     5.1,  3.8     9.2,  6.9   10.4,  9.6   11.9, 12.7
+//    1 x 16000 f32     5.1,  4.7     9.5,  9.0   10.2, 13.3   12.5, 19.4
+//  200 x 16000 f32     8.0,  5.7    15.4, 10.8   18.9, 15.2   25.0, 21.1
+//  200 x 32000 bf16    9.4,  7.0    16.3, 13.2   20.5, 18.2   27.6, 24.8
+//  256 x 131072 bf16  17.2, 16.9    25.0, 29.9   32.4, 41.7   46.4, 61.1
+//  400 x 50001 bf16      -, 14.3       -, 22.1      -, 29.9      -, 42.2
+// (of the last, split: 24.5, 32.3, 45.8 with alternatives)
 constexpr int64_t kWant = 1024;
 constexpr int64_t kWantPlain = 512;
 constexpr int64_t kWhole = 384;
+constexpr int64_t kSome = 128;  // rows from which twice as long ones are short
 constexpr int64_t kMaxSplits = 64;
 // of distillation: up to 4 rows a wave, where a launch less is the shorter way
 constexpr int64_t kOneBlock = 64;
@@ -1037,12 +1045,17 @@ Plan plan_of(LmType t, int64_t rows, int64_t v, int top) {
   Plan p;
   int64_t word = (int64_t)kThreads * vec_of(t);
   const int64_t want = top ? kWant : kWantPlain;
-  p.unroll = rows * ((v + 4 * word - 1) / (4 * word)) >= want ? 4 : 1;
+  const bool alone =
+      rows >= kWhole || v <= (top && rows < kSome ? 8 : 16) * word;
+  p.unroll =
+      v > word && (alone || rows * ((v + 4 * word - 1) / (4 * word)) >= want)
+          ? 4
+          : 1;
   int64_t chunk = word * p.unroll;
   int64_t chunks = (v + chunk - 1) / chunk;
   int64_t splits = std::min(std::min(chunks, kMaxSplits),
                             std::max<int64_t>(1, want / rows));
-  if (rows >= kWhole) splits = 1;
+  if (alone) splits = 1;
   if (top) splits = std::min<int64_t>(splits, kMaxKeys / top);
   p.part_len = (chunks + splits - 1) / splits * chunk;
   p.splits = (v + p.part_len - 1) / p.part_len;
