@@ -8,14 +8,14 @@
 // captured graph, its own. The operators with gradients are nodes of torch's
 // graph. All of that stands here and not in python because the host's part
 // is the longer one where there is little work (us of host time, python and
-// here: quantising 16 x 4096 8.3, 6; a row's log probabilities 18, 10; a
+// here: quantising 16 x 4096 8.3, 5.4; a row's log probabilities 18, 8; a
 // loss with its gradient 94, 55, of which torch's own engine takes 40). It
 // is host code: the only file that uses torch's headers.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -77,8 +77,15 @@ std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t last) {
   return size;
 }
 
+// what at::empty comes to for a GPU tensor, without its way there
 Tensor empty(const Tensor& like, at::IntArrayRef size, at::ScalarType type) {
-  return at::empty(size, like.options().dtype(type).requires_grad(false));
+  return Tensor(
+      at::detail::empty_cuda(size, type, like.device(), std::nullopt));
+}
+
+// scratch of a call
+Tensor bytes(const Tensor& like, int64_t size) {
+  return size ? empty(like, {size}, at::kByte) : Tensor();
 }
 
 template <class T = float>
@@ -124,8 +131,7 @@ Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
   if (!y.numel()) return y;
   const int64_t m = y.numel() / n;
   Launch on(x);
-  const int64_t need = mx_linear_workspace(m, n, k, packed);
-  Tensor work = need ? empty(wc, {need}, at::kByte) : Tensor();
+  Tensor work = bytes(wc, mx_linear_workspace(m, n, k, packed));
   const Tensor b = bias.defined() ? plain(bias) : bias;
   if (packed) {
     launch_mx_linear((LmType)code, nullptr, 0, data<uint8_t>(x),
@@ -171,13 +177,12 @@ Scores score(const Tensor& logits, const Tensor& tokens, const Tensor& top_lp,
   if (grad) s.stats = empty(logits, {r.rows, 4}, at::kFloat);
   if (r.rows) {
     Launch on(logits);
-    Tensor work =
-        empty(logits, {score_workspace(t, r.rows, r.v, top)}, at::kByte);
+    Tensor work = bytes(logits, score_workspace(t, r.rows, r.v, top));
     launch_token_logprobs(t, r.x.data_ptr(), r.stride, r.rows, r.v,
                           data<int64_t>(tokens), ignore, (float)inv_t, top,
                           data(s.logprobs), data(s.entropy), data(top_lp),
                           data<int64_t>(top_ids), data<RowStats>(s.stats),
-                          work.data_ptr(), on.stream);
+                          data<void>(work), on.stream);
   }
   return s;
 }
@@ -247,12 +252,12 @@ Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
   float* q = stats + 4 * r.rows;
   float* count = how ? q + r.rows * k : nullptr;
   Launch on(logits);
-  Tensor work = empty(logits, {score_workspace(t, r.rows, r.v, 0)}, at::kByte);
+  Tensor work = bytes(logits, score_workspace(t, r.rows, r.v, 0));
   launch_distill(t, r.x.data_ptr(), r.stride, r.rows, r.v,
                  (LmType)teacher_code, record.data_ptr(), data<int64_t>(ids),
                  (int)k, (float)inv_t, how ? count + 1 : data(l.loss), q,
                  (RowStats*)stats, how ? data(l.loss) : nullptr, count,
-                 how == 2, work.data_ptr(), on.stream);
+                 how == 2, data<void>(work), on.stream);
   return l;
 }
 
@@ -415,13 +420,14 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(args, n, 6);
-  const Tensor &logits = a.tensor(), &tokens = a.tensor();
+  const Tensor &logits = a.tensor(), &ids = a.tensor();
   const int64_t code = a.type(), top = a.integer(0, kMaxTop);
   const double inv_t = a.real();
   const int64_t ignore = a.integer();
   Tensor logprobs, entropy, top_lp, top_ids;
   {
     pybind11::gil_scoped_release no_gil;
+    const Tensor tokens = ids.contiguous();
     const auto size = with_last(lead(logits), top);
     top_lp = empty(logits, size, at::kFloat);
     top_ids = empty(logits, size, at::kLong);
@@ -445,15 +451,17 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(args, n, 7);
-  const Tensor &logits = a.tensor(), &teacher = a.tensor(), &ids = a.tensor();
+  const Tensor &logits = a.tensor(), &teacher = a.tensor();
+  const Tensor& teacher_ids = a.tensor();
   const int64_t code = a.type(), teacher_code = a.type();
   const double inv_t = a.real();
   const int64_t how = a.integer(0, 2);
-  TORCH_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= kMaxRecord,
+  TORCH_CHECK(teacher_ids.size(-1) >= 1 && teacher_ids.size(-1) <= kMaxRecord,
               "bad record length");
   Tensor loss;
   {
     pybind11::gil_scoped_release no_gil;
+    const Tensor ids = teacher_ids.contiguous();
     if (needs_grad(logits)) {
       loss = Distill::apply(logits, teacher, ids, code, teacher_code, inv_t,
                             how)[0];

@@ -56,16 +56,16 @@ def _check_temperature(temperature) -> float:
 
 def _check_ids(torch, name, ids, shape, device):
     hiptorch.check_tensor(name, ids)
-    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
-        raise TypeError(f"{name} must be int64 or int32, got {ids.dtype}")
+    if ids.dtype != torch.int64:
+        if ids.dtype != torch.int32:
+            raise TypeError(f"{name} must be int64 or int32, got {ids.dtype}")
+        ids = ids.long()
     if ids.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got "
                          f"{list(ids.shape)}")
     if ids.device != device:
         raise ValueError(f"{name} are on {ids.device}, logits on {device}")
-    if ids.dtype != torch.int64:
-        ids = ids.long()
-    return ids.contiguous()
+    return ids
 
 
 def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
@@ -88,16 +88,17 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature=1.0,
     torch = hiptorch.lm_torch()
     code = _check_logits(logits)
     t = _check_temperature(temperature)
-    lead, v = logits.shape[:-1], logits.shape[-1]
+    shape = logits.shape
     top = int(top)
-    if not 0 <= top <= min(MAX_TOP, v):
-        raise ValueError(f"top must be in [0, {min(MAX_TOP, v)}], got {top}")
-    tokens = _check_ids(torch, "tokens", tokens, lead, logits.device)
+    if not 0 <= top <= MAX_TOP or top > shape[-1]:
+        raise ValueError(f"top must be in [0, {min(MAX_TOP, shape[-1])}], got "
+                         f"{top}")
+    tokens = _check_ids(torch, "tokens", tokens, shape[:-1], logits.device)
     if not logits.is_cuda:
         return _cpu_token_logprobs(torch, logits, tokens, top, t,
                                    int(ignore_index))
     STATS["token_logprobs"] += 1
-    return TokenLogprobs(*hiptorch.ensure_hiplm().token_logprobs(
+    return TokenLogprobs._make(hiptorch.ensure_hiplm().token_logprobs(
         logits, tokens, code, top, 1.0 / t, int(ignore_index)))
 
 
