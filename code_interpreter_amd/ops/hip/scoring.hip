@@ -1031,7 +1031,8 @@ constexpr int64_t kWantPlain = 512;
 constexpr int64_t kWhole = 384;
 constexpr int64_t kSome = 128;  // rows from which twice as long ones are short
 constexpr int64_t kMaxSplits = 64;
-// of distillation: up to 4 rows a wave, where a launch less is the shorter way
+// rows of distillation whose parts one block joins, up to 4 a wave, and adds
+// up: a launch less
 constexpr int64_t kOneBlock = 64;
 
 struct Plan {
@@ -1110,7 +1111,7 @@ void run_score(LmType t, const void* x, int64_t stride, int64_t rows,
 
 int64_t score_workspace(LmType t, int64_t rows, int64_t v, int top) {
   Plan p = plan_of(t, rows, v, top);
-  if (p.splits == 1 && rows > kOneBlock) return 0;  // one block makes a row
+  if (p.splits == 1) return 0;  // one block makes a row
   return rows * p.splits * (int64_t)(sizeof(Part) + 8 * (int64_t)top);
 }
 
@@ -1171,8 +1172,8 @@ void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
   const float c = inv_t * kLog2e;
   Part* parts = (Part*)ws;
   const DistillEnd e = {tt, teacher, ids, k, inv_t, row_loss, q, stats};
-  const bool whole = total && rows <= kOneBlock;
-  const bool direct = p.splits == 1 && !whole;
+  const bool direct = p.splits == 1;
+  const bool whole = !direct && total && rows <= kOneBlock;
   run_score(t, x, stride, rows, v, p, c, false, direct, e, parts, nullptr,
             stream);
   if (!direct)
