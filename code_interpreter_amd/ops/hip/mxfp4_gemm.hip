@@ -644,8 +644,8 @@ __global__ __launch_bounds__(WM* WN* WK * 64) void small_kernel(
 // ---------------------------------------------------------------------------
 // few tokens
 // ---------------------------------------------------------------------------
-// The weights are read once, from memory into registers, and bound the time;
-// up to 16 tokens are held against them. A block makes 16 outputs of all
+// The weights are read once, from memory into registers, and bound the time; G
+// groups of 16 tokens are held against them. A block makes 16 outputs of all
 // tokens: its 8 waves take turns along k, 512 elements a turn, and add up
 // through shared memory at the end, in a fixed order. The loads of two turns
 // are under way before the first is worked on. The tokens come from memory
@@ -691,8 +691,8 @@ __device__ __forceinline__ void load_turn(const uint8_t* codes,
   }
 }
 
-template <LmType T, bool kPacked>
-__global__ __launch_bounds__(512) void few_kernel(
+template <LmType T, bool kPacked, int G>
+__global__ __launch_bounds__(512, G > 1 ? 2 : 4) void few_kernel(
     const void* __restrict__ x, int64_t stride,
     const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs,
     const uint8_t* __restrict__ wc, const uint8_t* __restrict__ ws,
@@ -750,71 +750,99 @@ __global__ __launch_bounds__(512) void few_kernel(
     __syncthreads();
   }
 
-  v4f acc = {};
-  const int token = min(l15, m - 1);
+  v4f acc[G] = {};
+  int token[G];
+#pragma unroll
+  for (int g = 0; g < G; g++) token[g] = min(g * 16 + l15, m - 1);
   for (int turn = wave; turn < turns; turn += kWaves) {
     Turn now = next;
     next = after;
     if (turn + 2 * kWaves < turns)
       load_turn<true>(wrow, srow, (turn + 2 * kWaves) * 16, nb, q, after);
-    Turn tok;
-    if constexpr (kPacked) {
-      load_turn<true>(xc + (int64_t)token * nb * 16, xs + (int64_t)token * nb,
-                      turn * 16, nb, q, tok);
-    } else {
-      load_turn<false>((const uint8_t*)smem + token * crow, nullptr, turn * 16,
-                       nb, q, tok);
-      tok.s = *(const u32x4*)(lds_s + token * sstride + turn * 16);
-    }
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          operand(now.c[j]), operand(tok.c[j]), acc, 4, 4, 0,
-          (int)(now.s[j] >> (8 * q)), 0, (int)(tok.s[j] >> (8 * q)));
+    for (int g = 0; g < G; g++) {
+      Turn tok;
+      if constexpr (kPacked) {
+        load_turn<true>(xc + (int64_t)token[g] * nb * 16,
+                        xs + (int64_t)token[g] * nb, turn * 16, nb, q, tok);
+      } else {
+        load_turn<false>((const uint8_t*)smem + token[g] * crow, nullptr,
+                         turn * 16, nb, q, tok);
+        tok.s = *(const u32x4*)(lds_s + token[g] * sstride + turn * 16);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        acc[g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            operand(now.c[j]), operand(tok.c[j]), acc[g], 4, 4, 0,
+            (int)(now.s[j] >> (8 * q)), 0, (int)(tok.s[j] >> (8 * q)));
+    }
   }
 
   __syncthreads();  // the tokens' place is taken by the partial sums
-  v4f* part = (v4f*)smem;  // [wave][64]
-  part[threadIdx.x] = acc;
+  v4f* part = (v4f*)smem;  // [group][wave][64]
+#pragma unroll
+  for (int g = 0; g < G; g++) part[g * 512 + threadIdx.x] = acc[g];
   __syncthreads();
-  if (wave) return;
+  if (wave >= G) return;  // a wave adds up a group
   const int64_t col = n0 + 4 * q;
   const int valid = (int)min((int64_t)4, n - col);
-  if (l15 >= m || valid <= 0) return;
-  v4f sum = part[lane];
+  const int row = wave * 16 + l15;
+  if (row >= m || valid <= 0) return;
+  v4f sum = part[wave * 512 + lane];
 #pragma unroll
-  for (int w = 1; w < kWaves; w++) sum += part[w * 64 + lane];
+  for (int w = 1; w < kWaves; w++) sum += part[wave * 512 + w * 64 + lane];
   float f[4];
   for (int r = 0; r < 4; r++)
     f[r] = sum[r] + (bias && r < valid ? bias_at<T>(bias, col + r) : 0.f);
-  store4<T>(y, (int64_t)l15 * n + col, f, valid);
+  store4<T>(y, (int64_t)row * n + col, f, valid);
 }
 
 // ---------------------------------------------------------------------------
 // launching
 // ---------------------------------------------------------------------------
-// Few tokens: up to 16. Their kernel quantises them itself where that is
-// less work than a launch more (us, itself and with a launch: weights of 4096
-// x 4096, m = 4: 5.0, 6.2; m = 8: 6.5, 6.4; 8192 x 8192, m = 4: 12.7, 14.2; m
-// = 8: 17.1, 15.1; 8192 x 1024, m = 16: 4.9, 6.5). From codes it is the better
-// one for weights up to 2^25 elements, above which the tokens that each
-// block reads weigh more (m = 16, against small tiles: 4096 x 4096 7.1, 9.3;
-// 8192 x 8192 17.0, 13.5).
+// Few tokens are up to 16, or 64 of which each block quantises all. The latter
+// takes 0.1 ns an element for each of the chip's fills with blocks (two a
+// compute unit, one of more than 16 tokens), and saves a launch of 3 us, as
+// much of the host's time again. In us, itself and with a launch:
+// 4096 x  512, m = 17: 4.2,  5.9; m = 48:   6.0, 6.1
+// 4096 x 1024, m = 32: 6.1,  6.3
+// 8192 x 1024, m = 16: 4.9,  6.5; m = 32:  10.3, 6.4
+// 4096 x 4096, m =  4: 5.0,  6.2; m =  8:   6.5, 6.4
+// 8192 x 8192, m =  1: 10.3, 12.2; m = 4:  13.0, 13.0
+// 131072 x 4096, m = 1: 68.6, 71; m =  8: 121.5, 72
 constexpr int64_t kFewTokens = 16;
+constexpr int64_t kFusedTokens = 64;
 constexpr int64_t kFusedElements = 1 << 15;
+constexpr int64_t kFill = 512 * 16;  // outputs
+// From codes a block reads all tokens' along the whole of k, which weighs more
+// the longer it is. Against small tiles, m = 1, 8, 16:
+//   8192 x  4096  6.0,  6.8,  7.6
+//   8192 x  8192  9.2, 10.8, 12.2  tiles 12.3, 12.7, 12.9
+//  16384 x  8192 16.7, 18.5, 21.0        18.5, 18.5, 18.6
+//   8192 x 16384 15.7, 18.3, 21.1        18.7, 19.3, 19.2
+//  32768 x  4096 17.7, 18.7, 21.1        22.4, 24.2, 25.1
+// 131072 x  4096 68.7, 68.3, 76.9        95.5, 95.1, 96.4
+// Tokens that are quantised first cost the tiles nothing more, and this 3 us.
+constexpr int64_t kFewK = 4096;
 constexpr int64_t kFewWeights = 1 << 25;
 
 int64_t few_lds(int64_t m, int64_t nb) {
   return m * (few_codes((int)nb) + few_scales((int)nb));
 }
 
-bool fuses(int64_t m, int64_t nb) {
-  return m <= kFewTokens && m * nb * kMxBlock <= kFusedElements;
+bool fuses(int64_t m, int64_t n, int64_t nb) {
+  const int64_t elements = m * nb * kMxBlock;
+  if (m > kFewTokens)
+    return m <= kFusedTokens && n <= kFill / 2 && elements <= kFusedElements;
+  return elements * ((n + kFill - 1) / kFill) <= kFusedElements;
 }
 
 bool few(int64_t m, int64_t n, int64_t nb, bool packed) {
-  return m <= kFewTokens &&
-         ((!packed && fuses(m, nb)) || n * nb * kMxBlock <= kFewWeights);
+  const int64_t k = nb * kMxBlock;
+  if (!packed && fuses(m, n, nb)) return true;
+  if (m > kFewTokens) return false;
+  if (k <= kFewK || n * k <= kFewWeights) return true;
+  return packed && (m <= kFewTokens / 2 || n * k <= 2 * kFewWeights);
 }
 
 template <LmType T, int WM, int WN, int FM, int FN>
@@ -934,10 +962,21 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
     return run_tiles<T>(x, stride, xc, xs, wc, ws, bias, y, m, n, k, scratch,
                         stream);
   const dim3 grid = lm_grid((n + 15) / 16, 512);
-  const int64_t sums = 512 * sizeof(v4f);
-  if (x && fuses(m, nb)) {
-    few_kernel<T, false><<<grid, 512, std::max(few_lds(m, nb), sums), stream>>>(
-        x, stride, nullptr, nullptr, wc, ws, bias, y, (int)m, n, k, (int)nb);
+  const int64_t sums = 512 * sizeof(v4f);  // of 16 tokens
+  if (x && fuses(m, n, nb)) {
+    auto go = [&](auto groups) {
+      constexpr int G = decltype(groups)::value;
+      few_kernel<T, false, G>
+          <<<grid, 512, std::max(few_lds(m, nb), G * sums), stream>>>(
+              x, stride, nullptr, nullptr, wc, ws, bias, y, (int)m, n, k,
+              (int)nb);
+    };
+    if (m <= 16)
+      go(std::integral_constant<int, 1>{});
+    else if (m <= 32)
+      go(std::integral_constant<int, 2>{});
+    else
+      go(std::integral_constant<int, 4>{});
   } else {
     if (x) {
       uint8_t* codes = (uint8_t*)scratch;
@@ -946,7 +985,7 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
       xc = codes;
       xs = scales;
     }
-    few_kernel<T, true><<<grid, 512, sums, stream>>>(
+    few_kernel<T, true, 1><<<grid, 512, sums, stream>>>(
         nullptr, 0, xc, xs, wc, ws, bias, y, (int)m, n, k, (int)nb);
   }
   HIP_CHECK(hipGetLastError());
@@ -957,7 +996,7 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
 int64_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, bool packed) {
   const int64_t nb = mx_blocks(k);
   if (few(m, n, nb, packed))
-    return packed || fuses(m, nb) ? 0 : m * nb * (kMxBytes + 1);
+    return packed || fuses(m, n, nb) ? 0 : m * nb * (kMxBytes + 1);
   TileSpace space = tile_space(m, n, nb, packed);
   return space.codes + space.xs + space.ws;
 }

@@ -387,3 +387,24 @@ def test_views_that_negate(mx, m):
     assert bias.is_neg()
     assert torch.equal(hipmx.linear(x, w, bias),
                        hipmx.linear(x.resolve_neg(), w, bias.resolve_neg()))
+
+
+@pytest.mark.parametrize("m,n,k", [
+    # 17 to 64 tokens that every block quantises, and just more than it does
+    (17, 4095, 1900), (31, 33, 1000), (32, 100, 1024), (32, 100, 1025),
+    (33, 40, 992), (47, 4096, 690), (63, 4095, 520), (64, 17, 31),
+    (64, 4097, 100), (64, 1, 1), (50, 15, 600),
+    # few tokens and many outputs
+    (3, 20001, 4096), (8, 40000, 700), (16, 33000, 1030), (2, 9000, 8200),
+])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_few_tokens(mx, m, n, k, dtype):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, n, k, dtype, m + n + k)
+    y = hipmx.linear(x, w, bias)
+    check_linear(torch, hipmx, y, x, w, bias)
+    check_linear(torch, hipmx, hipmx.linear(hipmx.quantize(x), w, dtype=x.dtype),
+                 x, w, None)
+    wide = torch.full((m, k + 3), 9.0, dtype=x.dtype, device="cuda")
+    wide[:, 1:k + 1] = x
+    assert torch.equal(hipmx.linear(wide[:, 1:k + 1], w, bias), y)
