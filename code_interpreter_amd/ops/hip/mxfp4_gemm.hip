@@ -800,20 +800,20 @@ __global__ __launch_bounds__(512, G > 1 ? 2 : 4) void few_kernel(
 // ---------------------------------------------------------------------------
 // launching
 // ---------------------------------------------------------------------------
-// Few tokens are up to 16, or 64 of which each block quantises all. The latter
-// takes 0.1 ns an element for each of the chip's fills with blocks (two a
-// compute unit, one of more than 16 tokens), and saves a launch of 3 us, as
-// much of the host's time again. In us, itself and with a launch:
+// Few tokens are up to 16, or 64 where one block a compute unit makes all
+// outputs: two do not fit, of more than 16.
+constexpr int64_t kFewTokens = 16, kFewTokensAtOnce = 64;
+constexpr int64_t kFill = 512 * 16;  // outputs, of two blocks a unit
+// Quantised by each block for itself they take 0.1 ns an element for each of
+// the chip's fills with blocks, and save a launch of 3 us, as much of the
+// host's time again. In us, so and with a launch:
 // 4096 x  512, m = 17: 4.2,  5.9; m = 48:   6.0, 6.1
 // 4096 x 1024, m = 32: 6.1,  6.3
 // 8192 x 1024, m = 16: 4.9,  6.5; m = 32:  10.3, 6.4
 // 4096 x 4096, m =  4: 5.0,  6.2; m =  8:   6.5, 6.4
 // 8192 x 8192, m =  1: 10.3, 12.2; m = 4:  13.0, 13.0
 // 131072 x 4096, m = 1: 68.6, 71; m =  8: 121.5, 72
-constexpr int64_t kFewTokens = 16;
-constexpr int64_t kFusedTokens = 64;
 constexpr int64_t kFusedElements = 1 << 15;
-constexpr int64_t kFill = 512 * 16;  // outputs
 // From codes a block reads all tokens' along the whole of k, which weighs more
 // the longer it is. Against small tiles, m = 1, 8, 16:
 //   8192 x  4096  6.0,  6.8,  7.6
@@ -822,7 +822,14 @@ constexpr int64_t kFill = 512 * 16;  // outputs
 //   8192 x 16384 15.7, 18.3, 21.1        18.7, 19.3, 19.2
 //  32768 x  4096 17.7, 18.7, 21.1        22.4, 24.2, 25.1
 // 131072 x  4096 68.7, 68.3, 76.9        95.5, 95.1, 96.4
-// Tokens that are quantised first cost the tiles nothing more, and this 3 us.
+// and m = 17, 32, 33, 64:
+//   4096 x  4096  4.9,  5.7,  6.4,  8.1         8.5,  8.4,  8.7,  8.8
+//   4096 x  8192  8.5, 10.0, 11.3, 14.7        11.5, 11.4, 11.6, 11.6
+//   4096 x 16384 14.3, 16.8, 19.3, 25.7        16.9, 17.0, 17.3, 17.3
+// Tokens that are quantised first cost the tiles nothing more, and this 3 us:
+//   4096 x  2048  6.4,  6.8,  7.3,  8.2         6.9,  7.0,  7.1,  7.1
+//   4096 x  4096  7.6,  8.7,  9.2, 11.3         9.3,  9.3,  9.4,  9.5
+//   4096 x  8192 11.6, 13.3, 14.6, 18.0        12.1, 12.2, 12.4, 12.4
 constexpr int64_t kFewK = 4096;
 constexpr int64_t kFewWeights = 1 << 25;
 
@@ -833,14 +840,18 @@ int64_t few_lds(int64_t m, int64_t nb) {
 bool fuses(int64_t m, int64_t n, int64_t nb) {
   const int64_t elements = m * nb * kMxBlock;
   if (m > kFewTokens)
-    return m <= kFusedTokens && n <= kFill / 2 && elements <= kFusedElements;
+    return m <= kFewTokensAtOnce && n <= kFill / 2 &&
+           elements <= kFusedElements;
   return elements * ((n + kFill - 1) / kFill) <= kFusedElements;
 }
 
 bool few(int64_t m, int64_t n, int64_t nb, bool packed) {
   const int64_t k = nb * kMxBlock;
   if (!packed && fuses(m, n, nb)) return true;
-  if (m > kFewTokens) return false;
+  if (m > kFewTokens) {
+    const int64_t most = packed ? kFewTokensAtOnce : kFewTokensAtOnce / 2;
+    return m <= most && n <= kFill / 2 && m * k <= most * kFewK;
+  }
   if (k <= kFewK || n * k <= kFewWeights) return true;
   return packed && (m <= kFewTokens / 2 || n * k <= 2 * kFewWeights);
 }
@@ -952,6 +963,16 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
     run_small<T, 1, 1, 4, 6>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
 }
 
+template <class F>
+void by_groups(int64_t m, F f) {
+  if (m <= 16)
+    f(std::integral_constant<int, 1>{});
+  else if (m <= 32)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 4>{});
+}
+
 template <LmType T>
 void run_linear(const void* x, int64_t stride, const uint8_t* xc,
                 const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
@@ -964,19 +985,13 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
   const dim3 grid = lm_grid((n + 15) / 16, 512);
   const int64_t sums = 512 * sizeof(v4f);  // of 16 tokens
   if (x && fuses(m, n, nb)) {
-    auto go = [&](auto groups) {
+    by_groups(m, [&](auto groups) {
       constexpr int G = decltype(groups)::value;
       few_kernel<T, false, G>
           <<<grid, 512, std::max(few_lds(m, nb), G * sums), stream>>>(
               x, stride, nullptr, nullptr, wc, ws, bias, y, (int)m, n, k,
               (int)nb);
-    };
-    if (m <= 16)
-      go(std::integral_constant<int, 1>{});
-    else if (m <= 32)
-      go(std::integral_constant<int, 2>{});
-    else
-      go(std::integral_constant<int, 4>{});
+    });
   } else {
     if (x) {
       uint8_t* codes = (uint8_t*)scratch;
@@ -985,8 +1000,11 @@ void run_linear(const void* x, int64_t stride, const uint8_t* xc,
       xc = codes;
       xs = scales;
     }
-    few_kernel<T, true, 1><<<grid, 512, sums, stream>>>(
-        nullptr, 0, xc, xs, wc, ws, bias, y, (int)m, n, k, (int)nb);
+    by_groups(m, [&](auto groups) {
+      constexpr int G = decltype(groups)::value;
+      few_kernel<T, true, G><<<grid, 512, G * sums, stream>>>(
+          nullptr, 0, xc, xs, wc, ws, bias, y, (int)m, n, k, (int)nb);
+    });
   }
   HIP_CHECK(hipGetLastError());
 }
