@@ -92,9 +92,12 @@ constexpr int kLayRows = kPrepareThreads, kLaySteps = 4;  // of one that does no
 __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
                                                uint2* to, int64_t rows,
                                                int nb, int steps, int blk) {
-  const int parts = (steps + kLaySteps - 1) / kLaySteps;
-  const int64_t row = (int64_t)(blk / parts) * kLayRows + threadIdx.x;
-  const int t0 = blk % parts * kLaySteps;
+  // a row's parts share its cache lines: by blocks of one chiplet, which gets
+  // every eighth
+  const int parts = (steps + kLaySteps - 1) / kLaySteps, eight = 8 * parts;
+  const int64_t row =
+      ((int64_t)(blk / eight) * 8 + blk % 8) * kLayRows + threadIdx.x;
+  const int t0 = blk % eight / 8 * kLaySteps;
   if (row >= rows) return;
   const uint8_t* p = from + row * nb;
   struct __attribute__((packed)) raw8 {
@@ -906,7 +909,7 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   uint8_t* xst = codes + space.codes;
   uint2* wst = (uint2*)(xst + space.xs);
   auto lay_blocks = [&](int64_t rows) {
-    return (rows + kLayRows - 1) / kLayRows *
+    return (rows + 8 * kLayRows - 1) / (8 * kLayRows) * 8 *
            ((steps + kLaySteps - 1) / kLaySteps);
   };
   const int64_t w_blocks = lay_blocks(n);
@@ -929,9 +932,10 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   HIP_CHECK(hipGetLastError());
   if (x) xc = codes;
   auto* xs2 = (const uint2*)xst;
-  // The largest tiles of which there are enough to fill the chip. In us, of
-  // m x n x k with tiles of 256 x 256, 128 x 128 (2 buffers), 64 x 128, 64 x
-  // 64 (3), 32 x 64 (4), 32 x 32 (6):
+  // The largest tiles of which there are enough to fill the chip, and of which
+  // the tokens fill more than half of one. In us, of m x n x k with tiles of
+  // 256 x 256, 128 x 128 (2 buffers), 64 x 128, 64 x 64 (3), 32 x 64 (4), 32 x
+  // 32 (6):
   // 2000 x 5001 x 2056 30.6, 33.0,    -,    -, 49.0, 74.0
   // 2000 x 4096 x 4096 38.8, 33.5, 40.5,    -, 56.8, 86.9
   // 1200 x 8192 x 8192 60.6, 74.8, 78.2,    -,    -,    -
@@ -943,15 +947,19 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   //  200 x 4096 x 4096    -, 19.5, 14.2, 13.0, 12.5,    -
   //  100 x 4096 x 4096 30.8, 19.3, 13.5, 12.2, 10.8, 11.1
   //  333 x 700 x 700   20.9, 11.6,    -,  9.1,  8.2,  7.6
+  //  160 x 131072 x 4096 107, 124,  126,  137,  160,    -
+  //  128 x 131072 x 4096 106,  91,  104,  113,  138,    -
+  //   64 x 131072 x 4096 100,  86,   79,   86,   95,    -
+  //   32 x 32768 x 4096 33.4, 25.8, 19.2, 19.7, 19.1,   -
   auto tiles = [&](int64_t bm, int64_t bn) {
     return ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
   };
   const int b = (int)nb;
   // the small tiles' scales are addressed in 31 bits
   const bool far = std::max(m, n) * steps * 8 >= (int64_t)1 << 31;
-  if (tiles(256, 256) >= 144)
+  if (m > 128 && tiles(256, 256) >= 144)
     run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
-  else if (tiles(128, 128) >= 240 || far)
+  else if ((m > 64 && tiles(128, 128) >= 240) || far)
     run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if (tiles(64, 128) >= 160)
     run_small<T, 2, 4, 1, 3>(xc, xs2, wc, wst, bias, y, m, n, b, stream);

@@ -408,3 +408,15 @@ def test_linear_few_tokens(mx, m, n, k, dtype):
     wide = torch.full((m, k + 3), 9.0, dtype=x.dtype, device="cuda")
     wide[:, 1:k + 1] = x
     assert torch.equal(hipmx.linear(wide[:, 1:k + 1], w, bias), y)
+
+
+@pytest.mark.parametrize("m,n,k", [
+    # low and wide: tiles by their height, scales laid out in many blocks
+    (33, 40001, 300), (64, 33000, 1100), (65, 40001, 520), (128, 33000, 300),
+    (129, 40001, 264), (70, 2049, 2500),
+])
+def test_linear_wide(mx, m, n, k):
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, n, k, "bfloat16", m + n + k)
+    check_linear(torch, hipmx, hipmx.linear(x, w, bias), x, w, bias)
+    check_linear(torch, hipmx, hipmx.linear(hipmx.quantize(x), w), x, w, None)
