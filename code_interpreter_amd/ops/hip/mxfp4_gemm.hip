@@ -957,7 +957,14 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   const int b = (int)nb;
   // the small tiles' scales are addressed in 31 bits
   const bool far = std::max(m, n) * steps * 8 >= (int64_t)1 << 31;
-  if (m > 128 && tiles(256, 256) >= 144)
+  // A tile of 256 x 256 is a compute unit's alone, so that its start and end
+  // are not hidden: it wants a long k, and not a second round for a few:
+  // 8192 x 8192 x  512 56.1, 54.6, x 1024 77.1, 75.3, x 1536 91.5, 93.5
+  // 4096 x 4096 x  512 21.0, 20.7, x 1024 24.8, 25.2, x 1536 29.9, 30.8
+  //  164 x 43710 x 512 21.9, 17.2, x 1024 25.3, 21.3, x 1536 28.3, 24.9
+  // 7055 x 3310 x 1536 50.2, 41.9, x 3100 78.8, 75.9 (364 of them)
+  const int64_t large = tiles(256, 256);
+  if (m > 128 && k >= 1024 && large >= 144 && !(large > 256 && large <= 384))
     run_tile<T, 2, 2, 4, 4>(xc, xs2, wc, wst, bias, y, m, n, b, stream);
   else if ((m > 64 && tiles(128, 128) >= 240) || far)
     run_tile<T, 2, 2, 2, 2>(xc, xs2, wc, wst, bias, y, m, n, b, stream);

@@ -413,7 +413,7 @@ def test_linear_few_tokens(mx, m, n, k, dtype):
 @pytest.mark.parametrize("m,n,k", [
     # low and wide: tiles by their height, scales laid out in many blocks
     (33, 40001, 300), (64, 33000, 1100), (65, 40001, 520), (128, 33000, 300),
-    (129, 40001, 264), (70, 2049, 2500),
+    (129, 40001, 264), (70, 2049, 2500), (250, 40001, 1100), (1100, 9000, 1060),
 ])
 def test_linear_wide(mx, m, n, k):
     torch, hipmx = mx
