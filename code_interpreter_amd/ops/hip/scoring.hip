@@ -955,8 +955,9 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
     const float* __restrict__ count, typename Elem<T>::type* __restrict__ dx) {
   using E = Elem<T>;
   constexpr int kChunk = kThreads * E::kVec * U;
-  __shared__ int64_t s_id[kMaxRecord];
-  __shared__ float s_q[kMaxRecord];
+  static_assert(kMaxRecord == kThreads, "");
+  __shared__ alignas(16) int s_id[kMaxRecord];
+  __shared__ alignas(16) float s_q[kMaxRecord];
   const int64_t row = blockIdx.x / (unsigned)chunks;
   const int64_t base = (int64_t)(blockIdx.x % (unsigned)chunks) * kChunk;
   const int tid = threadIdx.x;
@@ -973,10 +974,9 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
     for (int i = 0; i < U; i++)
       w[i] = load_vec<T>(src, base + (int64_t)(i * kThreads + tid) * E::kVec,
                          v);
-    if (tid < k) {
-      s_id[tid] = ids[row * k + tid];
-      s_q[tid] = q[row * k + tid];
-    }
+    const int64_t id = tid < k ? ids[row * k + tid] : -1;
+    s_id[tid] = id >= 0 && id < v ? (int)id : -1;
+    s_q[tid] = tid < k ? q[row * k + tid] : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < U; i++) {
@@ -997,15 +997,24 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
   }
   if (!live) return;
   __syncthreads();  // also orders the block's stores
-  if (tid >= k) return;
-  const int64_t id = s_id[tid];
-  if (id < base || id >= min(v, base + kChunk)) return;
+  const int id = s_id[tid];
+  if (id < 0 || id < base || id >= base + kChunk) return;
+  // the first of equal ids writes; four a read, or the search would take as
+  // long as the chunk
   float share = 0.f;
-  for (int j = 0; j < k; j++) {
-    if (s_id[j] != id) continue;
-    if (j < tid) return;  // the first of equal ids writes
-    share += s_q[j];
+  bool first = true;
+#pragma unroll 2
+  for (int j = 0; j < k; j += 4) {
+    const int4 a = *(const int4*)&s_id[j];
+    const float4 b = *(const float4*)&s_q[j];
+    share += a.x == id ? b.x : 0.f;
+    share += a.y == id ? b.y : 0.f;
+    share += a.z == id ? b.z : 0.f;
+    share += a.w == id ? b.w : 0.f;
+    first &= !((a.x == id & j < tid) | (a.y == id & j + 1 < tid) |
+               (a.z == id & j + 2 < tid) | (a.w == id & j + 3 < tid));
   }
+  if (!first) return;
   float p = exp2_raw((E::load(src + id) - st.max) * c - st.log2_sum);
   E::store(dst + id, g * (p - share));
 }
