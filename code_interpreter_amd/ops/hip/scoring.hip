@@ -20,7 +20,7 @@
 // logits: 9 instructions an element forward, an exponential among them. 4096
 // x 131072 bf16: 217 us forward, 4.9 TB/s; backward 340 us, 6.3 TB/s (part
 // of what is read again comes from the chip's cache). Distillation backward,
-// 4096 x 65536: 190 us, 5.6 TB/s. A large copy: 4.8 TB/s.
+// 4096 x 65536: 183 us, 5.9 TB/s. A large copy: 4.8 TB/s.
 //
 // All sums are 32-bit, over a fixed split of the row and in a fixed order:
 // the same input gives the same bits.
@@ -556,6 +556,30 @@ __device__ float load_any(LmType t, const void* p, int64_t i) {
   }
 }
 
+// A wave's part of a row's record: 4 entries a lane. Read in two steps, the
+// logits at the entries' tokens upon the entries.
+template <LmType T>
+struct Record {
+  static constexpr int kMine = kMaxRecord / 64;
+  float z[kMine], x[kMine];
+  int64_t id[kMine];  // -1: none
+
+  __device__ void load_entries(int64_t row, const DistillEnd& e) {
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+      const int at = (threadIdx.x & 63) + 64 * i;
+      id[i] = at < e.k ? e.ids[row * e.k + at] : -1;
+      z[i] = at < e.k ? load_any(e.type, e.teacher, row * e.k + at) : 0.f;
+    }
+  }
+
+  __device__ void load_logits(const typename Elem<T>::type* src, int64_t v) {
+#pragma unroll
+    for (int i = 0; i < kMine; i++)
+      x[i] = id[i] >= 0 && id[i] < v ? Elem<T>::load(src + id[i]) : 0.f;
+  }
+};
+
 // a row by a wave: the teacher's softmax over its record, and
 // T^2 sum q (ln q - ln p). Returns (in every lane) the loss, and whether the
 // row has a record.
@@ -564,32 +588,24 @@ struct RowLoss {
   bool there;
 };
 
-template <LmType T, class GetSums>
-__device__ RowLoss distill_row(
-    int64_t row, const typename Elem<T>::type* x, int64_t stride, int64_t v,
-    const DistillEnd& e, float c, GetSums sums) {
-  constexpr int kMine = kMaxRecord / 64;
+template <LmType T>
+__device__ RowLoss distill_row(int64_t row, Record<T> rec, int64_t v,
+                               const DistillEnd& e, float c, const Triple& t) {
+  constexpr int kMine = Record<T>::kMine;
   const int lane = threadIdx.x & 63;
-  float z[kMine];
-  int64_t id[kMine];
+  auto& z = rec.z;
+  auto& id = rec.id;
   float top = -INFINITY;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < kMine; i++) {
-    int at = lane + 64 * i;
-    id[i] = at < e.k ? e.ids[row * e.k + at] : -1;
-    z[i] = id[i] != -1 ? load_any(e.type, e.teacher, row * e.k + at) : -INFINITY;
+    if (id[i] == -1) z[i] = -INFINITY;
     if (z[i] == -INFINITY) id[i] = -1;
     bad |= z[i] != z[i] || z[i] == INFINITY ||
            (id[i] != -1 && (id[i] < 0 || id[i] >= v));
     top = fmaxf(top, z[i]);
   }
   bad = __any(bad);
-  float xs[kMine];
-#pragma unroll
-  for (int i = 0; i < kMine; i++)
-    xs[i] = id[i] != -1 && !bad ? Elem<T>::load(x + row * stride + id[i]) : 0.f;
-  const Triple t = sums();
   const bool empty = t.m == -INFINITY && t.s == 0.f;
   const float log2_sum = log2f(t.s);
   top = wave_max(top);
@@ -608,7 +624,7 @@ __device__ RowLoss distill_row(
     if (id[i] != -1 && !bad) {
       float lq = (z[i] - top) * c - log2_q;
       share = exp2_raw(lq);
-      float lp = empty ? -INFINITY : (xs[i] - t.m) * c - log2_sum;
+      float lp = empty ? -INFINITY : (rec.x[i] - t.m) * c - log2_sum;
       if (share > 0.f) loss = fmaf(share, lq - lp, loss);
     }
     if (at < e.k) e.q[row * e.k + at] = share;
@@ -716,8 +732,12 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(
             tid < best.have ? sh.keys[tid] : 0;
     }
   } else if constexpr (kDistill) {
-    if (tid < 64)
-      distill_row<T>(row, x, stride, v, end_of_row, c, [&] { return t; });
+    if (tid < 64) {
+      Record<T> rec;
+      rec.load_entries(row, end_of_row);
+      rec.load_logits(src, v);
+      distill_row<T>(row, rec, v, end_of_row, c, t);
+    }
   } else {
     const Token token =
         token_of<T>(end_of_row.tokens[row], src, v, end_of_row);
@@ -897,32 +917,32 @@ __device__ void write_total(double s, double n, int mean, float* total,
   *count = (float)by;
 }
 
+// rows of distillation whose parts one block joins, a wave a row, and adds up:
+// a launch less. In us, so and with that launch: 3 x 70000 f16 7.0, 8.5; by
+// four rows a wave, 61 x 131072 17.3, 11.0.
+constexpr int kOneBlock = 16;
+
 // kWhole: one block for all rows, which also adds them up
 template <LmType T, bool kWhole>
-__global__ __launch_bounds__(kWhole ? 1024 : kThreads) void
+__global__ __launch_bounds__(kWhole ? kOneBlock * 64 : kThreads) void
 distill_rows_kernel(const typename Elem<T>::type* __restrict__ x,
                     int64_t stride, int64_t rows, int64_t v, float c,
                     const Part* __restrict__ parts, int splits, DistillEnd e,
                     int mean, float* __restrict__ total,
                     float* __restrict__ count) {
-  const int64_t first =
+  const int64_t row =
       (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
-  auto make = [&](int64_t row) {
-    return distill_row<T>(row, x, stride, v, e, c, [&] {
-      return join_parts(parts + row * splits, splits, c);
-    });
-  };
-  if constexpr (kWhole) {
-    double s = 0, n = 0;
-    for (int64_t row = first; row < rows; row += 16) {
-      const RowLoss r = make(row);
-      s += r.loss;
-      n += r.there;
-    }
-    write_total(s, n, mean, total, count);
-  } else {
-    if (first < rows) make(first);
+  double s = 0, n = 0;
+  if (row < rows) {
+    Record<T> rec;
+    rec.load_entries(row, e);
+    rec.load_logits(x + row * stride, v);
+    const Triple t = join_parts(parts + row * splits, splits, c);
+    const RowLoss r = distill_row<T>(row, rec, v, e, c, t);
+    s = r.loss;
+    n = r.there;
   }
+  if constexpr (kWhole) write_total(s, n, mean, total, count);
 }
 
 // sum or mean of the rows' losses, in a fixed order, in 64 bits; one block
@@ -1040,9 +1060,6 @@ constexpr int64_t kWantPlain = 512;
 constexpr int64_t kWhole = 384;
 constexpr int64_t kSome = 128;  // rows from which twice as long ones are short
 constexpr int64_t kMaxSplits = 64;
-// rows of distillation whose parts one block joins, up to 4 a wave, and adds
-// up: a launch less
-constexpr int64_t kOneBlock = 64;
 
 struct Plan {
   int unroll;        // words of 16 bytes a thread holds at a time
@@ -1192,7 +1209,7 @@ void launch_distill(LmType t, const void* x, int64_t stride, int64_t rows,
         constexpr bool W = decltype(w)::value;
         distill_rows_kernel<T, W>
             <<<lm_grid(W ? 1 : (rows + kWaves - 1) / kWaves, kThreads),
-               W ? 1024 : kThreads, 0, stream>>>(
+               W ? kOneBlock * 64 : kThreads, 0, stream>>>(
                 (const typename Elem<T>::type*)x, stride, rows, v, c, parts,
                 (int)p.splits, e, mean, total, count);
       };

@@ -377,6 +377,33 @@ def test_distill(lm, dtype, t_dtype, v, k, reduction):
                 assert got[i].isfinite().all()
 
 
+@pytest.mark.parametrize("rows", [16, 17, 64, 65, 390])
+@pytest.mark.parametrize("v", [600, 17003])
+def test_distill_by_the_number_of_rows(lm, rows, v):
+    """What finishes a call's rows goes by their number and length."""
+    torch, hiplm = lm
+    import lm_oracle as oracle
+
+    g = torch.Generator().manual_seed(rows + v)
+    x = torch.randn(rows, v, generator=g)
+    teacher = torch.randn(rows, 30, generator=g)
+    ids = torch.randint(v, (rows, 30), generator=g)
+    ids[::5, 20:] = -1
+    ids[3] = -1
+    ids[4, 7] = ids[4, 2]
+    for reduction in ("mean", "sum"):
+        leaf = x.cuda().requires_grad_(True)
+        loss = hiplm.topk_distill_loss(leaf, teacher.cuda(), ids.cuda(),
+                                       reduction=reduction)
+        want, grad, size = oracle.distill(
+            x.numpy(), teacher.numpy(), ids.numpy(), 1.0, reduction)
+        spread = (relative(v) + 64 * STEP) * 24
+        near(loss, want, spread * (1 + abs(want)) * (
+            rows if reduction == "sum" else 1))
+        (got,) = torch.autograd.grad(loss, [leaf])
+        check_grad(torch, got, grad, size, v, "float32")
+
+
 def test_distill_weights_rows(lm):
     torch, hiplm = lm
     x = torch.randn(5, 300, device="cuda", requires_grad=True)
