@@ -227,10 +227,6 @@ __device__ __forceinline__ uint32_t rth_of_wave(const uint32_t (&x)[kMany],
   return found;
 }
 
-// of a value's order in a key: all that a 16-bit type has, or all
-template <LmType T>
-constexpr int kOrderBits = T == LmType::F32 ? 32 : 20;
-
 // ---------------------------------------------------------------------------
 // alternatives
 // ---------------------------------------------------------------------------
@@ -781,14 +777,20 @@ constexpr int kTies = 8;
 
 template <LmType T>
 __device__ uint64_t rth_key(uint64_t key, int r) {
-  const uint32_t order = (uint32_t)(key >> 32);
-  const uint32_t found = rth_of_wave<kOrderBits<T>>({order}, r);
+  // the bits of a 16-bit type's order behind those are all 0, or 1 where the
+  // value is negative
+  constexpr int kBits = T == LmType::F32 ? 32 : 20;
+  constexpr uint32_t kRest = T == LmType::F32 ? 0 : 0xFFFu;
+  const uint32_t order = (uint32_t)(key >> 32) & ~kRest;
+  const uint32_t found = rth_of_wave<kBits>({order}, r);
+  if (!found) return 0;
   uint32_t below = 0;
-  if (__popcll(__ballot(order >= found)) >= r + kTies && found) {
+  if (__popcll(__ballot(order >= found)) >= r + kTies) {
     const int more = __popcll(__ballot(order > found));
     below = rth_of_wave<32>({order == found ? (uint32_t)key : 0u}, r - more);
   }
-  return (uint64_t)found << 32 | below;
+  const uint32_t rest = found & 0x80000000u ? 0 : kRest;
+  return (uint64_t)(found | rest) << 32 | below;
 }
 
 // A block a row, with alternatives: joins the parts' sorted lists. Where r

@@ -211,6 +211,24 @@ def test_top_of_narrow_rows(lm, rows, v):
             assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("value", [-7.5, 0.0, 3.0])
+def test_top_of_rows_of_few_values(lm, value):
+    """Rows in parts whose lists all end in the same value: of equal ones the
+    first by index, below and above 0."""
+    torch, hiplm = lm
+    g = torch.Generator().manual_seed(4)
+    x = torch.full((3, 131072), value)
+    x[1, torch.randint(131072, (70,), generator=g)] = value + 1
+    x[2] += torch.randint(0, 2, (131072,), generator=g)
+    tokens = torch.zeros(3, dtype=torch.long, device="cuda")
+    want = x.sort(dim=-1, descending=True, stable=True)[1]
+    for dtype in DTYPES:
+        for top in (1, 20, 100, 128):
+            r = hiplm.token_logprobs(x.to(getattr(torch, dtype)).cuda(),
+                                     tokens, top=top)
+            assert torch.equal(r.top_tokens.cpu(), want[:, :top])
+
+
 @pytest.mark.parametrize("rows", [1, 500])
 def test_top_of_rows_with_nan(lm, rows):
     """Numbers are chosen from what is one, also where some of a block's
