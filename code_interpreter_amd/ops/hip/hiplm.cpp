@@ -151,15 +151,17 @@ Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
 // rows of logits
 // ---------------------------------------------------------------------------
 // A gradient of a gradient is not computed. Where the backward itself is
-// recorded, its result answers with an error when one is asked for.
-Tensor once(const Tensor& dx, const variable_list& grads) {
+// recorded, its result is a node's that answers with an error when it is
+// differentiated: by the logits or the gradients that came in, so that it
+// stands on the way to either, where torch would leave out a node beside it.
+Tensor once(const Tensor& dx, const Tensor& logits,
+            const variable_list& grads) {
   if (!at::GradMode::is_enabled()) return dx;
-  bool recorded = false;
-  for (const Tensor& g : grads) recorded |= g.defined() && g.requires_grad();
-  if (!recorded) return dx;
+  variable_list of{dx, logits};
+  of.insert(of.end(), grads.begin(), grads.end());
   auto error = std::make_shared<torch::autograd::DelayedError>(
-      "this operator has no second derivative", 1);
-  return (*error)({dx.detach().requires_grad_()})[0];
+      "this operator has no second derivative", (int64_t)of.size());
+  return (*error)(std::move(of))[0];
 }
 
 struct Scores {
@@ -205,11 +207,11 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(7);
     if (!grads[0].defined() && !grads[1].defined()) return result;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
     Tensor dx;
     {
       at::NoGradGuard no_grad;
-      auto saved = ctx->get_saved_variables();
-      const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
@@ -224,7 +226,7 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
             dx.data_ptr(), on.stream);
       }
     }
-    result[0] = once(dx, grads);
+    result[0] = once(dx, logits, grads);
     return result;
   }
 };
@@ -277,11 +279,11 @@ class Distill : public torch::autograd::Function<Distill> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(7);
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &ids = saved[1], &kept = saved[2];
     Tensor dx;
     {
       at::NoGradGuard no_grad;
-      auto saved = ctx->get_saved_variables();
-      const Tensor &logits = saved[0], &ids = saved[1], &kept = saved[2];
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
@@ -300,7 +302,7 @@ class Distill : public torch::autograd::Function<Distill> {
                            on.stream);
       }
     }
-    result[0] = once(dx, grads);
+    result[0] = once(dx, logits, grads);
     return result;
   }
 };

@@ -17,7 +17,8 @@ are -inf (or very low) logits.
 
 GPU tensors run on the kernels, on torch's current stream of their device,
 and raise where the extension is missing; CPU tensors are computed in plain
-torch. Second derivatives are refused.
+torch. Kernels have no second derivative: differentiating a gradient raises a
+RuntimeError.
 """
 
 from collections import namedtuple

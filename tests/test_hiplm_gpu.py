@@ -682,3 +682,41 @@ def test_forward_mode_is_refused(lm):
                      lambda: hipmx.linear(dual, w)):
             with pytest.raises(RuntimeError, match="jvp|forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("op", ["logprobs", "entropy", "distill"])
+@pytest.mark.parametrize("leaf", [True, False])
+def test_a_gradient_penalty_is_refused(lm, op, leaf):
+    """A second derivative, also where the first one's incoming gradient is a
+    constant and the rest of the loss has a graph of its own: an error, no
+    gradient that lacks a term. The first derivative is the same as ever."""
+    torch, hiplm = lm
+    g = torch.Generator(device="cuda").manual_seed(6)
+    h = torch.randn(4, 8, generator=g, device="cuda", requires_grad=True)
+    w = torch.randn(8, 50, generator=g, device="cuda")
+    ids = torch.arange(8, device="cuda").reshape(4, 2)
+    teacher = torch.randn(4, 2, generator=g, device="cuda")
+
+    def loss_of(z):
+        if op == "distill":
+            return hiplm.topk_distill_loss(z, teacher, ids)
+        return getattr(hiplm.token_logprobs(z, ids[:, 0]), op).sum()
+
+    x = (h @ w).detach().requires_grad_(True) if leaf else h
+    logits = x if leaf else h @ w
+    loss = loss_of(logits)
+    (grad,) = torch.autograd.grad(loss, [x], create_graph=True)
+    first = loss_of(x if leaf else h @ w)
+    (plain,) = torch.autograd.grad(first, [x])
+    assert torch.equal(grad.detach(), plain)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (loss + grad.pow(2).sum()).backward(retain_graph=True)
+    # by some of the leaves only: torch runs what is on the way to them
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(loss + grad.pow(2).sum(), [x])
+    # an incoming gradient that has a graph itself
+    weight = torch.ones((), device="cuda", requires_grad=True)
+    loss = loss_of(x if leaf else h @ w)
+    (grad,) = torch.autograd.grad(loss, [x], weight, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(grad.sum(), [weight])
