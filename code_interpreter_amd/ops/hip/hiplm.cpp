@@ -88,9 +88,19 @@ Tensor bytes(const Tensor& like, int64_t size) {
   return size ? empty(like, {size}, at::kByte) : Tensor();
 }
 
+// A fake tensor and a subclass that wraps others have sizes and a device, but
+// no memory. By the storage's address: a tensor's adds its offset.
+void check_memory(const Tensor& t) {
+  TORCH_CHECK_TYPE(t.has_storage() && (!t.numel() || t.storage().data()),
+                   "a tensor with memory of its own is wanted, which a fake "
+                   "tensor or a wrapper of others does not have");
+}
+
 template <class T = float>
 T* data(const Tensor& t) {
-  return t.defined() ? (T*)t.data_ptr() : nullptr;
+  if (!t.defined()) return nullptr;
+  check_memory(t);
+  return (T*)t.data_ptr();
 }
 
 // ---------------------------------------------------------------------------
@@ -103,7 +113,7 @@ std::pair<Tensor, Tensor> quantize(const Tensor& x, int64_t code) {
   Tensor scales = empty(x, with_last(lead(x), nb), at::kByte);
   if (r.rows) {
     Launch on(x);
-    launch_mx_quantize((LmType)code, r.x.data_ptr(), r.stride,
+    launch_mx_quantize((LmType)code, data<void>(r.x), r.stride,
                        data<uint8_t>(codes), data<uint8_t>(scales), r.rows,
                        r.v, on.stream);
   }
@@ -116,7 +126,7 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t k,
   if (out.numel()) {
     Launch on(codes);
     launch_mx_dequantize((LmType)code, data<uint8_t>(codes),
-                         data<uint8_t>(scales), out.data_ptr(),
+                         data<uint8_t>(scales), data<void>(out),
                          out.numel() / k, k, on.stream);
   }
   return out;
@@ -136,13 +146,13 @@ Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
   if (packed) {
     launch_mx_linear((LmType)code, nullptr, 0, data<uint8_t>(x),
                      data<uint8_t>(xs), data<uint8_t>(wc), data<uint8_t>(ws),
-                     data<void>(b), y.data_ptr(), m, n, k, data<void>(work),
+                     data<void>(b), data<void>(y), m, n, k, data<void>(work),
                      on.stream);
   } else {
     Rows r(x);
-    launch_mx_linear((LmType)code, r.x.data_ptr(), r.stride, nullptr, nullptr,
+    launch_mx_linear((LmType)code, data<void>(r.x), r.stride, nullptr, nullptr,
                      data<uint8_t>(wc), data<uint8_t>(ws), data<void>(b),
-                     y.data_ptr(), m, n, k, data<void>(work), on.stream);
+                     data<void>(y), m, n, k, data<void>(work), on.stream);
   }
   return y;
 }
@@ -180,7 +190,7 @@ Scores score(const Tensor& logits, const Tensor& tokens, const Tensor& top_lp,
   if (r.rows) {
     Launch on(logits);
     Tensor work = bytes(logits, score_workspace(t, r.rows, r.v, top));
-    launch_token_logprobs(t, r.x.data_ptr(), r.stride, r.rows, r.v,
+    launch_token_logprobs(t, data<void>(r.x), r.stride, r.rows, r.v,
                           data<int64_t>(tokens), ignore, (float)inv_t, top,
                           data(s.logprobs), data(s.entropy), data(top_lp),
                           data<int64_t>(top_ids), data<RowStats>(s.stats),
@@ -219,11 +229,11 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
         const Tensor g_h = grads[1].defined() ? plain(grads[1]) : Tensor();
         Launch on(logits);
         launch_token_logprobs_bwd(
-            (LmType)ctx->saved_data["code"].toInt(), r.x.data_ptr(), r.stride,
+            (LmType)ctx->saved_data["code"].toInt(), data<void>(r.x), r.stride,
             r.rows, r.v, data<int64_t>(tokens),
             (float)ctx->saved_data["inv_t"].toDouble(),
             data<RowStats>(stats), data(g_lp), data(g_h),
-            dx.data_ptr(), on.stream);
+            data<void>(dx), on.stream);
       }
     }
     result[0] = once(dx, logits, grads);
@@ -255,8 +265,8 @@ Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
   float* count = how ? q + r.rows * k : nullptr;
   Launch on(logits);
   Tensor work = bytes(logits, score_workspace(t, r.rows, r.v, 0));
-  launch_distill(t, r.x.data_ptr(), r.stride, r.rows, r.v,
-                 (LmType)teacher_code, record.data_ptr(), data<int64_t>(ids),
+  launch_distill(t, data<void>(r.x), r.stride, r.rows, r.v,
+                 (LmType)teacher_code, data<void>(record), data<int64_t>(ids),
                  (int)k, (float)inv_t, how ? count + 1 : data(l.loss), q,
                  (RowStats*)stats, how ? data(l.loss) : nullptr, count,
                  how == 2, data<void>(work), on.stream);
@@ -294,11 +304,11 @@ class Distill : public torch::autograd::Function<Distill> {
         const float* q = stats + 4 * r.rows;
         Launch on(logits);
         launch_distill_bwd((LmType)ctx->saved_data["code"].toInt(),
-                           r.x.data_ptr(), r.stride, r.rows, r.v,
+                           data<void>(r.x), r.stride, r.rows, r.v,
                            data<int64_t>(ids), q, (int)k,
                            (float)ctx->saved_data["inv_t"].toDouble(),
                            (const RowStats*)stats, data(grad), whole ? 0 : 1,
-                           whole ? q + r.rows * k : nullptr, dx.data_ptr(),
+                           whole ? q + r.rows * k : nullptr, data<void>(dx),
                            on.stream);
       }
     }
@@ -318,7 +328,9 @@ class Args {
   }
   const Tensor& tensor() {
     TORCH_CHECK_TYPE(THPVariable_Check(*args_), "a tensor is wanted");
-    return THPVariable_Unpack(*args_++);
+    const Tensor& t = THPVariable_Unpack(*args_++);
+    check_memory(t);
+    return t;
   }
   Tensor tensor_or_none() {
     if (*args_ != Py_None) return tensor();

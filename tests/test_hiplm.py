@@ -221,3 +221,57 @@ def test_a_head_records_and_a_student_learns():
         "mean")
     want = dz.T @ x.double().numpy()
     np.testing.assert_allclose(grad.numpy(), want, atol=1e-5)
+
+
+class Wrapper(torch.Tensor):
+    """Has a type, sizes and a device, and no memory, as distributed tensors
+    have none."""
+
+    @staticmethod
+    def __new__(cls, like, device="cuda"):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, like.shape, strides=like.stride(), storage_offset=8,
+            dtype=like.dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+def fake(like):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        return torch.empty(like.shape, dtype=like.dtype, device="cuda")
+
+
+@pytest.mark.parametrize("make", [Wrapper, fake])
+def test_tensors_without_memory_are_refused(make):
+    """Before anything is launched: here no GPU is needed to see it."""
+    pytest.importorskip("_hiplm")
+    x, ids = make(torch.randn(3, 64)), make(torch.zeros(3, 2).long())
+    one = make(torch.zeros(3).long())
+    codes = make(torch.zeros(5, 32, dtype=torch.uint8))
+    scales = make(torch.zeros(5, 2, dtype=torch.uint8))
+    module = hiplm.hiptorch.ensure_hiplm()
+    for call in (
+        lambda: hiplm.token_logprobs(x, one, top=2),
+        lambda: hiplm.topk_distill_loss(x, make(torch.zeros(3, 2)), ids),
+        lambda: hipmx.quantize(x),
+        lambda: module.mx_dequantize(codes, scales, 64, 0),
+        lambda: module.mx_linear(x, None, codes, scales, None, 64, 0),
+    ):
+        with pytest.raises(TypeError, match="memory of its own"):
+            call()
+
+
+def test_batched_tensors_are_refused():
+    """vmap's tensors have no memory either, at the kernels' entry."""
+    module = pytest.importorskip("_hiplm")
+    for call in (
+        lambda x: module.mx_quantize(x, 0),
+        lambda x: module.token_logprobs(x, torch.zeros(3).long(), 0, 0, 1.0,
+                                        -100),
+    ):
+        with pytest.raises(TypeError, match="memory of its own"):
+            torch.vmap(call)(torch.randn(2, 3, 64))

@@ -720,3 +720,28 @@ def test_a_gradient_penalty_is_refused(lm, op, leaf):
     (grad,) = torch.autograd.grad(loss, [x], weight, create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(grad.sum(), [weight])
+
+
+def test_gradients_without_memory_are_refused(lm):
+    """An incoming gradient that wraps others, as a distributed tensor's."""
+    torch, hiplm = lm
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, like):
+            return torch.Tensor._make_wrapper_subclass(
+                cls, like.shape, dtype=like.dtype, device=like.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise TypeError(str(func))
+
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    ids = torch.zeros(3, 2, dtype=torch.long, device="cuda")
+    outs = [*hiplm.token_logprobs(x, ids[:, 0])[:2],
+            hiplm.topk_distill_loss(x, torch.zeros(3, 2, device="cuda"), ids)]
+    for out in outs:
+        with pytest.raises((TypeError, RuntimeError)):
+            torch.autograd.grad(out, [x], Wrapper(out))
+    with pytest.raises(TypeError, match="memory of its own"):
+        hiplm.token_logprobs(Wrapper(x), ids[:, 0])
