@@ -158,30 +158,39 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
 # ---------------------------------------------------------------------------
 # CPU tensors
 # ---------------------------------------------------------------------------
-def _cpu_log_softmax(torch, logits, t):
-    """ln softmax in float32, and which rows are masked as a whole (their
+def _cpu_log_softmax(torch, logits, t, without):
+    """ln softmax in float32 of rows but those `without` a result (their
     numbers are of no use, but no NaN either). The largest logit is taken off
     before the division: a lowest value divided would be an infinity."""
-    z = logits.float()
-    empty = (z == -math.inf).all(-1)
-    z = torch.where(empty[..., None], 0.0, z)
+    z = torch.where(without[..., None], 0.0, logits.float())
     z = z - z.detach().amax(-1, keepdim=True)
-    return torch.log_softmax(z / t, -1), empty
+    return torch.log_softmax(z / t, -1)
+
+
+def _cpu_empty(logits):
+    """Rows that are masked as a whole."""
+    return (logits.detach() == -math.inf).all(-1)
+
+
+def _cpu_wrong(torch, rows, o):
+    """o, with NaN in the given rows, and in their gradients."""
+    return o * torch.where(rows, math.nan, 1.0)
 
 
 def _cpu_token_logprobs(torch, logits, tokens, top, t, ignore):
     v = logits.shape[-1]
-    lp, empty = _cpu_log_softmax(torch, logits, t)
     ignored = tokens == ignore
     outside = ~ignored & ((tokens < 0) | (tokens >= v))
+    empty = _cpu_empty(logits) & ~outside
+    lp = _cpu_log_softmax(torch, logits, t, empty | ignored)
     at = tokens.clamp(0, v - 1)[..., None]
-    nan, zero = math.nan, 0.0
+    zero = 0.0
     logprobs = lp.gather(-1, at)[..., 0]
     logprobs = torch.where(empty, -math.inf, logprobs)
     entropy = -(lp.exp() * lp.clamp(min=-1e4)).sum(-1)
     entropy = torch.where(empty, zero, entropy)
     logprobs, entropy = (
-        torch.where(ignored, zero, torch.where(outside, nan, o))
+        torch.where(ignored, zero, _cpu_wrong(torch, outside, o))
         for o in (logprobs, entropy))
     with torch.no_grad():
         z = logits.float()
@@ -196,23 +205,23 @@ def _cpu_token_logprobs(torch, logits, tokens, top, t, ignore):
 
 def _cpu_distill(torch, logits, teacher, ids, t, reduction):
     v = logits.shape[-1]
-    lp, empty = _cpu_log_softmax(torch, logits, t)
     z = teacher.float()
     there = (ids != -1) & (z != -math.inf)
     bad = there & (z.isnan() | (z == math.inf) | (ids < 0) | (ids >= v))
     absent = ~there.any(-1)
+    wrong = bad.any(-1)
+    empty = _cpu_empty(logits) & ~wrong
+    lp = _cpu_log_softmax(torch, logits, t, empty | absent)
     z = torch.where(there & ~bad, z, -math.inf)
-    lq, _ = _cpu_log_softmax(torch, z, t)
+    lq = _cpu_log_softmax(torch, z, t, _cpu_empty(z))
     # a share of 0 adds nothing, whatever the student gives it
     there = there & (lq.exp() > 0)
-    lp = torch.where(empty[..., None], lp.detach(), lp)
     mine = lp.gather(-1, ids.clamp(0, v - 1))
     mine = torch.where(empty[..., None], -math.inf, mine)
     mine = torch.where(there, mine, 0.0)
     loss = (torch.where(there, lq.exp() * lq, 0.0)
             - torch.where(there, lq.exp() * mine, 0.0)).sum(-1) * (t * t)
-    loss = torch.where(absent, 0.0, loss)
-    loss = torch.where(bad.any(-1), math.nan, loss)
+    loss = torch.where(absent, 0.0, _cpu_wrong(torch, wrong, loss))
     if reduction == "none":
         return loss
     total = loss.sum()

@@ -275,3 +275,64 @@ def test_batched_tensors_are_refused():
     ):
         with pytest.raises(TypeError, match="memory of its own"):
             torch.vmap(call)(torch.randn(2, 3, 64))
+
+
+def garbage(v):
+    """Rows of trouble, and padded rows and wholly masked ones that hold or
+    are given what is wrong."""
+    x, tokens = rows_with_trouble(v)
+    more = x[:6].clone()
+    more[0, v // 2] = NAN
+    more[1, 0] = INF
+    more[2] = NAN
+    more[3] = -INF
+    more[4] = -INF
+    tokens = torch.cat([tokens, torch.tensor([-100, -100, -100, -100, v, -3])])
+    return torch.cat([x, more]), tokens
+
+
+@pytest.mark.parametrize("use", ["both", "logprobs", "entropy"])
+@pytest.mark.parametrize("v", [1, 7, 300])
+def test_gradients_of_wrong_and_padded_rows(v, use):
+    """Padding gets no gradient, whatever stands in it; a token outside of
+    the vocabulary and a NaN give NaN gradients, as on the kernels."""
+    x, tokens = garbage(v)
+    x = x.requires_grad_(True)
+    r = hiplm.token_logprobs(x, tokens, temperature=0.7)
+    g = torch.Generator().manual_seed(v)
+    gs = {name: torch.randn(len(x), generator=g) * (use in ("both", name))
+          for name in ("logprobs", "entropy")}
+    (grad,) = torch.autograd.grad(
+        [getattr(r, name) for name in gs], [x], list(gs.values()))
+    want, size = oracle.token_logprobs_grad(
+        x.detach().double().numpy(), tokens.numpy(), 0.7,
+        *(o.double().numpy() for o in gs.values()))
+    check(grad, want, 2.0 ** -17 * size + 1e-30)
+    lp, h, _, _ = oracle.token_logprobs(
+        x.detach().double().numpy(), tokens.numpy(), 0, 0.7)
+    check(r.logprobs, lp, 2.0 ** -18 * (
+        1 + np.abs(np.where(np.isfinite(lp), lp, 0))))
+    check(r.entropy, h, 2.0 ** -18 * (1 + math.log(v)))
+
+
+@pytest.mark.parametrize("v,k", [(1, 1), (9, 4), (300, 8)])
+def test_distill_gradients_of_wrong_and_padded_rows(v, k):
+    """The same of distillation: a row without a record has no gradient,
+    whatever its logits; a bad entry gives its row NaN gradients."""
+    x, _ = garbage(v)
+    teacher, ids = records(v, k, rows=18)
+    ids[[8, 12, 14]] = -1         # without a record: NaN in the logits,
+    teacher[[9, 13]] = -INF       # and an infinity
+    ids[16, k - 1] = v + 5        # bad: the row is masked as a whole,
+    teacher[17] = NAN             # and all of its entries are
+    x = x.requires_grad_(True)
+    loss = hiplm.topk_distill_loss(x, teacher, ids, temperature=1.5,
+                                   reduction="none")
+    want, grad, size = oracle.distill(
+        x.detach().double().numpy(), teacher.double().numpy(), ids.numpy(),
+        1.5, "none")
+    check(loss, want, 2.0 ** -16 * (
+        1 + np.abs(np.where(np.isfinite(want), want, 0))))
+    (got,) = torch.autograd.grad(loss.sum(), [x])
+    rows = ~np.isposinf(want)  # those with a masked entry are tested elsewhere
+    check(got[rows], grad[rows], 2.0 ** -16 * size[rows] + 1e-30)
