@@ -577,8 +577,9 @@ struct Record {
 };
 
 // a row by a wave: the teacher's softmax over its record, and
-// T^2 sum q (ln q - ln p). Returns (in every lane) the loss, and whether the
-// row has a record.
+// T^2 sum q (ln q - ln p). The logarithms are kept in units of 1 / T, so that a
+// recorded logit of the type's lowest value overflows only where the loss does.
+// Returns (in every lane) the loss, and whether the row has a record.
 struct RowLoss {
   float loss;
   bool there;
@@ -612,20 +613,22 @@ __device__ RowLoss distill_row(int64_t row, Record<T> rec, int64_t v,
     sum += id[i] != -1 ? exp2_raw((z[i] - top) * c) : 0.f;
   sum = wave_sum(sum);
   const float log2_q = log2f(sum);
+  const float temp = 1.f / e.inv_t;
+  const float log_q = log2_q * kLn2 * temp, log_p = log2_sum * kLn2 * temp;
   float loss = 0.f;
 #pragma unroll
   for (int i = 0; i < kMine; i++) {
     int at = lane + 64 * i;
     float share = 0.f;
     if (id[i] != -1 && !bad) {
-      float lq = (z[i] - top) * c - log2_q;
-      share = exp2_raw(lq);
-      float lp = empty ? -INFINITY : (rec.x[i] - t.m) * c - log2_sum;
+      share = exp2_raw((z[i] - top) * c - log2_q);
+      float lq = z[i] - top - log_q;
+      float lp = empty ? -INFINITY : rec.x[i] - t.m - log_p;
       if (share > 0.f) loss = fmaf(share, lq - lp, loss);
     }
     if (at < e.k) e.q[row * e.k + at] = share;
   }
-  loss = wave_sum(loss) * (kLn2 / (e.inv_t * e.inv_t));
+  loss = wave_sum(loss) * temp;
   loss = absent ? 0.f : bad ? NAN : loss;
   if (lane == 0) {
     e.row_loss[row] = loss;

@@ -158,13 +158,12 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
 # ---------------------------------------------------------------------------
 # CPU tensors
 # ---------------------------------------------------------------------------
-def _cpu_log_softmax(torch, logits, t, without):
-    """ln softmax in float32 of rows but those `without` a result (their
-    numbers are of no use, but no NaN either). The largest logit is taken off
-    before the division: a lowest value divided would be an infinity."""
+def _cpu_shifted(torch, logits, without):
+    """Rows in float32 less their largest logit: divided by a temperature
+    before that, a lowest value would be an infinity. Of rows `without` a
+    result the numbers are of no use, but no NaN either."""
     z = torch.where(without[..., None], 0.0, logits.float())
-    z = z - z.detach().amax(-1, keepdim=True)
-    return torch.log_softmax(z / t, -1)
+    return z - z.detach().amax(-1, keepdim=True)
 
 
 def _cpu_empty(logits):
@@ -182,7 +181,8 @@ def _cpu_token_logprobs(torch, logits, tokens, top, t, ignore):
     ignored = tokens == ignore
     outside = ~ignored & ((tokens < 0) | (tokens >= v))
     empty = _cpu_empty(logits) & ~outside
-    lp = _cpu_log_softmax(torch, logits, t, empty | ignored)
+    lp = torch.log_softmax(
+        _cpu_shifted(torch, logits, empty | ignored) / t, -1)
     at = tokens.clamp(0, v - 1)[..., None]
     zero = 0.0
     logprobs = lp.gather(-1, at)[..., 0]
@@ -211,16 +211,21 @@ def _cpu_distill(torch, logits, teacher, ids, t, reduction):
     absent = ~there.any(-1)
     wrong = bad.any(-1)
     empty = _cpu_empty(logits) & ~wrong
-    lp = _cpu_log_softmax(torch, logits, t, empty | absent)
+    # logarithms in units of 1 / t, so that a lowest value that is recorded
+    # overflows only where the loss does
+    x = _cpu_shifted(torch, logits, empty | absent)
+    lse = torch.logsumexp(x / t, -1, keepdim=True) * t
     z = torch.where(there & ~bad, z, -math.inf)
-    lq = _cpu_log_softmax(torch, z, t, _cpu_empty(z))
+    z = _cpu_shifted(torch, z, _cpu_empty(z))
+    q = torch.softmax(z / t, -1)
+    lq = z - torch.logsumexp(z / t, -1, keepdim=True) * t
     # a share of 0 adds nothing, whatever the student gives it
-    there = there & (lq.exp() > 0)
-    mine = lp.gather(-1, ids.clamp(0, v - 1))
+    there = there & (q > 0)
+    mine = x.gather(-1, ids.clamp(0, v - 1)) - lse
     mine = torch.where(empty[..., None], -math.inf, mine)
     mine = torch.where(there, mine, 0.0)
-    loss = (torch.where(there, lq.exp() * lq, 0.0)
-            - torch.where(there, lq.exp() * mine, 0.0)).sum(-1) * (t * t)
+    loss = (torch.where(there, q * lq, 0.0)
+            - torch.where(there, q * mine, 0.0)).sum(-1) * t
     loss = torch.where(absent, 0.0, _cpu_wrong(torch, wrong, loss))
     if reduction == "none":
         return loss

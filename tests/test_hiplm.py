@@ -336,3 +336,38 @@ def test_distill_gradients_of_wrong_and_padded_rows(v, k):
     (got,) = torch.autograd.grad(loss.sum(), [x])
     rows = ~np.isposinf(want)  # those with a masked entry are tested elsewhere
     check(got[rows], grad[rows], 2.0 ** -16 * size[rows] + 1e-30)
+
+
+def lowest_in_record(v, dtype):
+    """A student that gives the type's lowest value to tokens with a share of
+    the record, next to ordinary ones."""
+    g = torch.Generator().manual_seed(v)
+    x = torch.randn(6, v, generator=g).to(dtype)
+    teacher = torch.randn(6, 4, generator=g)
+    ids = torch.stack([torch.randperm(v, generator=g)[:4] for _ in range(6)])
+    for i in range(1, 6):
+        x[i, ids[i, :1 + i // 2]] = torch.finfo(dtype).min
+    return x, teacher, ids
+
+
+# a share is off by its exponent's rounding and scale, 5 steps of at most 16,
+# and its own; what it is multiplied with and added to by a few steps: relative
+# to a loss that these entries make up at most 128 steps
+LOWEST = 128 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("t", [0.3, 0.5, 1.0, 1.5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_of_lowest_logits_is_finite(dtype, t):
+    x, teacher, ids = lowest_in_record(50, dtype)
+    x = x.requires_grad_(True)
+    loss = hiplm.topk_distill_loss(x, teacher, ids, temperature=t,
+                                   reduction="none")
+    want, grad, size = oracle.distill(
+        x.detach().double().numpy(), teacher.double().numpy(), ids.numpy(),
+        t, "none")
+    check(loss, want, LOWEST * (1 + np.abs(want)))
+    (got,) = torch.autograd.grad(loss.sum(), [x])
+    # one rounding to the type
+    check(got, grad, 2.0 ** -16 * size + 1e-30
+          + torch.finfo(dtype).eps / 2 * np.abs(grad))

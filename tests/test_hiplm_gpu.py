@@ -745,3 +745,51 @@ def test_gradients_without_memory_are_refused(lm):
             torch.autograd.grad(out, [x], Wrapper(out))
     with pytest.raises(TypeError, match="memory of its own"):
         hiplm.token_logprobs(Wrapper(x), ids[:, 0])
+
+
+@pytest.mark.parametrize("v", [1, 7, 300, 20000])
+def test_kernels_and_host_agree_on_wrong_rows(lm, v):
+    """Padding that holds NaN, tokens outside of the vocabulary, bad records,
+    rows that are masked as a whole: what is NaN, 0 and infinite is so on GPU
+    and CPU tensors alike, in results and gradients."""
+    torch, hiplm = lm
+    import test_hiplm as on_host
+
+    x, tokens = on_host.garbage(v)
+    k = min(v, 4)
+    teacher, ids = on_host.records(v, k, rows=18)
+    ids[[8, 12, 14]] = -1
+    teacher[[9, 13]] = -INF
+    ids[16, k - 1] = v + 5
+    teacher[17] = math.nan
+    results = []
+    for device in ("cpu", "cuda"):
+        z = x.to(device).requires_grad_(True)
+        r = hiplm.token_logprobs(z, tokens.to(device), top=min(v, 3))
+        (g,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), [z])
+        loss = hiplm.topk_distill_loss(z, teacher.to(device), ids.to(device),
+                                       reduction="none")
+        (d,) = torch.autograd.grad(loss, [z], torch.ones_like(loss))
+        results.append([t.detach().cpu() for t in (*r, g, loss, d)])
+    for a, b in zip(*results):
+        # NaN where the other has one, infinities and exact zeros of rows too
+        torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-3, equal_nan=True)
+    for i in (3, 6):  # the gradients
+        none = [(t[i] == 0).all(-1) for t in results]
+        assert torch.equal(*none)
+
+
+@pytest.mark.parametrize("t", [0.3, 0.5, 1.0, 1.5])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("v", [50, 70001])
+def test_distill_of_lowest_logits_is_finite(lm, dtype, t, v):
+    torch, hiplm = lm
+    import lm_oracle as oracle
+    import test_hiplm as on_host
+
+    x, teacher, ids = on_host.lowest_in_record(v, getattr(torch, dtype))
+    loss = hiplm.topk_distill_loss(x.cuda(), teacher.cuda(), ids.cuda(),
+                                   temperature=t, reduction="none")
+    want, _, _ = oracle.distill(
+        x.double().numpy(), teacher.double().numpy(), ids.numpy(), t, "none")
+    near(loss, want, (on_host.LOWEST + relative(v)) * (1 + np.abs(want)))
