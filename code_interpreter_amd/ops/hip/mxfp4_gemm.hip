@@ -593,11 +593,11 @@ __global__ __launch_bounds__(WM* WN* WK * 64) void small_kernel(
 #pragma unroll
   for (int t = 0; t < kStages - 1; t++) stage(min(t, steps - 1), t);
   auto arrive = [] {
-    // this wave's loads of a step have landed; behind the barrier every
-    // wave's, and the step before is read
+    // this wave's loads of a step have landed, and its reads of the step
+    // before are done; behind the barrier every wave's
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((kWait & 15) | 7 << 4 | 15 << 8 |
-                               (kWait >> 4) << 14);
+    __builtin_amdgcn_s_waitcnt((kWait & 15) | 7 << 4 |
+                               (kWait >> 4) << 14);  // and lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };

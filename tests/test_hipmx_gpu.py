@@ -420,3 +420,19 @@ def test_linear_wide(mx, m, n, k):
     x, w, bias = operands(torch, hipmx, m, n, k, "bfloat16", m + n + k)
     check_linear(torch, hipmx, hipmx.linear(x, w, bias), x, w, bias)
     check_linear(torch, hipmx, hipmx.linear(hipmx.quantize(x), w), x, w, None)
+
+
+@pytest.mark.parametrize("m,n", [(333, 5001), (200, 4096), (100, 4096),
+                                 (40, 100)])
+@pytest.mark.parametrize("k", [8192, 8288])
+def test_linear_rings_go_round(mx, m, n, k):
+    """Each of the small tiles, long enough that its buffers are filled many
+    times over what was read before."""
+    torch, hipmx = mx
+    x, w, bias = operands(torch, hipmx, m, n, k, "bfloat16", m)
+    y = hipmx.linear(x, w, bias)
+    check_linear(torch, hipmx, y, x, w, bias)
+    q = hipmx.quantize(x)
+    for _ in range(8):
+        assert torch.equal(hipmx.linear(x, w, bias), y)
+        check_linear(torch, hipmx, hipmx.linear(q, w, bias), x, w, bias)
