@@ -64,15 +64,23 @@ def _needs(output: Path, sources) -> bool:
     return any(p.stat().st_mtime > out_mtime for p in deps)
 
 
-def needs_build() -> bool:
-    return any(_needs(out, sources) for out, sources in MODULES)
-
-
-def _torch_dir() -> Path:
+def _torch_dir() -> Path | None:
+    """Where torch for ROCm is, if it is here."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise RuntimeError("_hiplm is built against torch, which is not here")
-    return Path(spec.submodule_search_locations[0])
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    path = Path(spec.submodule_search_locations[0])
+    return path if (path / "lib" / "libtorch_hip.so").exists() else None
+
+
+def _buildable(sources) -> bool:
+    """What takes torch's tensors is of use, and built, only next to it."""
+    return TORCH_SOURCES.isdisjoint(sources) or _torch_dir() is not None
+
+
+def needs_build() -> bool:
+    return any(_needs(out, sources) for out, sources in MODULES
+               if _buildable(sources))
 
 
 def _run(cmd, verbose: bool) -> None:
@@ -128,7 +136,10 @@ def _compile(output: Path, sources, verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = True) -> Path:
     for out, sources in MODULES:
-        if force or _needs(out, sources):
+        if not _buildable(sources):
+            print(f"{out.name} is not built: there is no torch for ROCm here",
+                  flush=True)
+        elif force or _needs(out, sources):
             _compile(out, sources, verbose)
     return OUTPUT
 
