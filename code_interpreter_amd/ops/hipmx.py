@@ -223,8 +223,8 @@ def _cpu_quantize(torch, x):
     # a code is its place among the values; the border between two codes
     # falls to the even one
     borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0],
-                           dtype=a.dtype)
-    even_above = torch.tensor([False, True] * 3 + [False])
+                           dtype=a.dtype, device=a.device)
+    even_above = torch.tensor([False, True] * 3 + [False], device=a.device)
     code = ((a[..., None] > borders)
             | ((a[..., None] == borders) & even_above)).sum(-1)
     code = code + 8 * (torch.signbit(v) & good)
@@ -235,7 +235,8 @@ def _cpu_quantize(torch, x):
 
 
 def _cpu_dequantize(torch, q):
-    table = torch.tensor(_VALUES + [-f for f in _VALUES])
+    table = torch.tensor(_VALUES + [-f for f in _VALUES],
+                         dtype=torch.float32, device=q.device)
     v = torch.stack([table[(q.codes & 15).long()],
                      table[(q.codes >> 4).long()]], -1)
     v = v.reshape(*q.scales.shape, BLOCK)

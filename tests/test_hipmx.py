@@ -197,3 +197,22 @@ def test_parts_are_not_replaced():
             setattr(q, name, getattr(q, name))
     again = copy.deepcopy(q)
     assert torch.equal(again.codes, q.codes) and again.shape == q.shape
+
+
+def test_another_default_device_and_type():
+    """torch's defaults are for tensors that a program makes, not for these
+    operators' tables."""
+    x = edges(torch.float32)
+    w = hipmx.quantize(x)
+    y = hipmx.linear(x, w)
+    torch.set_default_device("meta")
+    torch.set_default_dtype(torch.float16)
+    try:
+        q = hipmx.quantize(x)
+        v, z = q.dequantize(torch.float32), hipmx.linear(x, w)
+    finally:
+        torch.set_default_device(None)
+        torch.set_default_dtype(torch.float32)
+    assert torch.equal(q.codes, w.codes) and torch.equal(q.scales, w.scales)
+    assert torch.equal(v, w.dequantize(torch.float32))
+    assert torch.equal(z, y)
