@@ -174,6 +174,15 @@ Tensor once(const Tensor& dx, const Tensor& logits,
   return (*error)(std::move(of))[0];
 }
 
+// A saved tensor comes back through hooks that a program may have set, which
+// can make it anything: the kernels want what was saved.
+void check_saved(const Tensor& t, const Tensor& grad, at::ScalarType type,
+                 bool fits) {
+  TORCH_CHECK(fits && t.device() == grad.device() && t.scalar_type() == type,
+              "a saved tensor came back with another size, type or device "
+              "than it was saved with");
+}
+
 struct Scores {
   Tensor logprobs, entropy, stats;
 };
@@ -218,10 +227,18 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
     variable_list result(7);
     if (!grads[0].defined() && !grads[1].defined()) return result;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
+    const Tensor &logits = saved[0], &grad = grads[grads[0].defined() ? 0 : 1];
+    const int64_t code = ctx->saved_data["code"].toInt();
+    check_saved(logits, grad, scalar_type(code),
+                logits.dim() && logits.size(-1) &&
+                    lead(logits) == grad.sizes());
+    check_saved(saved[1], grad, at::kLong, saved[1].sizes() == grad.sizes());
+    check_saved(saved[2], grad, at::kFloat,
+                saved[2].numel() == 4 * grad.numel());
     Tensor dx;
     {
       at::NoGradGuard no_grad;
+      const Tensor tokens = plain(saved[1]), stats = plain(saved[2]);
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
@@ -229,8 +246,8 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
         const Tensor g_h = grads[1].defined() ? plain(grads[1]) : Tensor();
         Launch on(logits);
         launch_token_logprobs_bwd(
-            (LmType)ctx->saved_data["code"].toInt(), data<void>(r.x), r.stride,
-            r.rows, r.v, data<int64_t>(tokens),
+            (LmType)code, data<void>(r.x), r.stride, r.rows, r.v,
+            data<int64_t>(tokens),
             (float)ctx->saved_data["inv_t"].toDouble(),
             data<RowStats>(stats), data(g_lp), data(g_h),
             data<void>(dx), on.stream);
@@ -247,6 +264,10 @@ struct Loss {
   Tensor loss, kept;
 };
 
+int64_t kept_size(int64_t rows, int64_t k, bool whole) {
+  return rows * (4 + k) + (whole ? 1 + rows : 0);
+}
+
 Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
              int64_t code, int64_t teacher_code, double inv_t, int64_t how) {
   const LmType t = (LmType)code;
@@ -254,8 +275,7 @@ Loss distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids,
   const Tensor record = plain(teacher);
   const int64_t k = ids.size(-1);
   Loss l = {empty(logits, how ? at::IntArrayRef() : lead(logits), at::kFloat),
-            empty(logits, {r.rows * (4 + k) + (how ? 1 + r.rows : 0)},
-                  at::kFloat)};
+            empty(logits, {kept_size(r.rows, k, how != 0)}, at::kFloat)};
   if (!r.rows) {
     l.loss.zero_();
     return l;
@@ -290,22 +310,33 @@ class Distill : public torch::autograd::Function<Distill> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(7);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &ids = saved[1], &kept = saved[2];
+    const Tensor& logits = saved[0];
+    const int64_t code = ctx->saved_data["code"].toInt();
+    const bool whole = ctx->saved_data["whole"].toBool();
+    check_saved(logits, grads[0], scalar_type(code),
+                logits.dim() && logits.size(-1) &&
+                    (whole || lead(logits) == grads[0].sizes()));
+    check_saved(saved[1], grads[0], at::kLong,
+                saved[1].dim() == logits.dim() &&
+                    lead(saved[1]) == lead(logits));
+    const int64_t rows = logits.numel() / logits.size(-1);
+    const int64_t k = saved[1].size(-1);
+    check_saved(saved[2], grads[0], at::kFloat,
+                k >= 1 && k <= kMaxRecord &&
+                    saved[2].numel() == kept_size(rows, k, whole));
     Tensor dx;
     {
       at::NoGradGuard no_grad;
+      const Tensor ids = plain(saved[1]), kept = plain(saved[2]);
       Rows r(logits);
       dx = empty(logits, logits.sizes(), logits.scalar_type());
       if (r.rows) {
         const Tensor grad = plain(grads[0]);
-        const int64_t k = ids.size(-1);
-        const bool whole = ctx->saved_data["whole"].toBool();
         const float* stats = data(kept);
         const float* q = stats + 4 * r.rows;
         Launch on(logits);
-        launch_distill_bwd((LmType)ctx->saved_data["code"].toInt(),
-                           data<void>(r.x), r.stride, r.rows, r.v,
-                           data<int64_t>(ids), q, (int)k,
+        launch_distill_bwd((LmType)code, data<void>(r.x), r.stride, r.rows,
+                           r.v, data<int64_t>(ids), q, (int)k,
                            (float)ctx->saved_data["inv_t"].toDouble(),
                            (const RowStats*)stats, data(grad), whole ? 0 : 1,
                            whole ? q + r.rows * k : nullptr, data<void>(dx),

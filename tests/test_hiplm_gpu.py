@@ -793,3 +793,58 @@ def test_distill_of_lowest_logits_is_finite(lm, dtype, t, v):
     want, _, _ = oracle.distill(
         x.double().numpy(), teacher.double().numpy(), ids.numpy(), t, "none")
     near(loss, want, (on_host.LOWEST + relative(v)) * (1 + np.abs(want)))
+
+
+def test_saved_tensors_through_hooks(lm):
+    """What is kept for the backward may go to the host and back. What comes
+    back as something else is refused before the kernels read it."""
+    torch, hiplm = lm
+    hooks = torch.autograd.graph
+    x = torch.randn(5, 700, device="cuda", requires_grad=True)
+    ids = torch.arange(15, device="cuda").reshape(5, 3)
+    teacher = torch.randn(5, 3, device="cuda")
+    calls = [
+        lambda: hiplm.token_logprobs(x, ids[:, 0], top=2).logprobs.sum(),
+        lambda: hiplm.token_logprobs(x, ids[:, 0], top=2).entropy.sum(),
+        lambda: hiplm.topk_distill_loss(x, teacher, ids),
+        lambda: hiplm.topk_distill_loss(x, teacher, ids,
+                                        reduction="none").sum(),
+    ]
+    changes = [
+        lambda t: t.cpu(),
+        lambda t: t.half() if t.is_floating_point() else t,
+        lambda t: t.int() if t.dtype == torch.int64 else t,
+        lambda t: t[:3],
+        lambda t: t[..., :2],
+        lambda t: t.flatten()[:1],
+        lambda t: t[None],
+    ]
+    for call in calls:
+        (want,) = torch.autograd.grad(call(), [x])
+        with hooks.save_on_cpu():
+            out = call()
+        (got,) = torch.autograd.grad(out, [x])
+        assert torch.equal(got, want)
+        # packed with a stride of their own
+        with hooks.saved_tensors_hooks(
+                lambda t: torch.stack([t, t], -1), lambda t: t[..., 0]):
+            out = call()
+        (got,) = torch.autograd.grad(out, [x])
+        assert torch.equal(got, want)
+        for change in changes:
+            for which in range(3):  # of what an operator keeps
+                count = iter(range(100))
+                with hooks.saved_tensors_hooks(
+                        lambda t: (next(count), t),
+                        lambda p: change(p[1]) if p[0] == which else p[1]):
+                    out = call()
+                kept = next(count)
+                assert kept >= 3
+                try:
+                    (got,) = torch.autograd.grad(out, [x])
+                except RuntimeError as e:
+                    # logits of another vocabulary: their own gradient is
+                    # computed, which torch does not take
+                    assert "came back" in str(e) or "invalid gradient" in str(e)
+                else:  # a change that changed nothing
+                    assert torch.equal(got, want)
