@@ -120,8 +120,24 @@ std::pair<Tensor, Tensor> quantize(const Tensor& x, int64_t code) {
   return {codes, scales};
 }
 
+// The parts of a quantised tensor are tensors, which a program can resize,
+// transpose or point elsewhere in place after they were checked.
+void check_parts(const Tensor& codes, const Tensor& scales, int64_t k) {
+  auto good = [](const Tensor& t) {
+    return t.is_cuda() && t.scalar_type() == at::kByte && t.dim() &&
+           t.is_contiguous();
+  };
+  const int64_t nb = mx_blocks(k);
+  TORCH_CHECK_VALUE(
+      good(codes) && good(scales) && codes.device() == scales.device() &&
+          scales.size(-1) == nb && codes.size(-1) == nb * kMxBytes &&
+          lead(codes) == lead(scales) && (uintptr_t)codes.data_ptr() % 16 == 0,
+      "codes and scales do not fit each other any more");
+}
+
 Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t k,
                   int64_t code) {
+  check_parts(codes, scales, k);
   Tensor out = empty(codes, with_last(lead(scales), k), scalar_type(code));
   if (out.numel()) {
     Launch on(codes);
@@ -136,6 +152,10 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t k,
 Tensor linear(const Tensor& x, const Tensor& xs, const Tensor& wc,
               const Tensor& ws, const Tensor& bias, int64_t k, int64_t code) {
   const bool packed = xs.defined();
+  check_parts(wc, ws, k);
+  if (packed) check_parts(x, xs, k);
+  TORCH_CHECK_VALUE(wc.dim() == 2 && x.device() == wc.device(),
+                    "the weight is not what it was");
   const int64_t n = ws.size(0);
   Tensor y = empty(wc, with_last(lead(x), n), scalar_type(code));
   if (!y.numel()) return y;

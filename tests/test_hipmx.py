@@ -216,3 +216,15 @@ def test_another_default_device_and_type():
     assert torch.equal(q.codes, w.codes) and torch.equal(q.scales, w.scales)
     assert torch.equal(v, w.dequantize(torch.float32))
     assert torch.equal(z, y)
+
+
+def test_the_kernels_take_no_parts_of_the_host():
+    module = pytest.importorskip("_hiplm")
+    q = hipmx.quantize(torch.randn(3, 40))
+    for call in (
+        lambda: module.mx_dequantize(q.codes, q.scales, 40, 0),
+        lambda: module.mx_linear(torch.randn(2, 40), None, q.codes, q.scales,
+                                 None, 40, 0),
+    ):
+        with pytest.raises(ValueError, match="fit each other"):
+            call()

@@ -436,3 +436,44 @@ def test_linear_rings_go_round(mx, m, n, k):
     for _ in range(8):
         assert torch.equal(hipmx.linear(x, w, bias), y)
         check_linear(torch, hipmx, hipmx.linear(q, w, bias), x, w, bias)
+
+
+def test_parts_that_were_changed_in_place(mx):
+    """Codes and scales are a program's to change, but not to resize, move or
+    turn around: refused before a kernel reads them."""
+    torch, hipmx = mx
+    x = torch.randn(40, 96, device="cuda")
+    byte = torch.zeros(10000, dtype=torch.uint8, device="cuda")
+    changes = [
+        lambda t: t.resize_(1, t.shape[1]),
+        lambda t: t.resize_(t.shape[0], 1),
+        lambda t: t.resize_(t.numel()),
+        lambda t: t.t_(),
+        lambda t: t.unsqueeze_(0),
+        lambda t: t.set_(byte[:1]),
+        lambda t: t.set_(byte.as_strided(t.shape, (1, 1))),
+        lambda t: setattr(t, "data", t.cpu()),
+        lambda t: setattr(t, "data", t.int()),
+    ]
+    for change in changes:
+        for part in ("codes", "scales"):
+            q = hipmx.quantize(x)
+            change(getattr(q, part))
+            w = hipmx.quantize(x)
+            calls = [lambda: hipmx.linear(x, q), lambda: hipmx.linear(q, w)]
+            if part == "scales" or q.codes.is_cuda:
+                calls.append(q.dequantize)
+            for call in calls:
+                with pytest.raises((ValueError, RuntimeError, TypeError)):
+                    call()
+    # one that is not a multiple of 16 bytes into memory
+    q = hipmx.quantize(x)
+    codes = byte[1:1 + q.codes.numel()].view(q.codes.shape)
+    codes.copy_(q.codes)
+    q.codes.set_(codes)
+    with pytest.raises(ValueError, match="fit each other"):
+        q.dequantize()
+    # changed values are what counts
+    q = hipmx.quantize(x)
+    q.codes.zero_()
+    assert (q.dequantize() == 0).all()
