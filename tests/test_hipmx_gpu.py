@@ -477,3 +477,44 @@ def test_parts_that_were_changed_in_place(mx):
     q = hipmx.quantize(x)
     q.codes.zero_()
     assert (q.dequantize() == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dequantize_every_code_and_scale(mx, dtype):
+    """Every code under every scale byte, to each type: also what float16 and
+    bfloat16 round, lose or make an infinity of, as torch rounds it."""
+    torch, hipmx = mx
+    pair = torch.arange(256, dtype=torch.uint8)
+    codes = pair.reshape(1, 16, 16).expand(256, 16, 16).reshape(4096, 16)
+    scales = pair.repeat_interleave(16)[:, None].contiguous()
+    q = hipmx.MXFP4Tensor(codes.contiguous(), scales, 32)
+    want = torch.from_numpy(values(torch, q)).to(getattr(torch, dtype))
+    got = q.to("cuda").dequantize(getattr(torch, dtype)).cpu()
+    assert got.dtype == want.dtype
+    same = (got == want) | (got.isnan() & want.isnan())
+    assert same.all(), (got[~same][:5], want[~same][:5])
+    host = q.dequantize(getattr(torch, dtype))
+    assert ((host == want) | (host.isnan() & want.isnan())).all()
+
+
+def test_vmap_is_refused(mx):
+    torch, hipmx = mx
+    import hiplm
+
+    x = torch.randn(2, 3, 64, device="cuda")
+    ids = torch.zeros(3, 2, dtype=torch.long, device="cuda")
+    w = hipmx.quantize(x[0])
+    for call in (
+        lambda a: hipmx.quantize(a).scales,
+        lambda a: hipmx.linear(a, w),
+        lambda a: hipmx.linear(x[0], w, a[:, 0]),
+        lambda a: hiplm.token_logprobs(a, ids[:, 0]).logprobs,
+        lambda a: hiplm.token_logprobs(x[0], ids[:, 0] + (a[:, 0] > 0)
+                                       ).logprobs,
+        lambda a: hiplm.topk_distill_loss(x[0], a[:, :2], ids),
+    ):
+        with pytest.raises((TypeError, RuntimeError)):
+            torch.vmap(call)(x)
+    with pytest.raises((TypeError, RuntimeError)):
+        torch.func.grad(lambda a: hiplm.topk_distill_loss(
+            a, x[0, :, :2], ids))(x[0])
