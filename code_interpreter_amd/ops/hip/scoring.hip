@@ -577,9 +577,10 @@ struct Record {
 };
 
 // a row by a wave: the teacher's softmax over its record, and
-// T^2 sum q (ln q - ln p). The logarithms are kept in units of 1 / T, so that a
-// recorded logit of the type's lowest value overflows only where the loss does.
-// Returns (in every lane) the loss, and whether the row has a record.
+// T^2 sum q (ln q - ln p). The logarithms are kept in units of 1 / T, and their
+// sum in quarters, so that recorded logits of the type's lowest value overflow
+// only where the loss does. Returns (in every lane) the loss, and whether the
+// row has a record.
 struct RowLoss {
   float loss;
   bool there;
@@ -624,11 +625,11 @@ __device__ RowLoss distill_row(int64_t row, Record<T> rec, int64_t v,
       share = exp2_raw((z[i] - top) * c - log2_q);
       float lq = z[i] - top - log_q;
       float lp = empty ? -INFINITY : rec.x[i] - t.m - log_p;
-      if (share > 0.f) loss = fmaf(share, lq - lp, loss);
+      if (share > 0.f) loss = fmaf(share, (lq - lp) * 0.25f, loss);
     }
     if (at < e.k) e.q[row * e.k + at] = share;
   }
-  loss = wave_sum(loss) * temp;
+  loss = wave_sum(loss) * (4.f * temp);
   loss = absent ? 0.f : bad ? NAN : loss;
   if (lane == 0) {
     e.row_loss[row] = loss;

@@ -211,8 +211,8 @@ def _cpu_distill(torch, logits, teacher, ids, t, reduction):
     absent = ~there.any(-1)
     wrong = bad.any(-1)
     empty = _cpu_empty(logits) & ~wrong
-    # logarithms in units of 1 / t, so that a lowest value that is recorded
-    # overflows only where the loss does
+    # logarithms in units of 1 / t, and sums of them in quarters, so that
+    # recorded lowest values overflow only where the loss does
     x = _cpu_shifted(torch, logits, empty | absent)
     lse = torch.logsumexp(x / t, -1, keepdim=True) * t
     z = torch.where(there & ~bad, z, -math.inf)
@@ -224,12 +224,11 @@ def _cpu_distill(torch, logits, teacher, ids, t, reduction):
     mine = x.gather(-1, ids.clamp(0, v - 1)) - lse
     mine = torch.where(empty[..., None], -math.inf, mine)
     mine = torch.where(there, mine, 0.0)
-    loss = (torch.where(there, q * lq, 0.0)
-            - torch.where(there, q * mine, 0.0)).sum(-1) * t
+    loss = torch.where(there, q * ((lq - mine) * 0.25), 0.0).sum(-1) * (4 * t)
     loss = torch.where(absent, 0.0, _cpu_wrong(torch, wrong, loss))
     if reduction == "none":
         return loss
-    total = loss.sum()
+    total = loss.double().sum()
     if reduction == "mean":
         total = total / (~absent).sum().clamp(min=1)
-    return total
+    return total.float()

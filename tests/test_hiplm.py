@@ -371,3 +371,27 @@ def test_distill_of_lowest_logits_is_finite(dtype, t):
     # one rounding to the type
     check(got, grad, 2.0 ** -16 * size + 1e-30
           + torch.finfo(dtype).eps / 2 * np.abs(grad))
+
+
+def all_lowest(k):
+    """Records all of whose tokens the student gives the type's lowest value:
+    shares of 1 in sum, times the largest number that a float32 has."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(40, 400, generator=g)
+    ids = torch.stack([torch.randperm(400, generator=g)[:k]
+                       for _ in range(40)])
+    x.scatter_(1, ids, torch.finfo(torch.float32).min)
+    return x, torch.randn(40, k, generator=g), ids
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("t", [0.3, 0.9])
+@pytest.mark.parametrize("k", [1, 2, 7, 100])
+def test_distill_of_nothing_but_lowest_logits(k, t, reduction):
+    x, teacher, ids = all_lowest(k)
+    loss = hiplm.topk_distill_loss(x, teacher, ids, temperature=t,
+                                   reduction=reduction)
+    want, _, _ = oracle.distill(x.double().numpy(), teacher.double().numpy(),
+                                ids.numpy(), t, reduction)
+    assert np.isfinite(want).all()
+    check(loss, want, LOWEST * (1 + np.abs(want)))

@@ -848,3 +848,20 @@ def test_saved_tensors_through_hooks(lm):
                     assert "came back" in str(e) or "invalid gradient" in str(e)
                 else:  # a change that changed nothing
                     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("t", [0.3, 0.9])
+@pytest.mark.parametrize("k", [1, 2, 7, 100])
+def test_distill_of_nothing_but_lowest_logits(lm, k, t, reduction):
+    torch, hiplm = lm
+    import lm_oracle as oracle
+    import test_hiplm as on_host
+
+    x, teacher, ids = on_host.all_lowest(k)
+    loss = hiplm.topk_distill_loss(x.cuda(), teacher.cuda(), ids.cuda(),
+                                   temperature=t, reduction=reduction)
+    want, _, _ = oracle.distill(x.double().numpy(), teacher.double().numpy(),
+                                ids.numpy(), t, reduction)
+    assert np.isfinite(want).all()
+    near(loss, want, (on_host.LOWEST + relative(400)) * (1 + np.abs(want)))
