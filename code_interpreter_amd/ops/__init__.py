@@ -3,8 +3,9 @@
 ``_hipops`` (C extension, built in-tree by ops/build.py) provides the raw
 device API; ``hipnp`` provides DeviceArray and the numpy patches; ``hipmx``
 and ``hiplm`` provide microscaled 4-bit products and the scoring of logits
-for torch tensors (kernels: ``_hiplm``). All are import-path-flat so sandbox children can load them standalone via
-APP_OPS_DIR without pulling in the control plane.
+for torch tensors (kernels: ``_hiplm``). All are import-path-flat so sandbox
+children can load them standalone via APP_OPS_DIR without pulling in the
+control plane.
 """
 
 import os

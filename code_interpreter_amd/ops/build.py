@@ -129,8 +129,8 @@ def _compile(output: Path, sources, verbose: bool) -> None:
             cmd += ["-x", "none", str(obj)]
         if with_torch:
             # loaded after torch, which has them in the process already
-            cmd += [f"-L{_torch_dir() / 'lib'}", "-ltorch_python", "-ltorch_hip",
-                    "-ltorch_cpu", "-lc10_hip", "-lc10"]
+            cmd += [f"-L{_torch_dir() / 'lib'}", "-ltorch_python",
+                    "-ltorch_hip", "-ltorch_cpu", "-lc10_hip", "-lc10"]
         _run(cmd, verbose)
 
 

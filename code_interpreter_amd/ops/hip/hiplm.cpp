@@ -426,13 +426,6 @@ bool needs_grad(const Tensor& t) {
   return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t);
 }
 
-PyObject* py_is_available(PyObject*, PyObject*) {
-  int count = 0;
-  hipError_t e = hipGetDeviceCount(&count);
-  if (e != hipSuccess || count <= 0) Py_RETURN_FALSE;
-  Py_RETURN_TRUE;
-}
-
 PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(args, n, 2);
@@ -532,7 +525,8 @@ PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
                             how)[0];
     } else {
       at::NoGradGuard no_grad;
-      loss = distill(logits, teacher, ids, code, teacher_code, inv_t, how).loss;
+      loss = distill(logits, teacher, ids, code, teacher_code, inv_t, how)
+                 .loss;
     }
   }
   return THPVariable_Wrap(loss);
@@ -543,7 +537,6 @@ PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // a dtype is 0 float32, 1 bfloat16, 2 float16
 PyMethodDef methods[] = {
-    {"is_available", py_is_available, METH_NOARGS, "GPU present?"},
     {"mx_quantize", FAST(py_mx_quantize),
      "mx_quantize(x, dtype) -> (codes, scales)"},
     {"mx_dequantize", FAST(py_mx_dequantize),

@@ -87,7 +87,8 @@ constexpr int kPrepareThreads = 256;
 // A block that quantises takes kPrepareSteps steps of kPrepareRows rows: 8192
 // x 8192 bf16 in 42 us, 46 with 1 step, 45 with 4.
 constexpr int kPrepareSteps = 2, kPrepareRows = 32 / kPrepareSteps;
-constexpr int kLayRows = kPrepareThreads, kLaySteps = 4;  // of one that does not
+// of one that does not
+constexpr int kLayRows = kPrepareThreads, kLaySteps = 4;
 
 __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
                                                uint2* to, int64_t rows,
@@ -118,8 +119,8 @@ __device__ __forceinline__ void lay_out_scales(const uint8_t* from,
 }
 
 // blocks [0, x_blocks): x to codes and laid out scales, or (packed) its
-// scales laid out; the others: the weight's scales laid out. A quantising
-// block takes 32 rows of one step, so that its scales are 256 bytes in order.
+// scales laid out; the others: the weight's scales laid out. The scales of a
+// quantising block's rows are neighbours, 128 bytes for each of its two steps.
 template <LmType T, bool kPacked>
 __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
     const char* __restrict__ x, int64_t stride,
@@ -173,12 +174,12 @@ __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
 // index ^ (r / 2 & 7), so that 16 lanes that read the same unit of 16 rows
 // touch all of the 64 banks once.
 //
-// 8192^3 in 260 us on random codes, 4.2 PFLOP/s; the instructions alone reach
-// 5.2 there, since the power limit lowers the clock (on zeros 8.7, and this
-// kernel 4.8). The matrix units are busy half of the cycles: a wave's 128 x
-// 128 results take all of the accumulators, so that a tile's results go out
-// (28 us of writing in all) while no products run, and a block's loads start
-// anew.
+// 8192^3 in 260 us on random codes at the best clock, 4.2 PFLOP/s, and up to
+// 315 after long work; the instructions alone reach 5.2 there, since the power
+// limit lowers the clock (on zeros 8.7, and this kernel 4.8). The matrix units
+// are busy half of the cycles: a wave's 128 x 128 results take all of the
+// accumulators, so that a tile's results go out while no products run, and a
+// block's loads start anew. Without the stores the kernel takes 10 us less.
 //
 // A step is 4 instructions deep in k. While the matrix units work on one of
 // them the next one's operands are read; the last one's time covers the
@@ -958,7 +959,10 @@ void run_tiles(const void* x, int64_t stride, const uint8_t* xc,
   // the small tiles' scales are addressed in 31 bits
   const bool far = std::max(m, n) * steps * 8 >= (int64_t)1 << 31;
   // A tile of 256 x 256 is a compute unit's alone, so that its start and end
-  // are not hidden: it wants a long k, and not a second round for a few:
+  // are not hidden: it wants a long k, and not a second round for a few. The
+  // rule goes by k and the tiles' number alone, and near its borders takes up
+  // to a fifth more than 128 x 128 would: most for tokens that fill little
+  // more than half of a tile, as 164. 256 x 256 and 128 x 128:
   // 8192 x 8192 x  512 56.1, 54.6, x 1024 77.1, 75.3, x 1536 91.5, 93.5
   // 4096 x 4096 x  512 21.0, 20.7, x 1024 24.8, 25.2, x 1536 29.9, 30.8
   //  164 x 43710 x 512 21.9, 17.2, x 1024 25.3, 21.3, x 1536 28.3, 24.9

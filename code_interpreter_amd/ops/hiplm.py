@@ -118,8 +118,10 @@ def topk_distill_loss(logits, teacher_logits, teacher_tokens, *,
     twice.
 
     reduction: "mean" (over rows with a record; 0 if there are none), "sum"
-    or "none" ([...]); rows' losses and the result are float32. An entry that the student masks
-    (-inf) gives an infinite loss, with the finite gradient T (p - q) / rows.
+    or "none" ([...]); rows' losses and the result are float32. An entry that
+    the student masks (-inf) gives an infinite loss, with the finite gradient
+    T (p - q) / rows; a share q below the smallest normal float32 may count
+    as 0.
     A token outside of [0, v) but -1, or a NaN or +inf on either side, gives
     NaN.
     """

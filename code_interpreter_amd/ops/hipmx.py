@@ -145,9 +145,9 @@ def linear(input, weight: MXFP4Tensor, bias=None, *, dtype=None):
     input: a tensor [..., k] (float32, bfloat16, float16), which is quantised
     as by ``quantize`` on the way in and gives the result its type, or an
     MXFP4Tensor, with the result's type in ``dtype`` (bfloat16 if not given).
-    weight: [n, k], k below 2^24. bias: [n], of the result's type. Sums are float32; the
-    result is rounded once. There is no backward: tensors that require a
-    gradient are refused while gradients are enabled.
+    weight: [n, k], k below 2^24. bias: [n], of the result's type. Sums are
+    float32; the result is rounded once. There is no backward: tensors that
+    require a gradient are refused while gradients are enabled.
     """
     torch = hiptorch.lm_torch()
     if not isinstance(weight, MXFP4Tensor):

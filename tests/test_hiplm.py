@@ -395,3 +395,26 @@ def test_distill_of_nothing_but_lowest_logits(k, t, reduction):
                                 ids.numpy(), t, reduction)
     assert np.isfinite(want).all()
     check(loss, want, LOWEST * (1 + np.abs(want)))
+
+
+def test_second_derivatives_of_host_tensors():
+    """A gradient penalty, against torch's own operations in 64 bits."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(3, 20, generator=g)
+    teacher, ids = torch.randn(3, 4, generator=g), torch.arange(12).view(3, 4)
+
+    def penalty(loss, z):
+        (grad,) = torch.autograd.grad(loss, [z], create_graph=True)
+        return torch.autograd.grad(loss + grad.pow(2).sum(), [z])[0]
+
+    z = x.clone().requires_grad_(True)
+    r = hiplm.token_logprobs(z, ids[:, 0])
+    got = penalty(r.logprobs.sum() + r.entropy.sum()
+                  + hiplm.topk_distill_loss(z, teacher, ids), z)
+    z = x.double().requires_grad_(True)
+    lp, lq = torch.log_softmax(z, -1), torch.log_softmax(teacher.double(), -1)
+    at = lp.gather(-1, ids)
+    want = penalty(at[:, 0].sum() - (lp.exp() * lp).sum()
+                   + (lq.exp() * (lq - at)).sum() / 3, z)
+    # sums of some ten terms of size 1 to 10, a few roundings each
+    torch.testing.assert_close(got.double(), want, rtol=2e-5, atol=2e-5)
